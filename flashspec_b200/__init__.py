@@ -13,7 +13,8 @@ include/flashspec_b200.h).  There is no CPU or Triton fallback.
 
 from ._build import build
 from .attention import (BACKENDS, fused_dequant_attention_cuda, get_backend, merge_partials,
-                        paged_quant_attention_cuda, register_backend, reset_workspaces)
+                        paged_quant_attention_cuda, paged_quant_attention_weights_cuda, register_backend,
+                        reset_workspaces)
 from .paged import PagedKVAllocator, PagedKVCache
 from .paged import paged_cache_symmetric
 from .quant import (QuantizedTensor, SymQuantizedTensor, build_compression_stats, dequantize_int8_per_block,
@@ -34,6 +35,7 @@ __all__ = [
     "get_backend",
     "merge_partials",
     "paged_quant_attention_cuda",
+    "paged_quant_attention_weights_cuda",
     "quantize_int8_per_block",
     "register_backend",
     "SymQuantizedTensor",

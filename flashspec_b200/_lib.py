@@ -165,6 +165,9 @@ SIGNATURES = {
     "fs_fused_decode": (C.c_int, [C.POINTER(FsDecodeArgs), C.c_void_p]),
     "fs_paged_decode": (C.c_int, [C.POINTER(FsDecodeArgs), C.c_void_p]),
     "fs_paged_decode_noalloc": (C.c_int, [C.POINTER(FsDecodeArgs), C.c_void_p]),
+    "fs_paged_decode_weights_workspace_size": (C.c_int, [C.POINTER(FsDecodeArgs), C.POINTER(C.c_size_t),
+                                                         C.POINTER(C.c_int32)]),
+    "fs_paged_decode_weights": (C.c_int, [C.POINTER(FsDecodeArgs), C.c_void_p, C.c_void_p]),
     "fs_merge_partials": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_int64, C.c_void_p,
                                     C.c_int32, C.c_void_p]),
     "fs_quantize_blocks": (C.c_int, [C.POINTER(FsQuantizeArgs), C.c_void_p]),

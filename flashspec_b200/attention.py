@@ -26,6 +26,7 @@ PAGE_TOKENS = 16  # tokens per kernel step (one page / quant block)
 NUM_WARPS = 4
 _workspaces: Dict[Tuple[int, int], torch.Tensor] = {}
 _tickets: Dict[Tuple[int, int], torch.Tensor] = {}
+_weight_tickets: Dict[Tuple[int, int], torch.Tensor] = {}
 _plans: Dict[tuple, Tuple[int, int]] = {}
 # environment knobs the library's plan reads (decode.cu): part of the plan cache key
 _PLAN_KNOBS = ("FLASHSPEC_DECODE_KERNEL", "FLASHSPEC_KERNEL_SHAPE", "FLASHSPEC_NUM_WARPS", "FLASHSPEC_TIER_SKEW",
@@ -54,11 +55,25 @@ def _ticket_buffer(device: torch.device, stream: int, count: int) -> torch.Tenso
     return t
 
 
+def _weights_tickets(device: torch.device, stream: int, count: int) -> torch.Tensor:
+    """Merge counters of a weighted decode: kept per (device, stream) for eager calls; a
+    captured call gets its own, zeroed by the graph, so that replays share nothing with
+    other graphs or with eager calls."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(count, dtype=torch.int32, device=device)
+    key = (device.index, stream)
+    t = _weight_tickets.get(key)
+    if t is None or t.numel() < count:
+        t = _weight_tickets[key] = torch.zeros(max(count, 4096), dtype=torch.int32, device=device)
+    return t
+
+
 def reset_workspaces() -> None:
     """Drop cached workspaces and tickets (needed after a call reported FS_DEV_TIMEOUT,
     which can leave tickets non-zero)."""
     _workspaces.clear()
     _tickets.clear()
+    _weight_tickets.clear()
 
 
 def _env_splits() -> int:
@@ -95,12 +110,14 @@ def _i64(t: torch.Tensor) -> torch.Tensor:
     return t if t.dtype == torch.int64 and t.is_contiguous() else t.to(torch.int64).contiguous()
 
 
-def _run(entry: str, args: _lib.FsDecodeArgs, device: torch.device, splits_hint: int, xargs=None) -> int:
+def _run(entry: str, args: _lib.FsDecodeArgs, device: torch.device, splits_hint: int, xargs=None,
+         weights: Optional[torch.Tensor] = None) -> int:
     """Plan (cached), workspace and launch of one decode call; ``xargs`` (FsExchangeArgs)
-    selects fs_paged_decode_exchange and its own plan."""
+    selects fs_paged_decode_exchange and its own plan, ``weights`` fs_paged_decode_weights
+    and its."""
     if torch.cuda.current_device() != device.index:
         with torch.cuda.device(device):
-            return _run(entry, args, device, splits_hint, xargs)
+            return _run(entry, args, device, splits_hint, xargs, weights)
     lib = _lib.load()
     stream = stream_of(device)
     args.num_splits = splits_hint
@@ -114,13 +131,23 @@ def _run(entry: str, args: _lib.FsDecodeArgs, device: torch.device, splits_hint:
         nbytes = C.c_size_t(0)
         splits = C.c_int32(0)
         size_fn = lib.fs_paged_decode_exchange_workspace_size if xargs is not None else lib.fs_decode_workspace_size
+        if weights is not None:
+            size_fn = lib.fs_paged_decode_weights_workspace_size
         _lib.check(size_fn(C.byref(args), C.byref(nbytes), C.byref(splits)), entry)
         plan = _plans[key] = (nbytes.value, splits.value)
         if len(_plans) > 256:
             _plans.pop(next(iter(_plans)))
     nbytes = C.c_size_t(plan[0])
     splits = C.c_int32(plan[1])
-    if nbytes.value:
+    if weights is not None:
+        # scores can be large: scratch of this call (in a capture, of the graph's own pool)
+        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=device)
+        args.workspace = ws.data_ptr()
+        args.workspace_bytes = ws.numel()
+        tk = _weights_tickets(device, stream, args.batch * args.kv_heads)
+        args.tickets = tk.data_ptr()
+        args.ticket_count = tk.numel()
+    elif nbytes.value:
         ws = _workspace(device, stream, nbytes.value)
         args.workspace = ws.data_ptr()
         args.workspace_bytes = ws.numel()
@@ -129,6 +156,8 @@ def _run(entry: str, args: _lib.FsDecodeArgs, device: torch.device, splits_hint:
         args.ticket_count = tk.numel()
     if xargs is not None:
         _lib.check(getattr(lib, entry)(C.byref(args), C.byref(xargs), stream), entry)
+    elif weights is not None:
+        _lib.check(lib.fs_paged_decode_weights(C.byref(args), weights.data_ptr(), stream), entry)
     else:
         _lib.check(getattr(lib, entry)(C.byref(args), stream), entry)
     return splits.value
@@ -212,25 +241,8 @@ def fused_dequant_attention_cuda(q: torch.Tensor, k_quant, v_quant, lengths: Opt
                                         block_n=int(kq.block_size), num_warps=NUM_WARPS)
 
 
-def paged_quant_attention_cuda(q: torch.Tensor, cache, return_stats: bool = False, *,
-                               num_splits: Optional[int] = None, page_range: Optional[Tuple[int, int]] = None,
-                               partial_out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
-                               device_status: Optional[torch.Tensor] = None, exchange=None):
-    """Paged INT8 KV decode attention (backend ``cuda_paged``).
-
-    ``cache`` is a PagedKVCache (this package's or the reference's): pool
-    [P, Hkv, page / qb, qb, D] int8 + fp32/int16 qparams per quant block of qb tokens
-    (the page a multiple of qb), block_table int64 [B, cols] (-1 = unallocated),
-    lengths int64 [B], max_seq_len; q fp16 or bf16.  Validation follows
-    _validate_triton_paged_inputs (triton_paged.py:302-335).
-
-    Extensions used by sequence sharding: ``page_range=(lo, hi)`` restricts every
-    request to logical pages [lo, hi); ``partial_out=(O fp32 [B,Hq,D], LSE fp32
-    [B,Hq])`` receives the normalised partial result and its log-sum-exp instead
-    of the fp16 output (None is returned then); ``exchange=(FsExchangeArgs, out)``
-    runs the window's decode with the fused exchange epilogue
-    (``fs_paged_decode_exchange``): every rank's rows are merged into ``out`` (fp16 or
-    fp32 [B, Hq, D]), which is returned."""
+def _validate_paged(q: torch.Tensor, cache) -> Tuple[int, int]:
+    """_validate_triton_paged_inputs (triton_paged.py:302-335); returns (kv heads, head dim)."""
     _validate_query(q, "paged")
     kq, vq = cache.k_quant, cache.v_quant
     hkv = int(kq.original_shape[1])
@@ -252,6 +264,30 @@ def paged_quant_attention_cuda(q: torch.Tensor, cache, return_stats: bool = Fals
         raise RuntimeError("q and the cache's quantized K/V must be on the same CUDA device")
     if cache.block_table.device != q.device or cache.lengths.device != q.device:
         raise RuntimeError("block_table and lengths must be on q's CUDA device")
+    return hkv, d
+
+
+def paged_quant_attention_cuda(q: torch.Tensor, cache, return_stats: bool = False, *,
+                               num_splits: Optional[int] = None, page_range: Optional[Tuple[int, int]] = None,
+                               partial_out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
+                               device_status: Optional[torch.Tensor] = None, exchange=None):
+    """Paged INT8 KV decode attention (backend ``cuda_paged``).
+
+    ``cache`` is a PagedKVCache (this package's or the reference's): pool
+    [P, Hkv, page / qb, qb, D] int8 + fp32/int16 qparams per quant block of qb tokens
+    (the page a multiple of qb), block_table int64 [B, cols] (-1 = unallocated),
+    lengths int64 [B], max_seq_len; q fp16 or bf16.  Validation follows
+    _validate_triton_paged_inputs (triton_paged.py:302-335).
+
+    Extensions used by sequence sharding: ``page_range=(lo, hi)`` restricts every
+    request to logical pages [lo, hi); ``partial_out=(O fp32 [B,Hq,D], LSE fp32
+    [B,Hq])`` receives the normalised partial result and its log-sum-exp instead
+    of the fp16 output (None is returned then); ``exchange=(FsExchangeArgs, out)``
+    runs the window's decode with the fused exchange epilogue
+    (``fs_paged_decode_exchange``): every rank's rows are merged into ``out`` (fp16 or
+    fp32 [B, Hq, D]), which is returned."""
+    hkv, d = _validate_paged(q, cache)
+    kq, vq = cache.k_quant, cache.v_quant
     kq, vq = _contig_quant(kq), _contig_quant(vq)
     table = _i64(cache.block_table)
     lengths = _i64(cache.lengths)
@@ -292,6 +328,43 @@ def paged_quant_attention_cuda(q: torch.Tensor, cache, return_stats: bool = Fals
                                     physical_blocks=float(cache.block_table.ge(0).sum().item()),
                                     num_splits=splits, block_n=int(kq.block_size), num_warps=NUM_WARPS)
     return out, stats
+
+
+def paged_quant_attention_weights_cuda(q: torch.Tensor, cache, weights: torch.Tensor, return_stats: bool = False, *,
+                                       num_splits: Optional[int] = None,
+                                       device_status: Optional[torch.Tensor] = None):
+    """``paged_quant_attention_cuda`` that also adds up the attention every cached token
+    receives: in place, weights[page, kv head, t] grows by the softmax weights that the kv
+    head's query heads put on the token in row t of the page.
+
+    ``weights`` is a contiguous fp32 tensor [P, Hkv, page] beside the cache's pool (zeros to
+    begin with; rows of tokens that are not live, and pages outside the table, stay as they
+    are).  ``evict_tokens_cuda`` keeps the tokens with the largest sums.  A page of one
+    request gets exactly one addition a call, so its sums are reproducible; pages that
+    requests share add up as well, in varying order.  The scores take a workspace of 4 bytes
+    a query head and token."""
+    hkv, _ = _validate_paged(q, cache)
+    num_pages, page = int(cache.k_quant.values.shape[0]), int(cache.block_size)
+    _check_weights(weights, (num_pages, hkv, page), q.device, "weights")
+    kq, vq = _contig_quant(cache.k_quant), _contig_quant(cache.v_quant)
+    qc, table, lengths = q.contiguous(), _i64(cache.block_table), _i64(cache.lengths)
+    out = torch.empty_like(qc)
+    a = _decode_args(_lib.FS_LAYOUT_PAGED, qc, kq, vq, out, lengths, table, num_pages, int(cache.max_seq_len), hkv,
+                     device_status, page_size=page)
+    splits = _run("fs_paged_decode_weights", a, q.device, num_splits or _env_splits(), weights=weights)
+    if not return_stats:
+        return out
+    dense = 2 * q.shape[0] * hkv * int(cache.max_seq_len) * q.shape[2] * qc.element_size()
+    return out, build_compression_stats(dense, cache.estimated_bytes(), materializes_dense_kv=False,
+                                        physical_blocks=float(cache.block_table.ge(0).sum().item()),
+                                        num_splits=splits, block_n=int(kq.block_size), num_warps=NUM_WARPS)
+
+
+def _check_weights(w: torch.Tensor, shape: Tuple[int, ...], device: torch.device, name: str) -> None:
+    if w.device != device:
+        raise RuntimeError(f"{name} must be on the cache's CUDA device")
+    if tuple(w.shape) != shape or w.dtype != torch.float32 or not w.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous fp32 tensor [pages, kv heads, page] beside the pool")
 
 
 def merge_partials(o_parts: torch.Tensor, lse_parts: torch.Tensor, out_dtype: torch.dtype = torch.float16):

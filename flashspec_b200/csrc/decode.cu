@@ -40,6 +40,7 @@
 #include "common.h"
 #include "generic.h"
 #include "ptx.cuh"
+#include "weights.h"
 #include "xwords.cuh"
 
 namespace fsb {
@@ -94,6 +95,10 @@ struct DecodeParams {
   int64_t xslot;
   int64_t xtimeout_ns;
   int xworld, xrank, xout_dtype;
+  // decode with accumulated weights (the kernels' kWts instantiations only)
+  float* scores;        // [B, Hq, score_stride] scores in the log2 domain
+  float* lse_out;       // [B, Hq] natural-log LSE beside `out`
+  int64_t score_stride;
 };
 
 // Shared-memory plan of one CTA: a ring of kNS page stages (K 2 KB + V 2 KB, 1024-byte
@@ -240,8 +245,16 @@ struct StageOffsets {
 // head dims [32c, 32c+32): word w covers dims 32c+4w .. 32c+4w+3, and k-step j uses
 // words 2j (logical k 4c..4c+3) and 2j+1 (logical k 16+4c..).  q16sum = sum of q16 over
 // the row (exact), used to apply the zero point once per page.
+// kWts (the weights themselves are results, in fp32): 24-bit fixed point in three bytes
+// (|q| <= 8355000, rounding error max|q| 2^-24), so a third MMA per step; with 16 bits a
+// weight would be off by about 3e-5 of itself for normal q and K.
+template <bool kWts>
 struct QueryFrag {
-  uint32_t hi[8], lo[8];
+  static constexpr int kBytes = kWts ? 3 : 2;  // signed bytes of the fixed point, most significant first
+  // the largest fixed-point value: 127 in every byte (127 * 2^16 + 127 * 2^8 + 127 is left a
+  // margin, since at 24 bits amax * (kTop / amax) can round to kTop + 1 and carry)
+  static constexpr float kTop = kWts ? 8355000.0f : 32639.0f;
+  uint32_t hi[8], lo[8], lo2[kWts ? 8 : 1];
   int q16sum;
   float qscale;
   __device__ __forceinline__ void load(const DecodeParams& p, int b, int h, int lane) {
@@ -270,28 +283,34 @@ struct QueryFrag {
     }
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    const float inv = amax > 0.f ? 32639.0f / amax : 0.f;
-    qscale = amax > 0.f ? amax / 32639.0f : 0.f;
+    const float inv = amax > 0.f ? kTop / amax : 0.f;
+    qscale = amax > 0.f ? amax / kTop : 0.f;
     int sum = 0;
 #pragma unroll
     for (int w = 0; w < 8; ++w) {
-      uint32_t hw = 0u, lw = 0u;
+      uint32_t hw = 0u, lw = 0u, lw2 = 0u;
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const float2 f2 = __half22float2(*reinterpret_cast<const __half2*>(&raw[2 * w + k]));
         const float v2[2] = {f2.x, f2.y};
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int q16 = __float2int_rn(v2[e] * inv);
+          int q16 = __float2int_rn(v2[e] * inv);
+          sum += q16;
+          if (kWts) {
+            const int up = (q16 + 128) >> 8;
+            lw2 |= (uint32_t)((q16 - (up << 8)) & 0xff) << (8 * (2 * k + e));
+            q16 = up;
+          }
           const int qh = (q16 + 128) >> 8;
           const int ql = q16 - (qh << 8);
-          sum += q16;
           hw |= (uint32_t)(qh & 0xff) << (8 * (2 * k + e));
           lw |= (uint32_t)(ql & 0xff) << (8 * (2 * k + e));
         }
       }
       hi[w] = hw;
       lo[w] = lw;
+      if (kWts) lo2[w] = lw2;
     }
     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
@@ -338,15 +357,16 @@ struct WarpState {
 
 // Consumer side: load stage `sbase`, release it on `empty_bar`, then fold the page into
 // the warp state.  pos0 = first token position of the page, len_eff = tokens that count.
-// kMode 1 stops after the loads (profiling).
-template <int kMode>
+// kMode 1 stops after the loads (profiling).  kWts: lanes of a query row g < G also store
+// the row's 16 scores (masked ones -inf) at srow (the row's page slot in the score array).
+template <int kMode, bool kWts = false>
 __device__ __forceinline__ void consume_page(uint32_t sbase, const StageOffsets& off, uint32_t empty_bar, int lane,
-                                             const StageInfo& si, const QueryFrag& qf, float qk_scale_log2,
-                                             int pos0, int len_eff, WarpState& ws) {
+                                             const StageInfo& si, const QueryFrag<kWts>& qf, float qk_scale_log2,
+                                             int pos0, int len_eff, WarpState& ws, float* srow = nullptr) {
   const int c = lane & 3;
   // ---- S = Q K^T on the int8 tensor cores, straight from the stored bytes s = u - 128:
   // sum_d q16 * s = 256 * (hi . s) + (lo . s); u - zp = s + (128 - zp) is applied per page
-  int shi[2][4], slo[2][4];
+  int shi[2][4], slo[2][4], slo2[kWts ? 2 : 1][4];
   {
     uint4 kr[2][2];
 #pragma unroll
@@ -356,7 +376,10 @@ __device__ __forceinline__ void consume_page(uint32_t sbase, const StageOffsets&
 #pragma unroll
     for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) shi[nt][k] = slo[nt][k] = 0;
+      for (int k = 0; k < 4; ++k) {
+        shi[nt][k] = slo[nt][k] = 0;
+        if (kWts) slo2[nt][k] = 0;
+      }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
 #pragma unroll
@@ -366,6 +389,7 @@ __device__ __forceinline__ void consume_page(uint32_t sbase, const StageOffsets&
         const uint32_t b1 = (j & 1) ? kv.w : kv.y;
         mma_16832_s8(shi[nt], qf.hi[2 * j], 0u, qf.hi[2 * j + 1], 0u, b0, b1);
         mma_16832_s8(slo[nt], qf.lo[2 * j], 0u, qf.lo[2 * j + 1], 0u, b0, b1);
+        if (kWts) mma_16832_s8(slo2[nt], qf.lo2[2 * j], 0u, qf.lo2[2 * j + 1], 0u, b0, b1);
       }
     }
   }
@@ -379,7 +403,7 @@ __device__ __forceinline__ void consume_page(uint32_t sbase, const StageOffsets&
     return;
   }
   const float f = si.ks * qf.qscale * qk_scale_log2;
-  const int zc = (128 - (int)si.kz) * qf.q16sum;
+  const int zc = kWts ? 0 : (128 - (int)si.kz) * qf.q16sum;
   // per-token scales of this thread's tokens 2c, 2c+1, 8+2c, 9+2c (symmetric format)
   float fk[4] = {f, f, f, f}, vk[4] = {si.vs, si.vs, si.vs, si.vs};
   if (si.tok != 0u) {
@@ -395,15 +419,27 @@ __device__ __forceinline__ void consume_page(uint32_t sbase, const StageOffsets&
     vk[3] = v89.y;
   }
   float t[4];
-  t[0] = (float)((shi[0][0] << 8) + slo[0][0] + zc) * fk[0];  // token 2c
-  t[1] = (float)((shi[0][1] << 8) + slo[0][1] + zc) * fk[1];  // token 2c+1
-  t[2] = (float)((shi[1][0] << 8) + slo[1][0] + zc) * fk[2];  // token 8+2c
-  t[3] = (float)((shi[1][1] << 8) + slo[1][1] + zc) * fk[3];  // token 9+2c
+  if (kWts) {  // 24 bits of q: the three sums pass 32 bits together, so the top one joins in fp32
+    const float zf = (float)(128 - (int)si.kz) * (float)qf.q16sum;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)  // tokens 2c, 2c+1, 8+2c, 9+2c
+      t[k] = (fmaf(65536.f, (float)shi[k >> 1][k & 1], (float)((slo[k >> 1][k & 1] << 8) + slo2[k >> 1][k & 1])) + zf) *
+             fk[k];
+  } else {
+    t[0] = (float)((shi[0][0] << 8) + slo[0][0] + zc) * fk[0];  // token 2c
+    t[1] = (float)((shi[0][1] << 8) + slo[0][1] + zc) * fk[1];  // token 2c+1
+    t[2] = (float)((shi[1][0] << 8) + slo[1][0] + zc) * fk[2];  // token 8+2c
+    t[3] = (float)((shi[1][1] << 8) + slo[1][1] + zc) * fk[3];  // token 9+2c
+  }
   if (pos0 + kPage > len_eff) {
     if (pos0 + 2 * c >= len_eff) t[0] = -INFINITY;
     if (pos0 + 2 * c + 1 >= len_eff) t[1] = -INFINITY;
     if (pos0 + 8 + 2 * c >= len_eff) t[2] = -INFINITY;
     if (pos0 + 9 + 2 * c >= len_eff) t[3] = -INFINITY;
+  }
+  if (kWts && srow != nullptr) {
+    *reinterpret_cast<float2*>(srow + 2 * c) = make_float2(t[0], t[1]);
+    *reinterpret_cast<float2*>(srow + 8 + 2 * c) = make_float2(t[2], t[3]);
   }
   float mx = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
   mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
@@ -447,9 +483,14 @@ __device__ __forceinline__ void consume_page(uint32_t sbase, const StageOffsets&
   }
 }
 
-// Writes one normalised output value: fp16 `out`, or (O, LSE) into the shard outputs.
+// Writes one normalised output value: fp16 `out`, or (O, LSE) into the shard outputs;
+// kWts: `out` and the row's LSE.
+template <bool kWts = false>
 __device__ __forceinline__ void write_final(const DecodeParams& p, size_t row, int d, float o, float lse) {
-  if (p.shard_o != nullptr) {
+  if (kWts) {
+    p.out[row * kD + d] = __float2half_rn(o);
+    if (d == 0) p.lse_out[row] = lse;
+  } else if (p.shard_o != nullptr) {
     p.shard_o[row * kD + d] = o;
     if (d == 0) p.shard_lse[row] = lse;
   } else {
@@ -571,7 +612,7 @@ __device__ __forceinline__ void exchange_pair(const DecodeParams& p, int b, int 
 // qparam copies.  kMode is a profiling aid: 0 = normal; 1 = consumers read the stage and
 // release it but skip the math; 2 = consumers only wait and release (data movement).
 // ==================================================================================
-template <bool kPaged, int kW, int kNS, int kMinBlocks, int kMode>
+template <bool kPaged, int kW, int kNS, int kMinBlocks, int kMode, bool kWts = false>
 __global__ void __launch_bounds__((kW + 1) * 32, kMinBlocks)
     decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
                   const DecodeParams p) {
@@ -668,7 +709,7 @@ __global__ void __launch_bounds__((kW + 1) * 32, kMinBlocks)
     }
   } else {
     // ============================ consumer warps ===============================
-    QueryFrag qf;
+    QueryFrag<kWts> qf;
     qf.load(p, b, h, lane);
     const StageOffsets off(lane);
     for (int i = warp; i < n; i += kW) {
@@ -684,8 +725,11 @@ __global__ void __launch_bounds__((kW + 1) * 32, kMinBlocks)
         if (lane == 0) mbar_arrive(empty_s + 8 * st);
         continue;
       }
-      consume_page<kMode>(base_s + st * kStageBytes, off, empty_s + 8 * st, lane, si, qf, p.qk_scale_log2,
-                          (p0 + i) * kPage, len_eff, ws);
+      float* srow = nullptr;
+      if (kWts && g < p.G)
+        srow = p.scores + ((size_t)b * p.Hq + (size_t)h * p.G + g) * p.score_stride + (size_t)(p0 + i) * kPage;
+      consume_page<kMode, kWts>(base_s + st * kStageBytes, off, empty_s + 8 * st, lane, si, qf, p.qk_scale_log2,
+                                (p0 + i) * kPage, len_eff, ws, srow);
     }
     ws.l_run += __shfl_xor_sync(0xffffffffu, ws.l_run, 1);
     ws.l_run += __shfl_xor_sync(0xffffffffu, ws.l_run, 2);
@@ -767,10 +811,10 @@ __global__ void __launch_bounds__((kW + 1) * 32, kMinBlocks)
       *reinterpret_cast<float4*>(xo + idx) = o;
       if (d == 0) xl[qg] = lse;
     } else if (S == 1) {
-      write_final(p, row, d, o.x, lse);
-      write_final(p, row, d + 1, o.y, lse);
-      write_final(p, row, d + 2, o.z, lse);
-      write_final(p, row, d + 3, o.w, lse);
+      write_final<kWts>(p, row, d, o.x, lse);
+      write_final<kWts>(p, row, d + 1, o.y, lse);
+      write_final<kWts>(p, row, d + 2, o.z, lse);
+      write_final<kWts>(p, row, d + 3, o.w, lse);
     } else {
       const size_t prow = ((size_t)bh * S + split) * p.G + qg;
       *reinterpret_cast<float4*>(p.part_o + prow * kD + d) = o;
@@ -904,10 +948,10 @@ __global__ void __launch_bounds__((kW + 1) * 32, kMinBlocks)
         *reinterpret_cast<float4*>(xo + 4 * u4) = o;
         if (d == 0) xl[qg] = lse_out;
       } else {
-        write_final(p, row, d, o.x, lse_out);
-        write_final(p, row, d + 1, o.y, lse_out);
-        write_final(p, row, d + 2, o.z, lse_out);
-        write_final(p, row, d + 3, o.w, lse_out);
+        write_final<kWts>(p, row, d, o.x, lse_out);
+        write_final<kWts>(p, row, d + 1, o.y, lse_out);
+        write_final<kWts>(p, row, d + 2, o.z, lse_out);
+        write_final<kWts>(p, row, d + 3, o.w, lse_out);
       }
     }
   }
@@ -936,7 +980,7 @@ __global__ void __launch_bounds__((kW + 1) * 32, kMinBlocks)
       xo[idx] = o;
       if (d == 0) xl[qg] = lse_out;
     } else {
-      write_final(p, (size_t)b * p.Hq + (size_t)h * p.G + qg, d, o, lse_out);
+      write_final<kWts>(p, (size_t)b * p.Hq + (size_t)h * p.G + qg, d, o, lse_out);
     }
   }
   if (tid == 0) p.counters[bh] = 0u;  // leave the ticket clean for the next call
@@ -1047,9 +1091,10 @@ __device__ __forceinline__ Shares make_shares(const DecodeParams& p, int T) {
 // with the first four partial rows, then each lane accumulates head dims 4*lane .. +3
 // four rows at a time.  (Inlined: as an out-of-line call it cost the streaming loop
 // around it 3-5% on B200.)
+template <bool kWts>
 __device__ __forceinline__ void merge_pair(const float* part_o, const float* part_lse, __half* out, float* shard_o,
                                         float* shard_lse, int G, int64_t k0, int64_t k1, bool k0_first,
-                                        size_t row0, int lane) {
+                                        size_t row0, int lane, float* lse_row) {
   const int n = (int)(k1 - k0 + 1);
   auto slot = [&](int j) -> size_t { return ((size_t)(k0 + j) * 2 + ((j == 0 && !k0_first) ? 1 : 0)) * G; };
   const float4 zero4 = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -1094,7 +1139,8 @@ __device__ __forceinline__ void merge_pair(const float* part_o, const float* par
     const float lse_out = W > 0.f ? M + logf(W) : -INFINITY;
     const size_t r = row0 + qg;
     const int d = 4 * lane;
-    if (shard_o != nullptr) {
+    if (kWts && lane == 0) lse_row[r] = lse_out;
+    if (!kWts && shard_o != nullptr) {
       *reinterpret_cast<float4*>(shard_o + r * kD + d) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
       if (lane == 0) shard_lse[r] = lse_out;
     } else {
@@ -1137,7 +1183,7 @@ __device__ __forceinline__ void trace_mark(const DecodeParams& p, int nwarps, in
     p.trace[((size_t)blockIdx.x * nwarps + (threadIdx.x >> 5)) * 8 + k] = k >= 5 ? v : globaltimer_ns();
 }
 
-template <bool kPaged, int kW, int kNS, int kMaxRegs, bool kTrace>
+template <bool kPaged, int kW, int kNS, int kMaxRegs, bool kTrace, bool kWts = false>
 __global__ void __maxnreg__(kMaxRegs)
     decode_balanced_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
                            const DecodeParams p) {
@@ -1274,7 +1320,7 @@ __global__ void __maxnreg__(kMaxRegs)
       const int r = pr / Hkv, h = pr % Hkv;
       if (pre[r + 1] != pre[r]) continue;
       for (int idx = lane; idx < p.G * kD; idx += 32)
-        write_final(p, (size_t)r * p.Hq + (size_t)h * p.G + (idx >> 7), idx & (kD - 1), 0.f, -INFINITY);
+        write_final<kWts>(p, (size_t)r * p.Hq + (size_t)h * p.G + (idx >> 7), idx & (kD - 1), 0.f, -INFINITY);
     }
   }
   if (T == 0) return;
@@ -1282,7 +1328,7 @@ __global__ void __maxnreg__(kMaxRegs)
   const int64_t f_begin = starts[warp];
   const int len_w = starts[warp + 1] - starts[warp];
   const StageOffsets off(lane);
-  QueryFrag qf;
+  QueryFrag<kWts> qf;
   WarpState ws;
   ws.reset();
   int r = 0, h = 0, nb = 1, len_eff = 0;
@@ -1309,8 +1355,11 @@ __global__ void __maxnreg__(kMaxRegs)
     if (j == 0) trace_mark<kTrace>(p, kW + 1, lane, 2);
     StageInfo si;
     if (read_stage_info(meta_p, st, si, meta_s) && p.debug_mode != 2 && p.debug_mode != 4) {
-      consume_page<0>(base_s + st * kStageBytes, off, empty_s + 8 * st, lane, si, qf, p.qk_scale_log2,
-                      (lo + (int)(f - pair_P)) * kPage, len_eff, ws);
+      const int pos0 = (lo + (int)(f - pair_P)) * kPage;
+      float* srow = nullptr;
+      if (kWts && g < p.G) srow = p.scores + ((size_t)r * p.Hq + (size_t)h * p.G + g) * p.score_stride + pos0;
+      consume_page<0, kWts>(base_s + st * kStageBytes, off, empty_s + 8 * st, lane, si, qf, p.qk_scale_log2, pos0,
+                            len_eff, ws, srow);
     } else {
       __syncwarp();
       if (lane == 0) mbar_arrive(empty_s + 8 * st);
@@ -1335,12 +1384,12 @@ __global__ void __maxnreg__(kMaxRegs)
       for (int i2 = 0; i2 < 8; ++i2) {
         const int d = 16 * i2 + 2 * g;
         if (2 * c < p.G) {
-          write_final(p, row0 + 2 * c, d, ws.acc[i2][0] * inv0, lse0);
-          write_final(p, row0 + 2 * c, d + 1, ws.acc[i2][2] * inv0, lse0);
+          write_final<kWts>(p, row0 + 2 * c, d, ws.acc[i2][0] * inv0, lse0);
+          write_final<kWts>(p, row0 + 2 * c, d + 1, ws.acc[i2][2] * inv0, lse0);
         }
         if (2 * c + 1 < p.G) {
-          write_final(p, row0 + 2 * c + 1, d, ws.acc[i2][1] * inv1, lse1);
-          write_final(p, row0 + 2 * c + 1, d + 1, ws.acc[i2][3] * inv1, lse1);
+          write_final<kWts>(p, row0 + 2 * c + 1, d, ws.acc[i2][1] * inv1, lse1);
+          write_final<kWts>(p, row0 + 2 * c + 1, d + 1, ws.acc[i2][3] * inv1, lse1);
         }
       }
     } else {
@@ -1373,8 +1422,8 @@ __global__ void __maxnreg__(kMaxRegs)
       ticket = __shfl_sync(0xffffffffu, ticket, 0);
       if (ticket == contributors - 1) {  // last contributor: merge the pair
         fence_acq_rel_gpu();
-        merge_pair(p.part_o, p.part_lse, p.out, p.shard_o, p.shard_lse, p.G, k0, k1, sh.start(k0) >= c0 - cm.ovh,
-                   row0, lane);
+        merge_pair<kWts>(p.part_o, p.part_lse, p.out, p.shard_o, p.shard_lse, p.G, k0, k1, sh.start(k0) >= c0 - cm.ovh,
+                   row0, lane, p.lse_out);
         if (lane == 0) p.counters[pair_id] = 0u;  // leave the ticket clean for the next call
       }
     }
@@ -1451,6 +1500,13 @@ static DecodeKernelFn balanced_for(int shape) {
   return trace_ptr() != nullptr ? balanced_inst<kPaged, 0, true>() : balanced_inst<kPaged, 0>();
 }
 
+// The kernels that also store scores and LSEs (weighted decode) exist in shape 0, paged.
+static DecodeKernelFn weights_kernel(bool balanced) {
+  constexpr Shape sh = kShapes[0];
+  if (balanced) return decode_balanced_kernel<true, sh.warps, sh.stages, sh.max_regs, false, true>;
+  return decode_kernel<true, sh.warps, sh.stages, sh.min_blocks, 0, true>;
+}
+
 static int smem_bytes(int shape) {
   const Shape sh = kShapes[shape];
   return 1024 + sh.stages * (kStageBytes + kMetaBytes + 16);
@@ -1481,6 +1537,21 @@ static int shape_choice() {
       if (kShapes[s].warps == w) return s;
   }
   return -1;
+}
+
+static int configure_weights(int device) {
+  static bool done[kMaxDevices] = {};
+  static std::mutex mu;
+  std::lock_guard<std::mutex> lock(mu);
+  if (device < 0 || device >= kMaxDevices) return fail_cuda("device ordinal beyond the library's table");
+  if (done[device]) return FS_OK;
+  for (int balanced = 0; balanced < 2; ++balanced)
+    if (cudaError_t e = cudaFuncSetAttribute(weights_kernel(balanced != 0), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             balanced ? smem_balanced(0, kMaxSKBatch) : smem_bytes(0));
+        e != cudaSuccess)
+      return fail_cuda("shared-memory limit of the weighted decode kernels", e);
+  done[device] = true;
+  return FS_OK;
 }
 
 template <bool kPaged>
@@ -1837,7 +1908,8 @@ static int validate_exchange(const FsDecodeArgs* a, const FsExchangeArgs* x) {
 }
 
 template <bool kPaged>
-static int launch_decode(const FsDecodeArgs* a_in, void* stream, const FsExchangeArgs* x = nullptr) {
+static int launch_decode(const FsDecodeArgs* a_in, void* stream, const FsExchangeArgs* x = nullptr,
+                         const ScoreTarget* w = nullptr) {
   FsDecodeArgs ax;
   const FsDecodeArgs* a = a_in;
   if (x != nullptr && a_in != nullptr) {  // the exchange writes x->out; the decode's own output is unused
@@ -1850,9 +1922,10 @@ static int launch_decode(const FsDecodeArgs* a_in, void* stream, const FsExchang
   if (x != nullptr && (st = validate_exchange(a_in, x)) != FS_OK) return st;
   int device = 0;
   if (cudaError_t e = cudaGetDevice(&device); e != cudaSuccess) return fail_cuda("cudaGetDevice", e);
-  if (!tuned_shape(a)) return launch_generic_decode(a, device, stream);
-  const int forced = shape_choice();
+  if (!tuned_shape(a)) return launch_generic_decode(a, device, stream, w);
+  const int forced = w != nullptr ? kDefaultShape : shape_choice();
   if ((st = configure_shapes<kPaged>(device, forced)) != FS_OK) return st;
+  if (w != nullptr && (st = configure_weights(device)) != FS_OK) return st;
   Plan pl;
   if (x != nullptr) {
     if ((st = exchange_plan(a, device, forced, &pl)) != FS_OK) return st;
@@ -1912,6 +1985,11 @@ static int launch_decode(const FsDecodeArgs* a_in, void* stream, const FsExchang
     p.xrank = x->rank;
     p.xout_dtype = x->out_dtype;
   }
+  if (w != nullptr) {
+    p.scores = w->scores;
+    p.lse_out = w->lse;
+    p.score_stride = w->stride;
+  }
   if (need > 0) {
     const size_t G = (size_t)p.G;
     const size_t units = pl.balanced ? (size_t)pl.ctas * kShapes[shape].warps * 2 * G
@@ -1923,20 +2001,85 @@ static int launch_decode(const FsDecodeArgs* a_in, void* stream, const FsExchang
   p.counters = reinterpret_cast<unsigned*>(a->tickets);
   const int threads = (kShapes[shape].warps + 1) * 32;
   if (pl.balanced) {
-    balanced_for<kPaged>(shape)<<<(unsigned)pl.ctas, threads, smem_balanced(shape, a->batch),
+    (w != nullptr ? weights_kernel(true) : balanced_for<kPaged>(shape))<<<(unsigned)pl.ctas, threads, smem_balanced(shape, a->batch),
                                   reinterpret_cast<cudaStream_t>(stream)>>>(tmk, tmv, p);
   } else {
     const int64_t grid = (int64_t)a->batch * a->kv_heads * pl.splits;
     if (grid >= (1ll << 31)) return FS_ERR_UNSUPPORTED;
-    kernel_for<kPaged>(shape, debug_mode())<<<(unsigned)grid, threads, smem_bytes(shape),
+    (w != nullptr ? weights_kernel(false) : kernel_for<kPaged>(shape, debug_mode()))<<<(unsigned)grid, threads, smem_bytes(shape),
                                               reinterpret_cast<cudaStream_t>(stream)>>>(tmk, tmv, p);
   }
   return launch_status(pl.balanced ? "balanced decode kernel launch" : "split decode kernel launch");
 }
 
+// Decode workspace, then scores [B, Hq, stride] and LSEs [B, Hq] of a weighted decode.
+struct WeightsPlan {
+  size_t decode, scores, lse;
+  int64_t stride;
+  int splits;  // 0: balanced
+};
+
+static int weights_plan(const FsDecodeArgs* a, int device, WeightsPlan* w) {
+  int st = validate(a, FS_LAYOUT_PAGED);
+  if (st != FS_OK) return st;
+  if (a->page_begin != 0 || a->page_end > 0 || a->shard_o != nullptr) return FS_ERR_INVALID_ARGUMENT;
+  if (!tuned_shape(a)) {
+    w->decode = generic_workspace(a, device, &w->splits);
+  } else {
+    if ((st = configure_shapes<true>(device, kDefaultShape)) != FS_OK) return st;
+    const Plan pl = make_plan(a, device, kDefaultShape);
+    w->decode = pl.balanced ? workspace_balanced(a, pl.ctas, pl.shape) : workspace_for(a, pl.splits);
+    w->splits = pl.balanced ? 0 : pl.splits;
+  }
+  w->decode = align256(w->decode);
+  const int64_t page = a->page_size > 0 ? a->page_size : a->block_size;
+  w->stride = (std::min<int64_t>(a->max_seq_len, page * a->table_cols) + kPage - 1) / kPage * kPage;
+  const size_t rows = (size_t)a->batch * a->q_heads;
+  if (w->stride > 65535ll * 1024) return FS_ERR_UNSUPPORTED;  // the grid of launch_add_weights
+  w->scores = align256(rows * (size_t)w->stride * 4);
+  w->lse = align256(rows * 4);
+  return FS_OK;
+}
+
 }  // namespace fsb
 
 extern "C" {
+
+int fs_paged_decode_weights_workspace_size(const FsDecodeArgs* a, size_t* bytes, int32_t* splits_out) {
+  if (a == nullptr || bytes == nullptr) return FS_ERR_INVALID_ARGUMENT;
+  int device = 0;
+  int st = fsb::validate(a, FS_LAYOUT_PAGED);
+  if (st != FS_OK) return st;
+  if (cudaError_t e = cudaGetDevice(&device); e != cudaSuccess) return fsb::fail_cuda("cudaGetDevice", e);
+  fsb::WeightsPlan w{};
+  if ((st = fsb::weights_plan(a, device, &w)) != FS_OK) return st;
+  *bytes = w.decode + w.scores + w.lse;
+  if (splits_out) *splits_out = w.splits;
+  return FS_OK;
+}
+
+int fs_paged_decode_weights(const FsDecodeArgs* a, float* weights, void* stream) {
+  if (a == nullptr || weights == nullptr) return FS_ERR_INVALID_ARGUMENT;
+  if (reinterpret_cast<uintptr_t>(weights) & 3) return FS_ERR_ALIGNMENT;
+  int device = 0;
+  int st = fsb::validate(a, FS_LAYOUT_PAGED);
+  if (st != FS_OK) return st;
+  if (cudaError_t e = cudaGetDevice(&device); e != cudaSuccess) return fsb::fail_cuda("cudaGetDevice", e);
+  fsb::WeightsPlan w{};
+  if ((st = fsb::weights_plan(a, device, &w)) != FS_OK) return st;
+  if (a->workspace == nullptr || a->workspace_bytes < w.decode + w.scores + w.lse) return FS_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(a->workspace) & 255) return FS_ERR_ALIGNMENT;
+  uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+  const fsb::ScoreTarget t{reinterpret_cast<float*>(ws + w.decode), reinterpret_cast<float*>(ws + w.decode + w.scores),
+                           w.stride};
+  FsDecodeArgs d = *a;
+  d.workspace_bytes = w.decode;
+  if ((st = fsb::launch_decode<true>(&d, stream, nullptr, &t)) != FS_OK) return st;
+  // the generic kernel's splits leave their LSEs apart, behind the split outputs
+  const int parts = fsb::tuned_shape(a) || w.splits <= 1 ? 1 : w.splits;
+  const float* lse = parts == 1 ? t.lse : fsb::generic_part_lse(a, w.splits);
+  return fsb::launch_add_weights(a, t, lse, parts, weights, stream);
+}
 
 int fs_decode_workspace_size(const FsDecodeArgs* a, size_t* bytes, int32_t* splits_out) {
   if (a == nullptr || bytes == nullptr) return FS_ERR_INVALID_ARGUMENT;

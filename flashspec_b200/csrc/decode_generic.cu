@@ -56,6 +56,9 @@ struct GenericParams {
   int64_t num_blocks;  // paged: pages; contiguous: quant blocks per (request, kv head)
   int64_t max_seq_len, page_begin, page_end;
   float qk_scale_log2;
+  float* scores;  // weighted decode (kWts): scores [B, Hq, score_stride], LSEs [B, Hq]
+  float* lse_out;
+  int64_t score_stride;
 };
 
 __device__ __forceinline__ void cp_async16(void* smem, const void* gmem) {
@@ -90,7 +93,7 @@ __device__ __forceinline__ int64_t generic_block(const GenericParams& p, int r, 
   return (phys * p.Hkv + h) * p.bpp + sub;
 }
 
-template <int kDim>
+template <int kDim, bool kWts>
 __global__ void __launch_bounds__(kGW * 32) decode_generic_kernel(const GenericParams p) {
   constexpr int kRow = kDim + 16;  // padded shared-memory row of one token
   constexpr int kDpl = kDim / 32;  // head dims per lane in the O accumulation
@@ -206,6 +209,7 @@ __global__ void __launch_bounds__(kGW * 32) decode_generic_kernel(const GenericP
         for (int g = 0; g < kGMaxG; ++g) {
           if (g < G) {
             const float t = valid ? s[g] * ksc * p.qk_scale_log2 : -INFINITY;
+            if (kWts && valid) p.scores[((size_t)r * p.Hq + (size_t)h * G + g) * p.score_stride + tok] = t;
             float mx = t;
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
@@ -276,6 +280,7 @@ __global__ void __launch_bounds__(kGW * 32) decode_generic_kernel(const GenericP
     const float o = L > 0.f ? O / L : 0.f;
     const float lse = L > 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
     const size_t row = (size_t)r * p.Hq + (size_t)h * G + g;
+    if (kWts && S == 1 && d == 0) p.lse_out[row] = lse;
     if (S > 1) {
       const size_t prow = (size_t)split * p.B * p.Hq + row;
       p.part_o[prow * kDim + d] = o;
@@ -325,7 +330,7 @@ static int generic_splits(const FsDecodeArgs* a, int device, size_t smem) {
   if (a->shard_o != nullptr) return 1;
   if (a->num_splits > 0) return a->num_splits;
   int per_sm = 0;
-  cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, decode_generic_kernel<128>, kGW * 32, smem);
+  cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, decode_generic_kernel<128, false>, kGW * 32, smem);
   if (per_sm <= 0) per_sm = 1;
   const int64_t slots = (int64_t)per_sm * device_sm_count(device) * 2;
   const int64_t pairs = (int64_t)a->batch * a->kv_heads;
@@ -351,7 +356,12 @@ size_t generic_workspace(const FsDecodeArgs* a, int device, int* splits_out) {
   return align256g((size_t)s * rows * a->head_dim * 4) + align256g((size_t)s * rows * 4);
 }
 
-int launch_generic_decode(const FsDecodeArgs* a, int device, void* stream) {
+const float* generic_part_lse(const FsDecodeArgs* a, int splits) {
+  return reinterpret_cast<const float*>(static_cast<const uint8_t*>(a->workspace) +
+                                        align256g((size_t)splits * a->batch * a->q_heads * a->head_dim * 4));
+}
+
+int launch_generic_decode(const FsDecodeArgs* a, int device, void* stream, const ScoreTarget* w) {
   const size_t smem = generic_smem_for(a->head_dim, a->block_size);
   int S = 1;
   const size_t need = generic_workspace(a, device, &S);
@@ -386,6 +396,11 @@ int launch_generic_decode(const FsDecodeArgs* a, int device, void* stream) {
   p.page_begin = a->page_begin;
   p.page_end = a->page_end;
   p.qk_scale_log2 = a->sm_scale * 1.4426950408889634f;
+  if (w != nullptr) {
+    p.scores = w->scores;
+    p.lse_out = w->lse;
+    p.score_stride = w->stride;
+  }
   if (S > 1) {
     const size_t rows = (size_t)a->batch * a->q_heads;
     uint8_t* ws = reinterpret_cast<uint8_t*>(a->workspace);
@@ -404,10 +419,10 @@ int launch_generic_decode(const FsDecodeArgs* a, int device, void* stream) {
   };
   int rc;
   switch (a->head_dim) {
-    case 32: rc = go(decode_generic_kernel<32>); break;
-    case 64: rc = go(decode_generic_kernel<64>); break;
-    case 128: rc = go(decode_generic_kernel<128>); break;
-    default: rc = go(decode_generic_kernel<256>); break;
+    case 32: rc = w ? go(decode_generic_kernel<32, true>) : go(decode_generic_kernel<32, false>); break;
+    case 64: rc = w ? go(decode_generic_kernel<64, true>) : go(decode_generic_kernel<64, false>); break;
+    case 128: rc = w ? go(decode_generic_kernel<128, true>) : go(decode_generic_kernel<128, false>); break;
+    default: rc = w ? go(decode_generic_kernel<256, true>) : go(decode_generic_kernel<256, false>); break;
   }
   if (rc != FS_OK || S <= 1) return rc;
   const int64_t rows = (int64_t)a->batch * a->q_heads;

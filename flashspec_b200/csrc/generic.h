@@ -4,6 +4,7 @@
 #include <stddef.h>
 
 #include "../../include/flashspec_b200.h"
+#include "weights.h"
 
 namespace fsb {
 
@@ -13,6 +14,9 @@ namespace fsb {
 bool generic_supports(const FsDecodeArgs* a);
 // Workspace bytes of a generic call (its split partials) and the split count used.
 size_t generic_workspace(const FsDecodeArgs* a, int device, int* splits_out);
-int launch_generic_decode(const FsDecodeArgs* a, int device, void* stream);
+// w != nullptr: also store the scores, and the LSEs when one split runs.
+int launch_generic_decode(const FsDecodeArgs* a, int device, void* stream, const ScoreTarget* w = nullptr);
+// Where a generic call of `splits` > 1 splits leaves their LSEs, [splits, B * Hq].
+const float* generic_part_lse(const FsDecodeArgs* a, int splits);
 
 }  // namespace fsb

@@ -139,6 +139,19 @@ int fs_paged_decode(const FsDecodeArgs* args, void* stream);
  * the array: calls that may overlap on the GPU race and must be serialised. */
 int fs_paged_decode_noalloc(const FsDecodeArgs* args, void* stream);
 
+/* Paged decode attention that also adds up the softmax weight every cached token
+ * receives: the output of fs_paged_decode, and
+ *   weights[page, kv head, t] += sum of the kv head's queries' weights on that token
+ * for every live token, weights fp32 [num_blocks (pages), Hkv, page] beside the pool (the
+ * measure fs_evict_select keeps tokens by).  No page window, no shard outputs.  The
+ * workspace (256-byte aligned; the size comes from fs_paged_decode_weights_workspace_size)
+ * also holds the scores, 4 bytes a query head and token.  Weights are off by at most about
+ * 1e-6 of themselves (24-bit fixed-point q in the tuned kernels).  A page of one request
+ * gets one addition a call; pages shared by requests add up too, in varying order.
+ * Requests up to 65535 * 1024 tokens.  No counterpart in the reference. */
+int fs_paged_decode_weights_workspace_size(const FsDecodeArgs* args, size_t* bytes, int32_t* splits);
+int fs_paged_decode_weights(const FsDecodeArgs* args, float* weights, void* stream);
+
 /* Log-sum-exp merge of n_parts partial results (split-K partials, or per-GPU
  * shards gathered over NVLink).  Part i's O is o_parts + i*S ([rows, head_dim] fp32)
  * and its LSE lse_parts + i*S' ([rows] fp32), where S = part_stride and S' =
