@@ -15,6 +15,7 @@ from ._build import build
 from .attention import (BACKENDS, fused_dequant_attention_cuda, get_backend, merge_partials,
                         paged_quant_attention_cuda, paged_quant_attention_weights_cuda, register_backend,
                         reset_workspaces)
+from .evict import evict_tokens_cuda
 from .paged import PagedKVAllocator, PagedKVCache
 from .paged import paged_cache_symmetric
 from .quant import (QuantizedTensor, SymQuantizedTensor, build_compression_stats, dequantize_int8_per_block,
@@ -31,6 +32,7 @@ __all__ = [
     "build_compression_stats",
     "dequantize_int8_per_block",
     "estimate_quantized_bytes",
+    "evict_tokens_cuda",
     "fused_dequant_attention_cuda",
     "get_backend",
     "merge_partials",

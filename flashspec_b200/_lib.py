@@ -157,6 +157,37 @@ class FsTreeArgs(C.Structure):
 
 
 # every symbol the header declares, with its signature
+class FsEvictArgs(C.Structure):
+    _fields_ = [
+        ("kv_format", C.c_int32),
+        ("batch", C.c_int32),
+        ("kv_heads", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("page_size", C.c_int32),
+        ("table_cols", C.c_int32),
+        ("max_seq_len", C.c_int32),
+        ("budget", C.c_int32),
+        ("recent", C.c_int32),
+        ("sinks", C.c_int32),
+        ("num_pages", C.c_int64),
+        ("block_table", C.c_void_p),
+        ("lengths", C.c_void_p),
+        ("k_values", C.c_void_p),
+        ("k_scale", C.c_void_p),
+        ("k_zero", C.c_void_p),
+        ("v_values", C.c_void_p),
+        ("v_scale", C.c_void_p),
+        ("v_zero", C.c_void_p),
+        ("weights", C.c_void_p),
+        ("weights_out", C.c_void_p),
+        ("kept", C.c_void_p),
+        ("new_lengths", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t),
+        ("device_status", C.c_void_p),
+    ]
+
+
 SIGNATURES = {
     "fs_abi_version": (C.c_int, []),
     "fs_status_string": (C.c_char_p, [C.c_int]),
@@ -168,6 +199,8 @@ SIGNATURES = {
     "fs_paged_decode_weights_workspace_size": (C.c_int, [C.POINTER(FsDecodeArgs), C.POINTER(C.c_size_t),
                                                          C.POINTER(C.c_int32)]),
     "fs_paged_decode_weights": (C.c_int, [C.POINTER(FsDecodeArgs), C.c_void_p, C.c_void_p]),
+    "fs_evict_workspace_size": (C.c_int, [C.POINTER(FsEvictArgs), C.POINTER(C.c_size_t)]),
+    "fs_evict_tokens": (C.c_int, [C.POINTER(FsEvictArgs), C.c_void_p]),
     "fs_merge_partials": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_int64, C.c_void_p,
                                     C.c_int32, C.c_void_p]),
     "fs_quantize_blocks": (C.c_int, [C.POINTER(FsQuantizeArgs), C.c_void_p]),

@@ -1,0 +1,515 @@
+// Eviction from the paged cache by accumulated attention weight: two kernels.
+//
+// select_tokens_kernel, per (request, kv head) with n > budget live tokens: the first
+// `sinks` and the last `recent` tokens stay, and of the n - sinks - recent between them the
+// K = budget - sinks - recent with the largest weights (ties: the lower position).  A
+// cluster of CTAs takes one row.  It reads the row's weights once, as order-preserving
+// 32-bit keys, into shared memory; three counting passes (11 + 11 + 10 bits) over those
+// find the K-th largest key, the CTAs' histograms being summed over distributed shared
+// memory; then an ordered pass numbers the kept tokens, writes their positions to `kept`
+// and their weights to their new places (zeros behind them).
+//
+// move_tokens_kernel moves the kept tokens' K and V, in place, into the first pages of the
+// request.  In place is what a cache under pressure needs, and the order makes it safe: a
+// kept token never moves up (kept[i] >= i), so page j's sources lie in pages >= j.  A
+// cluster takes one (request, kv head, K|V) and walks its pages in rounds: every warp loads
+// its pages' source tokens into registers, the cluster synchronises, then the warps write.
+// A round writes pages below all that later rounds read.  Affine pages are dequantized and
+// requantized by the format's rule (quant_math.cuh, as fs_page_update does), symmetric ones
+// keep their codes and scales.  A page whose kept tokens stand in it already is left as it
+// is.
+//
+// Both are bound by memory traffic: 4 bytes of weights for every live token, then 2 (D + a
+// scale) bytes read and written for every kept one.
+#include <cooperative_groups.h>
+#include <cuda_runtime.h>
+
+#include <math.h>
+#include <stdint.h>
+#include <algorithm>
+
+#include "../../include/flashspec_b200.h"
+#include "common.h"
+#include "quant_math.cuh"
+
+namespace fsb {
+
+namespace cg = cooperative_groups;
+
+constexpr int kSelThreads = 512;
+constexpr int kBins = 2048;
+constexpr int kSelMaxCluster = 8;
+// keys of one CTA held in shared memory at most (192 KB); longer rows keep them in the workspace
+constexpr int kSelSmemKeys = 48 * 1024;
+constexpr int kSelKeysPerCta = 4096;  // keys a CTA should have before the row gets a larger cluster
+
+struct EvictParams {
+  const int64_t* table;
+  const int64_t* lengths;
+  const float* weights;
+  float* weights_out;
+  int32_t* kept;
+  int64_t* new_lengths;
+  uint32_t* keys;  // workspace [rows, cluster * chunk_cap], or null
+  uint32_t* status;
+  int8_t* values[2];
+  float* scale[2];
+  int16_t* zero[2];
+  int64_t num_pages, max_seq_len;
+  int Hkv, cols, page, D, budget, recent, sinks;
+  int chunk_cap;  // keys of one CTA at most
+  int sym;
+};
+
+__device__ __forceinline__ int64_t live_tokens(const EvictParams& p, int b) {
+  return max((int64_t)0, min(min(p.lengths[b], p.max_seq_len), (int64_t)p.cols * p.page));
+}
+
+// Physical page behind position `pos` of request b; -1 when unallocated or outside the pool.
+__device__ __forceinline__ int64_t page_at(const EvictParams& p, int b, int lp) {
+  const int64_t phys = p.table[(size_t)b * p.cols + lp];
+  if (phys >= p.num_pages) {
+    if (p.status != nullptr) atomicOr(p.status, FS_DEV_BAD_PAGE);
+    return -1;
+  }
+  return phys;
+}
+
+// Larger weight <-> larger key; -0 counts as +0, NaN (of either sign) is above all, and 0 is
+// left for tokens without a page.
+__device__ __forceinline__ uint32_t key_of(float w) {
+  if (isnan(w)) return 0xffffffffu;
+  const uint32_t u = __float_as_uint(w + 0.0f);
+  return (u & 0x80000000u) ? max(~u, 1u) : (u | 0x80000000u);
+}
+__device__ __forceinline__ float weight_of(uint32_t key) {
+  if (key == 0u) return 0.f;
+  return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
+}
+
+// Inclusive scan of v over the block; *total receives the block's sum.
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* warp_sums, uint32_t* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t y = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += y;
+  }
+  __syncthreads();  // warp_sums is free
+  if (lane == 31) warp_sums[warp] = v;
+  __syncthreads();
+  uint32_t before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kSelThreads / 32; ++w) {
+    const uint32_t x = warp_sums[w];
+    if (w < warp) before += x;
+    all += x;
+  }
+  *total = all;
+  return v + before;
+}
+
+// kSmem: the keys live in shared memory, else in the workspace (each CTA in its own part).
+template <bool kSmem>
+__global__ void __launch_bounds__(kSelThreads) select_tokens_kernel(const EvictParams p) {
+  extern __shared__ uint32_t sel_smem[];
+  __shared__ __align__(16) uint32_t hist[kBins];
+  __shared__ uint32_t warp_sums[kSelThreads / 32];
+  __shared__ uint32_t found[2];   // bin of the K-th key, keys above that bin
+  __shared__ uint32_t counts[2];  // this CTA's keys above and equal to the threshold
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int row = blockIdx.x / C, b = row / p.Hkv, h = row % p.Hkv;
+  const int tid = threadIdx.x;
+  const int64_t cap = (int64_t)p.cols * p.page;
+  const int n = (int)live_tokens(p, b);
+  const int count = min(n, p.budget);
+  if (h == 0 && rank == 0 && tid == 0) p.new_lengths[b] = count;
+  int32_t* kept = p.kept + (size_t)row * p.budget;
+  const int lo = n > p.budget ? p.sinks : 0, hi = n > p.budget ? n - p.recent : 0;  // the contested range
+  const int K = n > p.budget ? p.budget - p.sinks - p.recent : 0;
+
+  // ---- the row's weights, as keys of positions [c0, c1)
+  const int chunk = (n + 4 * C - 1) / (4 * C) * 4;  // <= chunk_cap
+  const int c0 = min(rank * chunk, n), c1 = min(c0 + chunk, n);
+  uint32_t* keys = kSmem ? sel_smem : p.keys + (size_t)blockIdx.x * p.chunk_cap;
+  for (int i = c0 + tid; i < c1; i += kSelThreads) {
+    const int lp = i / p.page;
+    const int64_t phys = page_at(p, b, lp);
+    keys[i - c0] = phys < 0 ? 0u : key_of(p.weights[(phys * p.Hkv + h) * p.page + (i - lp * p.page)]);
+  }
+
+  // ---- the K-th largest key T of the contested range, and how many equal to T stay
+  uint32_t T = 0xffffffffu, quota = 0;  // kept: key > T, and the first `quota` keys == T
+  const bool contest = K > 0;
+  if (contest) {
+    uint32_t prefix = 0, need = (uint32_t)K;
+    const int a0 = max(c0, lo), a1 = min(c1, hi);
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+      for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0u;
+      __syncthreads();
+      for (int i = a0 + tid; i < a1; i += kSelThreads) {
+        const uint32_t k = keys[i - c0];
+        if (pass == 0 || (k >> (shift + bits)) == prefix) atomicAdd(hist + ((k >> shift) & ((1u << bits) - 1)), 1u);
+      }
+      cluster.sync();  // every CTA's histogram is complete
+      // thread t sums bins [4t, 4t + 4) from the top over the cluster
+      const int top = kBins - 4 * (tid + 1);
+      uint32_t v[4] = {0, 0, 0, 0};
+      for (int r = 0; r < C; ++r) {
+        const uint4 x = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(hist, r) + top);
+        v[3] += x.x, v[2] += x.y, v[1] += x.z, v[0] += x.w;
+      }
+      const uint32_t mine = v[0] + v[1] + v[2] + v[3];
+      uint32_t total;
+      uint32_t before = block_scan(mine, warp_sums, &total) - mine;
+      if (before < need && before + mine >= need) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (before < need && before + v[j] >= need) {
+            found[0] = (uint32_t)(top + 3 - j);
+            found[1] = before;
+          }
+          before += v[j];
+        }
+      }
+      cluster.sync();  // found is written; no CTA reads a histogram that is cleared next
+      prefix = (prefix << bits) | found[0];
+      need -= found[1];
+    }
+    T = prefix;
+    quota = need;
+    uint32_t above = 0, equal = 0;
+    for (int i = a0 + tid; i < a1; i += kSelThreads) {
+      const uint32_t k = keys[i - c0];
+      above += k > T;
+      equal += k == T;
+    }
+    uint32_t total;
+    block_scan(above, warp_sums, &total);
+    if (tid == 0) counts[0] = total;
+    block_scan(equal, warp_sums, &total);
+    if (tid == 0) counts[1] = total;
+  }
+  cluster.sync();  // counts are written; every weight of the row has been read
+  uint32_t base_above = 0, base_equal = 0;
+  if (contest) {
+    for (int r = 0; r < rank; ++r) {
+      const uint32_t* c = cluster.map_shared_rank(counts, r);
+      base_above += c[0];
+      base_equal += c[1];
+    }
+  }
+
+  // ---- number the kept tokens in order; four consecutive positions a thread
+  auto put = [&](int dst, int pos, uint32_t key) {
+    kept[dst] = pos;
+    const int lp = dst / p.page;
+    const int64_t phys = page_at(p, b, lp);
+    if (phys >= 0) p.weights_out[(phys * p.Hkv + h) * p.page + (dst - lp * p.page)] = weight_of(key);
+  };
+  for (int t0 = c0; t0 < c1; t0 += 4 * kSelThreads) {
+    const int i0 = t0 + 4 * tid;
+    uint32_t key[4], packed = 0;  // above in the low half, equal in the high half (<= 2048 each)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = i0 + j;
+      key[j] = i < c1 ? keys[i - c0] : 0u;
+      if (contest && i < c1 && i >= lo && i < hi) packed += key[j] > T ? 1u : key[j] == T ? 0x10000u : 0u;
+    }
+    uint32_t total = 0, at = 0;
+    if (contest) at = block_scan(packed, warp_sums, &total) - packed;
+    uint32_t above = base_above + (at & 0xffffu), equal = base_equal + (at >> 16);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = i0 + j;
+      if (i >= c1) continue;
+      if (n <= p.budget || i < lo) {
+        put(i, i, key[j]);
+      } else if (i >= hi) {
+        put(p.budget - (n - i), i, key[j]);
+      } else if (contest && key[j] > T) {
+        put(lo + (int)(above + min(equal, quota)), i, key[j]);
+        ++above;
+      } else if (contest && key[j] == T) {
+        if (equal < quota) put(lo + (int)(above + equal), i, key[j]);
+        ++equal;
+      }
+    }
+    base_above += total & 0xffffu;
+    base_equal += total >> 16;
+  }
+  // ---- no tokens behind the kept ones: positions -1, weights zero
+  for (int i = count + rank * kSelThreads + tid; i < p.budget; i += C * kSelThreads) kept[i] = -1;
+  for (int64_t i = count + rank * kSelThreads + tid; i < cap; i += C * kSelThreads) {
+    const int64_t lp = i / p.page, phys = page_at(p, b, (int)lp);
+    if (phys >= 0) p.weights_out[(phys * p.Hkv + h) * p.page + (i - lp * p.page)] = 0.f;
+  }
+  cluster.sync();  // no CTA leaves while its counts may still be read
+}
+
+constexpr int kMoveWarps = 16;
+
+// One page of K or V in a warp's registers: kCh 16-byte chunks a lane, chunk c of lane l
+// being bytes [16 (32 c + l), ...) of the page's [page, D] block.
+template <int kCh, bool kSym>
+struct PageRegs {
+  uint4 raw[kCh];
+  float scale[kSym ? 1 : kCh];  // affine: scale and zero point of each chunk's source block
+  int16_t zero[kSym ? 1 : kCh];
+  float tok_scale[2];  // symmetric: scales of tokens `lane` and `lane + 32`
+  int64_t dst;         // block index of the destination, -1: nothing to write
+};
+
+template <int kCh, int kPages, bool kSym>
+__global__ void __launch_bounds__(kMoveWarps * 32) move_tokens_kernel(const EvictParams p) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int item = blockIdx.x / C, kv = item & 1, row = item >> 1, b = row / p.Hkv, h = row % p.Hkv;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t n = live_tokens(p, b);
+  if (n <= p.budget) return;  // the whole cluster: nothing moves
+  const int page = p.page, D = p.D, E = page * D, npg = (p.budget + page - 1) / page;
+  const int32_t* kept = p.kept + (size_t)row * p.budget;
+  int8_t* values = p.values[kv];
+  float* scale = p.scale[kv];
+  int16_t* zero = p.zero[kv];
+  const int per_round = C * kMoveWarps * kPages;
+  for (int r0 = 0; r0 < npg; r0 += per_round) {
+    PageRegs<kCh, kSym> regs[kPages];
+#pragma unroll
+    for (int q = 0; q < kPages; ++q) {
+      PageRegs<kCh, kSym>& g = regs[q];
+      const int pg = r0 + (rank * kMoveWarps + warp) * kPages + q;
+      g.dst = -1;
+      if (pg >= npg) continue;
+      const int rows = min(page, p.budget - pg * page);  // kept tokens of the page
+      bool stays = true;
+      for (int t = lane; t < rows; t += 32) stays = stays && kept[pg * page + t] == pg * page + t;
+      const int64_t phys = page_at(p, b, pg);
+      if (__all_sync(0xffffffffu, stays) || phys < 0) continue;
+      g.dst = phys * p.Hkv + h;
+#pragma unroll
+      for (int c = 0; c < kCh; ++c) {
+        const int e = 16 * (32 * c + lane), t = e / D;
+        g.raw[c] = make_uint4(0u, 0u, 0u, 0u);
+        if (!kSym) g.scale[c] = 0.f, g.zero[c] = 128;  // an absent token dequantizes to 0
+        if (e < E && t < rows) {
+          const int src = kept[pg * page + t], lp = src / page;
+          const int64_t sp = page_at(p, b, lp);
+          if (sp >= 0) {
+            const int64_t blk = sp * p.Hkv + h;
+            g.raw[c] = *reinterpret_cast<const uint4*>(values + blk * E + (src - lp * page) * D + (e - t * D));
+            if (!kSym) g.scale[c] = scale[blk], g.zero[c] = zero[blk];
+          }
+        }
+      }
+      if (kSym) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int t = lane + 32 * u;
+          g.tok_scale[u] = 1.0e-8f;
+          if (t < rows) {
+            const int src = kept[pg * page + t], lp = src / page;
+            const int64_t sp = page_at(p, b, lp);
+            if (sp >= 0) g.tok_scale[u] = scale[(sp * p.Hkv + h) * page + (src - lp * page)];
+          }
+        }
+      }
+    }
+    cluster.sync();  // all sources of this round are in registers
+#pragma unroll
+    for (int q = 0; q < kPages; ++q) {
+      const PageRegs<kCh, kSym>& g = regs[q];
+      if (g.dst < 0) continue;
+      if (kSym) {
+#pragma unroll
+        for (int c = 0; c < kCh; ++c) {
+          const int e = 16 * (32 * c + lane);
+          if (e < E) *reinterpret_cast<uint4*>(values + g.dst * E + e) = g.raw[c];
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          if (lane + 32 * u < page) scale[g.dst * page + lane + 32 * u] = g.tok_scale[u];
+        continue;
+      }
+      float mn = INFINITY, mx = -INFINITY, v[16];
+#pragma unroll
+      for (int c = 0; c < kCh; ++c) {
+        if (16 * (32 * c + lane) >= E) continue;
+        dequant16(make_int4((int)g.raw[c].x, (int)g.raw[c].y, (int)g.raw[c].z, (int)g.raw[c].w), g.scale[c],
+                  g.zero[c], v);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          mn = fminf(mn, v[j]);
+          mx = fmaxf(mx, v[j]);
+        }
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      }
+      const QParams qp = qparams_from_range(mn, mx);
+#pragma unroll
+      for (int c = 0; c < kCh; ++c) {
+        const int e = 16 * (32 * c + lane);
+        if (e >= E) continue;
+        dequant16(make_int4((int)g.raw[c].x, (int)g.raw[c].y, (int)g.raw[c].z, (int)g.raw[c].w), g.scale[c],
+                  g.zero[c], v);
+        *reinterpret_cast<uint4*>(values + g.dst * E + e) = quantize16_fast(v, qp);
+      }
+      if (lane == 0) {
+        scale[g.dst] = qp.scale;
+        zero[g.dst] = (int16_t)qp.zp;
+      }
+    }
+  }
+}
+
+// Cluster of a row of `tokens` positions, and the keys of one of its CTAs.
+static int select_cluster(int64_t tokens, int* chunk_cap) {
+  int C = 1;
+  while (C < kSelMaxCluster && tokens > (int64_t)C * kSelKeysPerCta) C *= 2;
+  *chunk_cap = (int)((tokens + 4 * C - 1) / (4 * C) * 4);
+  return C;
+}
+
+static int evict_check(const FsEvictArgs* a) {
+  if (a == nullptr || a->block_table == nullptr || a->lengths == nullptr || a->weights == nullptr ||
+      a->weights_out == nullptr || a->kept == nullptr || a->new_lengths == nullptr || a->k_values == nullptr ||
+      a->v_values == nullptr || a->k_scale == nullptr || a->v_scale == nullptr)
+    return FS_ERR_INVALID_ARGUMENT;
+  if (a->kv_format != FS_KV_AFFINE_BLOCK && a->kv_format != FS_KV_SYMMETRIC) return FS_ERR_INVALID_ARGUMENT;
+  if (a->kv_format == FS_KV_AFFINE_BLOCK && (a->k_zero == nullptr || a->v_zero == nullptr))
+    return FS_ERR_INVALID_ARGUMENT;
+  if (a->batch <= 0 || a->kv_heads <= 0 || a->num_pages <= 0 || a->table_cols <= 0 || a->max_seq_len < 0 ||
+      a->budget <= 0 || a->recent < 0 || a->sinks < 0 || (int64_t)a->recent + a->sinks > a->budget)
+    return FS_ERR_INVALID_ARGUMENT;
+  // the kernels read `lengths` while new_lengths is being written
+  if (static_cast<const int64_t*>(a->new_lengths) == a->lengths) return FS_ERR_INVALID_ARGUMENT;
+  if (a->page_size <= 0 || a->page_size > 64 || a->head_dim <= 0 || a->head_dim % 16 ||
+      a->page_size * (a->head_dim + 16) > 12 * 1024)
+    return FS_ERR_UNSUPPORTED;
+  if ((int64_t)a->batch * a->kv_heads * 2 * kSelMaxCluster >= (1ll << 31)) return FS_ERR_UNSUPPORTED;
+  if ((int64_t)a->table_cols * a->page_size >= (1ll << 31) - 4 * kSelThreads) return FS_ERR_UNSUPPORTED;
+  if ((reinterpret_cast<uintptr_t>(a->k_values) | reinterpret_cast<uintptr_t>(a->v_values)) & 15)
+    return FS_ERR_ALIGNMENT;
+  if ((reinterpret_cast<uintptr_t>(a->weights) | reinterpret_cast<uintptr_t>(a->weights_out) |
+       reinterpret_cast<uintptr_t>(a->k_scale) | reinterpret_cast<uintptr_t>(a->v_scale)) & 3)
+    return FS_ERR_ALIGNMENT;
+  return FS_OK;
+}
+
+static int64_t evict_tokens_at_most(const FsEvictArgs* a) {
+  return std::min<int64_t>(a->max_seq_len, (int64_t)a->table_cols * a->page_size);
+}
+
+static size_t evict_workspace(const FsEvictArgs* a) {
+  int chunk = 0;
+  const int C = select_cluster(evict_tokens_at_most(a), &chunk);
+  return chunk <= kSelSmemKeys ? 0 : (size_t)a->batch * a->kv_heads * C * chunk * 4;
+}
+
+template <typename Kernel>
+static int launch_cluster(Kernel kernel, const char* what, int64_t rows, int cluster, int threads, size_t smem,
+                          const EvictParams& p, void* stream) {
+  if (smem > 0) {
+    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        e != cudaSuccess)
+      return fail_cuda(what, e);
+  }
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = (unsigned)cluster;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(rows * cluster));
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = reinterpret_cast<cudaStream_t>(stream);
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p); e != cudaSuccess) return fail_cuda(what, e);
+  return FS_OK;
+}
+
+template <bool kSym>
+static int launch_move(const FsEvictArgs* a, const EvictParams& p, void* stream) {
+  const int chunks = (a->page_size * a->head_dim + 511) / 512;
+  const int npg = (a->budget + a->page_size - 1) / a->page_size;
+  const int64_t rows = (int64_t)a->batch * a->kv_heads * 2;
+  auto go = [&](auto kernel, int pages) {
+    // as many CTAs as one round of the row's pages takes, so that few rounds wait for each other
+    int C = 1;
+    while (C < 8 && npg > C * kMoveWarps * pages) C *= 2;
+    return launch_cluster(kernel, "token move kernel launch", rows, C, kMoveWarps * 32, 0, p, stream);
+  };
+  if (chunks <= 1) return go(move_tokens_kernel<1, 4, kSym>, 4);
+  if (chunks <= 2) return go(move_tokens_kernel<2, 4, kSym>, 4);
+  if (chunks <= 4) return go(move_tokens_kernel<4, 2, kSym>, 2);
+  if (chunks <= 8) return go(move_tokens_kernel<8, 1, kSym>, 1);
+  if (chunks <= 16) return go(move_tokens_kernel<16, 1, kSym>, 1);
+  return go(move_tokens_kernel<24, 1, kSym>, 1);
+}
+
+}  // namespace fsb
+
+extern "C" {
+
+int fs_evict_workspace_size(const FsEvictArgs* a, size_t* bytes) {
+  if (bytes == nullptr) return FS_ERR_INVALID_ARGUMENT;
+  if (int st = fsb::evict_check(a); st != FS_OK) return st;
+  *bytes = fsb::evict_workspace(a);
+  return FS_OK;
+}
+
+int fs_evict_tokens(const FsEvictArgs* a, void* stream) {
+  using namespace fsb;
+  if (int st = evict_check(a); st != FS_OK) return st;
+  const size_t need = evict_workspace(a);
+  if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need)) return FS_ERR_WORKSPACE;
+  if (need > 0 && (reinterpret_cast<uintptr_t>(a->workspace) & 3)) return FS_ERR_ALIGNMENT;
+  EvictParams p{};
+  p.table = a->block_table;
+  p.lengths = a->lengths;
+  p.weights = a->weights;
+  p.weights_out = a->weights_out;
+  p.kept = a->kept;
+  p.new_lengths = a->new_lengths;
+  p.status = a->device_status;
+  p.values[0] = a->k_values;
+  p.values[1] = a->v_values;
+  p.scale[0] = a->k_scale;
+  p.scale[1] = a->v_scale;
+  p.zero[0] = a->k_zero;
+  p.zero[1] = a->v_zero;
+  p.num_pages = a->num_pages;
+  p.max_seq_len = a->max_seq_len;
+  p.Hkv = a->kv_heads;
+  p.cols = a->table_cols;
+  p.page = a->page_size;
+  p.D = a->head_dim;
+  p.budget = a->budget;
+  p.recent = a->recent;
+  p.sinks = a->sinks;
+  p.sym = a->kv_format == FS_KV_SYMMETRIC;
+  const int C = select_cluster(evict_tokens_at_most(a), &p.chunk_cap);
+  const int64_t rows = (int64_t)a->batch * a->kv_heads;
+  int st;
+  if (need > 0) {
+    p.keys = static_cast<uint32_t*>(a->workspace);
+    st = launch_cluster(select_tokens_kernel<false>, "token selection kernel launch", rows, C, kSelThreads, 0, p, stream);
+  } else {
+    st = launch_cluster(select_tokens_kernel<true>, "token selection kernel launch", rows, C, kSelThreads,
+                        (size_t)std::max(p.chunk_cap, 4) * 4, p, stream);
+  }
+  if (st != FS_OK) return st;
+  // no request can be longer than the budget: nothing to move
+  if (evict_tokens_at_most(a) <= a->budget) return FS_OK;
+  return p.sym ? launch_move<true>(a, p, stream) : launch_move<false>(a, p, stream);
+}
+
+}  // extern "C"

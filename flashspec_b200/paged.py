@@ -321,10 +321,14 @@ class PagedKVAllocator:
     (allocation takes the lowest free page, which is what the reference's sorted list +
     pop(0) does) and a slot-indexed numpy page table (row = live request, -1 padded), so
     ``to_cache`` and single-token ``append_batch`` are a few numpy operations rather than
-    a Python loop per request.  Every data write is one batched ``fs_page_update``."""
+    a Python loop per request.  Every data write is one batched ``fs_page_update``.
+
+    With ``track_weights`` the allocator keeps ``weights``, fp32 [capacity_blocks, heads,
+    block_size] beside the pool, for ``paged_quant_attention_weights_cuda`` to add to and
+    ``evict_batch`` to cut requests by; pages on the free list have weight zero."""
 
     def __init__(self, *, capacity_blocks: int, heads: int, head_dim: int, block_size: int = 16,
-                 device="cuda", dtype: torch.dtype = torch.float32) -> None:
+                 device="cuda", dtype: torch.dtype = torch.float32, track_weights: bool = False) -> None:
         if capacity_blocks <= 0:
             raise ValueError("capacity_blocks must be positive")
         if heads <= 0 or head_dim <= 0:
@@ -341,6 +345,10 @@ class PagedKVAllocator:
         self.dtype = dtype
         self.k_quant = empty_pool(self.capacity_blocks, self.heads, self.block_size, self.head_dim, self.device)
         self.v_quant = empty_pool(self.capacity_blocks, self.heads, self.block_size, self.head_dim, self.device)
+        self.weights: Optional[torch.Tensor] = None
+        if track_weights:
+            self.weights = torch.zeros((self.capacity_blocks, self.heads, self.block_size), dtype=torch.float32,
+                                       device=self.device)
         self._free: List[int] = list(range(self.capacity_blocks))  # a valid min-heap
         self._requests: Dict[int, _Request] = {}
         self._ptab = np.full((16, 16), -1, np.int64)  # [slot, logical page] -> physical page
@@ -498,7 +506,11 @@ class PagedKVAllocator:
     def release_request(self, request_id: int) -> None:
         """paged.py:146-151: the pages return to the free list (not zeroed)."""
         req = self._requests.pop(int(request_id))
-        for p in self._ptab[req.slot, : self._npages[req.slot]].tolist():
+        pages = self._ptab[req.slot, : self._npages[req.slot]].copy()
+        if self.weights is not None and pages.size:
+            with torch.cuda.device(self.device):
+                self.weights.index_fill_(0, _upload(pages, self.device).view(torch.int64), 0.0)
+        for p in pages.tolist():
             heapq.heappush(self._free, p)
         n_old = int(self._npages[req.slot])
         self._dirty_e.append((np.full(n_old, req.slot, np.int64), np.arange(n_old, dtype=np.int64)))
@@ -507,6 +519,34 @@ class PagedKVAllocator:
         self._npages[req.slot] = 0
         self._lens[req.slot] = 0
         self._free_slots.append(req.slot)
+
+    def evict_batch(self, request_ids: Sequence[int], budget: int, *, recent: int, sinks: int = 0) -> torch.Tensor:
+        """Cut the requests to at most ``budget`` tokens by their accumulated weights
+        (``evict_tokens_cuda`` in place on the pool and ``weights``) and free the pages that
+        fall empty.  Returns kept int32 [requests, heads, budget].  No host
+        synchronisation: the new lengths are min(length, budget)."""
+        if self.weights is None:
+            raise RuntimeError("evict_batch needs an allocator with track_weights=True")
+        from .evict import evict_tokens_cuda
+
+        ids, budget = [int(r) for r in request_ids], int(budget)
+        if len(set(ids)) != len(ids):
+            raise ValueError("a request can be cut once a call")
+        _, kept = evict_tokens_cuda(self.to_cache(ids), self.weights, budget, recent=recent, sinks=sinks)
+        left = (budget + self.block_size - 1) // self.block_size
+        for rid in ids:
+            req = self._requests[rid]
+            if req.length <= budget:
+                continue
+            slot, had = req.slot, int(self._npages[req.slot])
+            for p in self._ptab[slot, left:had].tolist():
+                heapq.heappush(self._free, p)
+            self._ptab[slot, left:had] = -1
+            self._dirty_e.append((np.full(had - left, slot, np.int64), np.arange(left, had, dtype=np.int64)))
+            self._dirty_l.append(np.array([slot], np.int64))
+            self._npages[slot] = left
+            self._lens[slot] = req.length = budget
+        return kept
 
     # -- views ---------------------------------------------------------------------------
     def block_table_numpy(self, request_ids: Sequence[int]) -> Tuple[np.ndarray, np.ndarray]:

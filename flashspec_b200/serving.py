@@ -12,7 +12,10 @@ with the token append placed before attention as the configuration specifies):
      lowest-first free list, never zeroed).
 
 Arrivals are Poisson(rate) per step, prompt lengths U[prompt_min, prompt_max], output
-lengths U[out_min, out_max]; everything is seeded.  The same schedule can be replayed
+lengths U[out_min, out_max]; everything is seeded.  With ``kv_budget`` the attention also
+adds up the weight every cached token receives, and after it the requests that have grown
+more than ``kv_slack`` tokens past the budget are cut back to it (``evict_batch``: the
+heaviest tokens and the last ``kv_recent`` of every head stay).  The same schedule can be replayed
 on the CPU oracle allocator (``schedule`` is pure host logic).
 """
 
@@ -42,6 +45,15 @@ class ServingConfig:
     page: int = 16
     seed: int = 0
     capacity_pages: Optional[int] = None  # default: max_live * pages of the longest request
+    kv_budget: Optional[int] = None  # tokens a request is cut back to; default: never
+    kv_slack: int = 256
+    kv_recent: int = 64
+
+    def held(self, prompt: int, out_len: int) -> int:
+        """Tokens a request holds at most: cut requests never pass their prompt (cut at its
+        first step) or the budget and its slack by more than the step's own token."""
+        whole = prompt + out_len
+        return whole if self.kv_budget is None else min(whole, max(prompt, self.kv_budget + self.kv_slack) + 1)
 
     def capacity(self) -> int:
         if self.capacity_pages:
@@ -88,13 +100,13 @@ def run(cfg: ServingConfig, device="cuda", measure: bool = True, recorder: Optio
     device = torch.device(device)
     gen = torch.Generator(device=device).manual_seed(cfg.seed + 1)
     alloc = fs.PagedKVAllocator(capacity_blocks=cfg.capacity(), heads=cfg.heads, head_dim=cfg.head_dim,
-                                block_size=cfg.page, device=device)
+                                block_size=cfg.page, device=device, track_weights=cfg.kv_budget is not None)
     sched = Schedule(cfg)
     live: Dict[int, Request] = {}
     committed = 0  # pages the live requests will hold at their full length
     t_attn = t_append = t_prefill = 0.0
     attn_bytes = append_bytes = 0
-    tokens = finished = admitted = 0
+    tokens = finished = admitted = cuts = 0
     launches = 0  # this library's kernels: one page update per prefill, per append, one decode per step
     ev = lambda: torch.cuda.Event(enable_timing=True)
     step_times = []
@@ -110,7 +122,7 @@ def run(cfg: ServingConfig, device="cuda", measure: bool = True, recorder: Optio
         admitted_before = admitted
         while sched.queue and len(live) < cfg.max_live:
             r = sched.queue[0]
-            need = _pages(r.prompt + r.out_len, cfg.page)
+            need = _pages(cfg.held(r.prompt, r.out_len), cfg.page)
             if committed + need > alloc.capacity_blocks:
                 break
             sched.queue.pop(0)
@@ -146,7 +158,10 @@ def run(cfg: ServingConfig, device="cuda", measure: bool = True, recorder: Optio
         lens = [alloc._requests[i].length for i in ids]
         t0 = ev()
         t0.record()
-        out = fs.paged_quant_attention_cuda(q, cache)
+        if cfg.kv_budget is None:
+            out = fs.paged_quant_attention_cuda(q, cache)
+        else:
+            out = fs.paged_quant_attention_weights_cuda(q, cache, alloc.weights)
         t1 = ev()
         t1.record()
         attn_bytes += algorithmic_bytes(b, cfg.heads, cfg.heads, lens, table_cols=int(cache.block_table.shape[1]))
@@ -154,6 +169,15 @@ def run(cfg: ServingConfig, device="cuda", measure: bool = True, recorder: Optio
         launches += 2
         if recorder is not None:
             recorder.append(("attn", list(ids), q.cpu().numpy(), out.cpu().numpy()))
+        if cfg.kv_budget is not None:
+            launches += 1  # the weighted decode is two kernels
+            over = [i for i, n in zip(ids, lens) if n > cfg.kv_budget + cfg.kv_slack]
+            if over:
+                kept = alloc.evict_batch(over, cfg.kv_budget, recent=cfg.kv_recent)
+                launches += 2
+                cuts += len(over)
+                if recorder is not None:
+                    recorder.append(("evict", list(over), kept.cpu().numpy(), None))
         # 4. release finished requests
         for rid in ids:
             live[rid].generated += 1
@@ -161,7 +185,7 @@ def run(cfg: ServingConfig, device="cuda", measure: bool = True, recorder: Optio
                 alloc.release_request(rid)
                 if recorder is not None:
                     recorder.append(("release", rid, None, None))
-                committed -= _pages(live[rid].prompt + live[rid].out_len, cfg.page)
+                committed -= _pages(cfg.held(live[rid].prompt, live[rid].out_len), cfg.page)
                 del live[rid]
                 finished += 1
         s1 = ev()
@@ -189,6 +213,8 @@ def run(cfg: ServingConfig, device="cuda", measure: bool = True, recorder: Optio
         "allocated_blocks": st["allocated_blocks"], "free_blocks": st["free_blocks"],
         "block_utilization": st["block_utilization"], "fragmentation": st["fragmentation"],
     }
+    if cfg.kv_budget is not None:
+        res["cuts"] = cuts
     if measure and step_times:
         res.update({
             "step_ms_median": float(np.median(step_times)), "step_ms_mean": float(np.mean(step_times)),

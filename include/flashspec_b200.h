@@ -143,7 +143,7 @@ int fs_paged_decode_noalloc(const FsDecodeArgs* args, void* stream);
  * receives: the output of fs_paged_decode, and
  *   weights[page, kv head, t] += sum of the kv head's queries' weights on that token
  * for every live token, weights fp32 [num_blocks (pages), Hkv, page] beside the pool (the
- * measure fs_evict_select keeps tokens by).  No page window, no shard outputs.  The
+ * measure fs_evict_tokens keeps tokens by).  No page window, no shard outputs.  The
  * workspace (256-byte aligned; the size comes from fs_paged_decode_weights_workspace_size)
  * also holds the scores, 4 bytes a query head and token.  Weights are off by at most about
  * 1e-6 of themselves (24-bit fixed-point q in the tuned kernels).  A page of one request
@@ -151,6 +151,46 @@ int fs_paged_decode_noalloc(const FsDecodeArgs* args, void* stream);
  * Requests up to 65535 * 1024 tokens.  No counterpart in the reference. */
 int fs_paged_decode_weights_workspace_size(const FsDecodeArgs* args, size_t* bytes, int32_t* splits);
 int fs_paged_decode_weights(const FsDecodeArgs* args, float* weights, void* stream);
+
+/* Eviction from the paged cache: every request with more than `budget` live tokens keeps,
+ * per kv head, its first `sinks` and last `recent` tokens and the budget - sinks - recent
+ * heaviest (by `weights`) of those between, ties going to the lower position; the kept
+ * tokens' K and V move, in order and in place, to positions 0 .. budget - 1 of the request's
+ * own pages, which must belong to that request alone and be listed once.  Affine pages are
+ * dequantized and requantized as fs_page_update does (rows behind the last kept token count
+ * as zeros), symmetric ones keep codes and scales; a page whose kept tokens stand in it
+ * already is left as it is, and so are all pages of a request within its budget.  Weights
+ * are ordered as numbers, -0 as 0, NaN above all; a token on an unallocated page comes last
+ * and moves as zeros.
+ *   kept [batch, kv_heads, budget]: the kept tokens' positions, ascending, -1 behind them
+ *   new_lengths [batch]: min(live tokens, budget); not the array `lengths`
+ *   weights_out: as `weights` (the same array for in place, else disjoint): the kept tokens'
+ *     weights at their new places and zeros at every other position of the request's pages
+ * Quant block = page, 1 .. 64 tokens, head_dim a multiple of 16, page * (head_dim + 16) <=
+ * 12 KB.  Workspace: fs_evict_workspace_size bytes (0 for requests up to 393216 tokens). */
+typedef struct FsEvictArgs {
+  int32_t kv_format;
+  int32_t batch, kv_heads, head_dim, page_size, table_cols, max_seq_len;
+  int32_t budget, recent, sinks;
+  int64_t num_pages;
+  const int64_t* block_table; /* [batch, table_cols] */
+  const int64_t* lengths;     /* [batch] */
+  int8_t* k_values;
+  float* k_scale;
+  int16_t* k_zero;
+  int8_t* v_values;
+  float* v_scale;
+  int16_t* v_zero;
+  const float* weights;       /* [num_pages, kv_heads, page_size] */
+  float* weights_out;
+  int32_t* kept;
+  int64_t* new_lengths;
+  void* workspace;
+  size_t workspace_bytes;
+  uint32_t* device_status;    /* optional device word receiving FS_DEV_BAD_PAGE */
+} FsEvictArgs;
+int fs_evict_workspace_size(const FsEvictArgs* args, size_t* bytes);
+int fs_evict_tokens(const FsEvictArgs* args, void* stream);
 
 /* Log-sum-exp merge of n_parts partial results (split-K partials, or per-GPU
  * shards gathered over NVLink).  Part i's O is o_parts + i*S ([rows, head_dim] fp32)

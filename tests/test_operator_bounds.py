@@ -1,0 +1,108 @@
+"""CPU checks of the cache operators' C boundary: struct layouts, and refusals that the
+entry points make before any CUDA call."""
+
+from __future__ import annotations
+
+import ctypes as C
+import subprocess
+from pathlib import Path
+
+import pytest
+
+HEADER = Path(__file__).resolve().parents[1] / "include" / "flashspec_b200.h"
+
+
+def layouts():
+    from flashspec_b200 import _lib
+
+    return {"FsEvictArgs": _lib.FsEvictArgs}
+
+
+def test_struct_layouts_match_c(tmp_path):
+    lines = ['#include <stdio.h>', '#include <stddef.h>', f'#include "{HEADER}"', "int main(void){"]
+    for name, cls in layouts().items():
+        lines.append(f'printf("{name} %zu\\n", sizeof({name}));')
+        lines += [f'printf("{name}.{f} %zu\\n", offsetof({name}, {f}));' for f, _ in cls._fields_]
+    src, exe = tmp_path / "layout.c", tmp_path / "layout"
+    src.write_text("\n".join(lines + ["return 0;}"]))
+    subprocess.run(["gcc", "-std=c99", str(src), "-o", str(exe)], check=True)
+    got = dict(x.split() for x in subprocess.run([str(exe)], check=True, capture_output=True, text=True)
+               .stdout.splitlines())
+    for name, cls in layouts().items():
+        assert int(got[name]) == C.sizeof(cls), name
+        for f, _ in cls._fields_:
+            assert int(got[f"{name}.{f}"]) == getattr(cls, f).offset, f"{name}.{f}"
+
+
+def decode_args():
+    from flashspec_b200 import _lib
+
+    a = _lib.FsDecodeArgs()
+    a.layout = _lib.FS_LAYOUT_PAGED
+    a.q = a.k_values = a.v_values = a.k_scale = a.v_scale = a.k_zero = a.v_zero = 4096
+    a.block_table = a.lengths = a.out = 4096
+    a.batch, a.q_heads, a.kv_heads, a.head_dim, a.block_size = 2, 8, 8, 128, 16
+    a.num_blocks, a.table_cols, a.max_seq_len = 64, 4, 64
+    a.sm_scale = 128 ** -0.5
+    return a
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(layout=0), 1), (dict(q_heads=7), 1), (dict(out=None), 1), (dict(lengths=None), 1), (dict(q_heads=72), 2),
+    (dict(head_dim=96), 2), (dict(k_values=4100), 5), (dict(q_dtype=2), 2)])
+def test_weighted_decode_refuses(change, status):
+    from flashspec_b200 import _lib
+
+    a = decode_args()
+    for k, v in change.items():
+        setattr(a, k, v)
+    assert _lib.load().fs_paged_decode_weights(C.byref(a), 4096, None) == status
+
+
+def test_weighted_decode_refuses_missing_or_unaligned_weights():
+    from flashspec_b200 import _lib
+
+    lib = _lib.load()
+    assert lib.fs_paged_decode_weights(C.byref(decode_args()), None, None) == 1
+    assert lib.fs_paged_decode_weights(None, 4096, None) == 1
+    assert lib.fs_paged_decode_weights(C.byref(decode_args()), 4097, None) == 5
+    assert lib.fs_paged_decode_weights_workspace_size(C.byref(decode_args()), None, None) == 1
+
+
+def evict_args():
+    from flashspec_b200 import _lib
+
+    a = _lib.FsEvictArgs()
+    a.batch, a.kv_heads, a.head_dim, a.page_size, a.table_cols, a.max_seq_len = 2, 4, 128, 16, 8, 128
+    a.budget, a.recent, a.sinks, a.num_pages = 32, 8, 4, 20
+    a.block_table = a.lengths = a.k_values = a.v_values = a.k_scale = a.v_scale = a.k_zero = a.v_zero = 4096
+    a.weights = a.weights_out = a.kept = 4096
+    a.new_lengths = 8192
+    return a
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(budget=0), 1), (dict(recent=30), 1), (dict(sinks=-1), 1), (dict(kv_format=2), 1), (dict(k_zero=None), 1),
+    (dict(kept=None), 1), (dict(new_lengths=4096), 1), (dict(page_size=65), 2), (dict(head_dim=72), 2),
+    (dict(page_size=64, head_dim=256), 2), (dict(k_values=4104), 5), (dict(weights=4098), 5),
+    (dict(table_cols=1 << 28), 2), (dict(num_pages=0), 1)])
+def test_evict_refuses(change, status):
+    from flashspec_b200 import _lib
+
+    a, n = evict_args(), C.c_size_t(0)
+    for k, v in change.items():
+        setattr(a, k, v)
+    assert _lib.load().fs_evict_tokens(C.byref(a), None) == status
+    assert _lib.load().fs_evict_workspace_size(C.byref(a), C.byref(n)) == status
+
+
+def test_evict_workspace():
+    from flashspec_b200 import _lib
+
+    lib, a, n = _lib.load(), evict_args(), C.c_size_t(0)
+    assert lib.fs_evict_workspace_size(C.byref(a), C.byref(n)) == 0 and n.value == 0
+    a.table_cols, a.max_seq_len = 393216 // 16, 393216
+    assert lib.fs_evict_workspace_size(C.byref(a), C.byref(n)) == 0 and n.value == 0
+    a.table_cols, a.max_seq_len = 393216 // 16 + 16, 393216 + 256
+    assert lib.fs_evict_workspace_size(C.byref(a), C.byref(n)) == 0 and n.value == 2 * 4 * (393216 + 256) * 4
+    assert lib.fs_evict_tokens(C.byref(a), None) == 4  # FS_ERR_WORKSPACE
