@@ -324,6 +324,14 @@ struct QueryFrag {
 // The PV MMAs multiply P by 1024 + u (the exact fp16 form of the stored byte) rather than
 // by u - zp; z_run collects this thread's share of sum_t P16[g][t] * (1024 + zp_page) for
 // query row g, and fold_zero_point() subtracts it once, when the warp's pages are done.
+// kWts keeps more of the output's precision on long flat contexts: there P V is a small
+// difference of large sums of P * (1024 + u) (off by about n 1.5e-6 of itself after n
+// tokens), and p * V scale can fall below fp16's normal range (0.039 of the output at 131072
+// tokens).  So V's zero point comes off before the MMA, and the running maximum m_run is that
+// of score + log2(V scale): P = 2^(t - m_run) * scale * 2^14 uses fp16's range from the top
+// whatever the scale, while l_run keeps sum 2^(t - m_run) in fp32 (at most 2^100 a token).
+constexpr float kWtsTop = 16384.f;
+
 struct WarpState {
   float m_run, l_run, z_run;
   float acc[8][4];
@@ -338,7 +346,15 @@ struct WarpState {
   }
   // acc[.][0|2] belong to query 2c and acc[.][1|3] to query 2c+1, whose corrections sit
   // (summed over the 4 lanes of a row) in lanes 8c and 8c+4.
+  template <bool kWts>
   __device__ __forceinline__ void fold_zero_point(int lane) {
+    if (kWts) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[i][k] *= 1.f / kWtsTop;
+      return;
+    }
     float z = z_run;
     z += __shfl_xor_sync(0xffffffffu, z, 1);
     z += __shfl_xor_sync(0xffffffffu, z, 2);
@@ -442,6 +458,11 @@ __device__ __forceinline__ void consume_page(uint32_t sbase, const StageOffsets&
     *reinterpret_cast<float2*>(srow + 8 + 2 * c) = make_float2(t[2], t[3]);
   }
   float mx = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+  if (kWts) {  // the reference point covers V's scale too (WarpState)
+    mx = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) mx = fmaxf(mx, t[k] + fmaxf(lg2_approx(vk[k]), -100.f));
+  }
   mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
   mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
   if (__any_sync(0xffffffffu, mx > ws.m_run)) {
@@ -464,9 +485,13 @@ __device__ __forceinline__ void consume_page(uint32_t sbase, const StageOffsets&
 #pragma unroll
   for (int k = 0; k < 4; ++k) pr[k] = ex2_approx(t[k] - ws.m_run);
   ws.l_run += (pr[0] + pr[1]) + (pr[2] + pr[3]);
+  if (kWts) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) vk[k] *= kWtsTop;
+  }
   const uint32_t pb0 = pack_half2(pr[0] * vk[0], pr[1] * vk[1]);
   const uint32_t pb1 = pack_half2(pr[2] * vk[2], pr[3] * vk[3]);
-  {  // the zero point, applied per page to the exact fp16 P values the MMAs see
+  if (!kWts) {  // the zero point, applied per page to the exact fp16 P values the MMAs see
     const float2 p01 = __half22float2(*reinterpret_cast<const __half2*>(&pb0));
     const float2 p23 = __half22float2(*reinterpret_cast<const __half2*>(&pb1));
     ws.z_run = fmaf(1024.f + (float)si.vz, (p01.x + p01.y) + (p23.x + p23.y), ws.z_run);
@@ -474,12 +499,19 @@ __device__ __forceinline__ void consume_page(uint32_t sbase, const StageOffsets&
   // ---- O += P V: vr(chunk i, tokens 0-7 | 8-15) hold bytes
   // [V[2c][d], V[2c][d+1], V[2c+1][d], V[2c+1][d+1]] with d = 16i + 2g; the stored byte
   // is u - 128, so XOR 0x80 gives u and PRMT with exponent bytes 0x64 the fp16 1024 + u.
+  // kWts subtracts 1024 + zp from it (exact: integers below 2048), see WarpState.
+  const __half2 vbase = __half2half2(__uint2half_rn(1024u + si.vz));
+  auto v_exact = [&](uint32_t x) -> uint32_t {
+    if (!kWts) return x;
+    const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&x), vbase);
+    return *reinterpret_cast<const uint32_t*>(&d);
+  };
 #pragma unroll
   for (int i2 = 0; i2 < 8; ++i2) {
     const uint32_t x0 = vr[4 * (i2 >> 1) + 2 * (i2 & 1)] ^ 0x80808080u;
     const uint32_t x1 = vr[4 * (i2 >> 1) + 2 * (i2 & 1) + 1] ^ 0x80808080u;
-    mma_16816(ws.acc[i2], prmt(x0, kMagic, 0x5240u), prmt(x0, kMagic, 0x5341u), prmt(x1, kMagic, 0x5240u),
-              prmt(x1, kMagic, 0x5341u), pb0, pb1);
+    mma_16816(ws.acc[i2], v_exact(prmt(x0, kMagic, 0x5240u)), v_exact(prmt(x0, kMagic, 0x5341u)),
+              v_exact(prmt(x1, kMagic, 0x5240u)), v_exact(prmt(x1, kMagic, 0x5341u)), pb0, pb1);
   }
 }
 
@@ -733,7 +765,7 @@ __global__ void __launch_bounds__((kW + 1) * 32, kMinBlocks)
     }
     ws.l_run += __shfl_xor_sync(0xffffffffu, ws.l_run, 1);
     ws.l_run += __shfl_xor_sync(0xffffffffu, ws.l_run, 2);
-    ws.fold_zero_point(lane);
+    ws.fold_zero_point<kWts>(lane);
   }
 
   // ---- merge the consumer warps through shared memory ---------------------------
@@ -1368,7 +1400,7 @@ __global__ void __maxnreg__(kMaxRegs)
     if (f + 1 != pair_end && j + 1 != len_w) continue;
 
     // ---- close the piece ------------------------------------------------------------
-    ws.fold_zero_point(lane);
+    ws.fold_zero_point<kWts>(lane);
     float l = ws.l_run;
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
