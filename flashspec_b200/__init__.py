@@ -16,6 +16,7 @@ from .attention import (BACKENDS, fused_dequant_attention_cuda, get_backend, mer
                         paged_quant_attention_cuda, paged_quant_attention_weights_cuda, register_backend,
                         reset_workspaces)
 from .evict import evict_tokens_cuda
+from .latent import LatentKVCache, latent_attention_cuda
 from .paged import PagedKVAllocator, PagedKVCache
 from .paged import paged_cache_symmetric
 from .quant import (QuantizedTensor, SymQuantizedTensor, build_compression_stats, dequantize_int8_per_block,
@@ -25,6 +26,7 @@ from .tree import tree_verify_attention_cuda
 
 __all__ = [
     "BACKENDS",
+    "LatentKVCache",
     "PagedKVAllocator",
     "PagedKVCache",
     "QuantizedTensor",
@@ -35,6 +37,7 @@ __all__ = [
     "evict_tokens_cuda",
     "fused_dequant_attention_cuda",
     "get_backend",
+    "latent_attention_cuda",
     "merge_partials",
     "paged_quant_attention_cuda",
     "paged_quant_attention_weights_cuda",

@@ -188,6 +188,61 @@ class FsEvictArgs(C.Structure):
     ]
 
 
+class FsLatentAppendArgs(C.Structure):
+    _fields_ = [
+        ("latent", C.c_void_p),
+        ("rope", C.c_void_p),
+        ("latent_stride_b", C.c_int64),
+        ("latent_stride_t", C.c_int64),
+        ("rope_stride_b", C.c_int64),
+        ("rope_stride_t", C.c_int64),
+        ("dtype", C.c_int32),
+        ("batch", C.c_int32),
+        ("tokens", C.c_int32),
+        ("latent_dim", C.c_int32),
+        ("rope_dim", C.c_int32),
+        ("page_size", C.c_int32),
+        ("table_cols", C.c_int32),
+        ("num_pages", C.c_int64),
+        ("block_table", C.c_void_p),
+        ("lengths", C.c_void_p),
+        ("counts", C.c_void_p),
+        ("values", C.c_void_p),
+        ("scale", C.c_void_p),
+        ("ropes", C.c_void_p),
+        ("held", C.c_void_p),
+        ("new_lengths", C.c_void_p),
+        ("device_status", C.c_void_p),
+    ]
+
+
+class FsLatentArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p),
+        ("q_rope", C.c_void_p),
+        ("out", C.c_void_p),
+        ("dtype", C.c_int32),
+        ("batch", C.c_int32),
+        ("tokens", C.c_int32),
+        ("heads", C.c_int32),
+        ("latent_dim", C.c_int32),
+        ("rope_dim", C.c_int32),
+        ("page_size", C.c_int32),
+        ("table_cols", C.c_int32),
+        ("max_seq_len", C.c_int32),
+        ("sm_scale", C.c_float),
+        ("num_pages", C.c_int64),
+        ("values", C.c_void_p),
+        ("scale", C.c_void_p),
+        ("ropes", C.c_void_p),
+        ("block_table", C.c_void_p),
+        ("lengths", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t),
+        ("device_status", C.c_void_p),
+    ]
+
+
 SIGNATURES = {
     "fs_abi_version": (C.c_int, []),
     "fs_status_string": (C.c_char_p, [C.c_int]),
@@ -201,6 +256,9 @@ SIGNATURES = {
     "fs_paged_decode_weights": (C.c_int, [C.POINTER(FsDecodeArgs), C.c_void_p, C.c_void_p]),
     "fs_evict_workspace_size": (C.c_int, [C.POINTER(FsEvictArgs), C.POINTER(C.c_size_t)]),
     "fs_evict_tokens": (C.c_int, [C.POINTER(FsEvictArgs), C.c_void_p]),
+    "fs_latent_append": (C.c_int, [C.POINTER(FsLatentAppendArgs), C.c_void_p]),
+    "fs_latent_workspace_size": (C.c_int, [C.POINTER(FsLatentArgs), C.POINTER(C.c_size_t)]),
+    "fs_latent_attention": (C.c_int, [C.POINTER(FsLatentArgs), C.c_void_p]),
     "fs_merge_partials": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_int64, C.c_void_p,
                                     C.c_int32, C.c_void_p]),
     "fs_quantize_blocks": (C.c_int, [C.POINTER(FsQuantizeArgs), C.c_void_p]),

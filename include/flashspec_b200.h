@@ -192,6 +192,67 @@ typedef struct FsEvictArgs {
 int fs_evict_workspace_size(const FsEvictArgs* args, size_t* bytes);
 int fs_evict_tokens(const FsEvictArgs* args, void* stream);
 
+/* Latent cache (keys and values of all heads from one shared vector a token), paged:
+ *   values int8 [P, page, latent_dim]  rint(c / s), s = max(absmax / 127, 1e-8) per token
+ *   scale  fp32 [P, page]
+ *   ropes  16 bit [P, page, rope_dim]  the rotary part of the key, as it is
+ * block_table int64 [batch, table_cols] (-1 = unallocated), lengths int64 [batch].
+ * latent_dim 128 / 256 / 512, rope_dim 32 / 64, page 16 / 32 / 64 / 128, dtype (of ropes and
+ * of everything that goes in and out) FS_F16 or FS_BF16.  No counterpart in the reference.
+ *
+ * fs_latent_append: writes counts[b] (NULL: all `tokens`) new tokens of latent
+ * [batch, tokens, latent_dim] and rope [batch, tokens, rope_dim] (element strides below,
+ * innermost 1) to the positions behind lengths[b], and lengths + counts to new_lengths (not
+ * the array `lengths`).  The pages must be in the table; a token without one is dropped and
+ * FS_DEV_BAD_PAGE reported.  held (optional) receives the values that the cache now stands
+ * for, codes times scale in dtype [batch, tokens, latent_dim], zeros behind counts[b]. */
+typedef struct FsLatentAppendArgs {
+  const void* latent;
+  const void* rope;
+  int64_t latent_stride_b, latent_stride_t, rope_stride_b, rope_stride_t;
+  int32_t dtype;
+  int32_t batch, tokens, latent_dim, rope_dim, page_size, table_cols;
+  int64_t num_pages;
+  const int64_t* block_table;
+  const int64_t* lengths;
+  const int64_t* counts;
+  int8_t* values;
+  float* scale;
+  void* ropes;
+  void* held;
+  int64_t* new_lengths;
+  uint32_t* device_status;
+} FsLatentAppendArgs;
+int fs_latent_append(const FsLatentAppendArgs* args, void* stream);
+
+/* Absorbed attention over the latent cache: for the last `tokens` positions of each request,
+ *   score(t, h, j) = sm_scale (scale_j q[b, t, h] . values_j + q_rope[b, t, h] . ropes_j)
+ *   out[b, t, h]   = sum_j softmax_j(score) scale_j values_j
+ * over the tokens j < lengths[b] - tokens + t + 1 (query t is the token at that end; none:
+ * zeros).  q and out [batch, tokens, heads, latent_dim], q_rope [batch, tokens, heads,
+ * rope_dim], contiguous, 16-byte aligned.  Unallocated pages are skipped.  At most 4096
+ * requests and 2^20 rows (tokens * heads) a request.  Workspace: fs_latent_workspace_size
+ * bytes, 256-byte aligned, any contents. */
+typedef struct FsLatentArgs {
+  const void* q;
+  const void* q_rope;
+  void* out;
+  int32_t dtype;
+  int32_t batch, tokens, heads, latent_dim, rope_dim, page_size, table_cols, max_seq_len;
+  float sm_scale;
+  int64_t num_pages;
+  const int8_t* values;
+  const float* scale;
+  const void* ropes;
+  const int64_t* block_table;
+  const int64_t* lengths;
+  void* workspace;
+  size_t workspace_bytes;
+  uint32_t* device_status; /* optional device word receiving FS_DEV_BAD_PAGE */
+} FsLatentArgs;
+int fs_latent_workspace_size(const FsLatentArgs* args, size_t* bytes);
+int fs_latent_attention(const FsLatentArgs* args, void* stream);
+
 /* Log-sum-exp merge of n_parts partial results (split-K partials, or per-GPU
  * shards gathered over NVLink).  Part i's O is o_parts + i*S ([rows, head_dim] fp32)
  * and its LSE lse_parts + i*S' ([rows] fp32), where S = part_stride and S' =
