@@ -16,7 +16,7 @@ from .attention import (BACKENDS, fused_dequant_attention_cuda, get_backend, mer
                         paged_quant_attention_cuda, paged_quant_attention_weights_cuda, register_backend,
                         reset_workspaces)
 from .evict import evict_tokens_cuda
-from .latent import LatentKVCache, latent_attention_cuda
+from .latent import LatentKVCache, latent_attention_cuda, latent_prefill_attention_cuda
 from .paged import PagedKVAllocator, PagedKVCache
 from .paged import paged_cache_symmetric
 from .quant import (QuantizedTensor, SymQuantizedTensor, build_compression_stats, dequantize_int8_per_block,
@@ -38,6 +38,7 @@ __all__ = [
     "fused_dequant_attention_cuda",
     "get_backend",
     "latent_attention_cuda",
+    "latent_prefill_attention_cuda",
     "merge_partials",
     "paged_quant_attention_cuda",
     "paged_quant_attention_weights_cuda",

@@ -17,7 +17,7 @@ CSRC = PKG / "csrc"
 BUILD = ROOT / "_build"
 LIB = PKG / "libflashspec_b200.so"
 SOURCES = ["decode.cu", "decode_generic.cu", "quant.cu", "noalloc.cu", "exchange.cu", "probe.cu", "tree.cu",
-           "weights.cu", "evict.cu", "latent.cu"]
+           "weights.cu", "evict.cu", "latent.cu", "latent_prefill.cu"]
 HEADERS = ["ptx.cuh", "common.h", "generic.h", "weights.h", "xwords.cuh",
            "quant_math.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

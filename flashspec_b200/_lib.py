@@ -243,6 +243,26 @@ class FsLatentArgs(C.Structure):
     ]
 
 
+class FsLatentPrefillArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p),
+        ("kv", C.c_void_p),
+        ("k_rope", C.c_void_p),
+        ("out", C.c_void_p),
+        ("q_offsets", C.c_void_p),
+        ("k_offsets", C.c_void_p),
+        ("q_rows", C.c_int64),
+        ("k_rows", C.c_int64),
+        ("dtype", C.c_int32),
+        ("batch", C.c_int32),
+        ("heads", C.c_int32),
+        ("nope_dim", C.c_int32),
+        ("rope_dim", C.c_int32),
+        ("value_dim", C.c_int32),
+        ("sm_scale", C.c_float),
+    ]
+
+
 SIGNATURES = {
     "fs_abi_version": (C.c_int, []),
     "fs_status_string": (C.c_char_p, [C.c_int]),
@@ -259,6 +279,7 @@ SIGNATURES = {
     "fs_latent_append": (C.c_int, [C.POINTER(FsLatentAppendArgs), C.c_void_p]),
     "fs_latent_workspace_size": (C.c_int, [C.POINTER(FsLatentArgs), C.POINTER(C.c_size_t)]),
     "fs_latent_attention": (C.c_int, [C.POINTER(FsLatentArgs), C.c_void_p]),
+    "fs_latent_prefill": (C.c_int, [C.POINTER(FsLatentPrefillArgs), C.c_void_p]),
     "fs_merge_partials": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_int64, C.c_void_p,
                                     C.c_int32, C.c_void_p]),
     "fs_quantize_blocks": (C.c_int, [C.POINTER(FsQuantizeArgs), C.c_void_p]),

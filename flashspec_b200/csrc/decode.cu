@@ -452,6 +452,11 @@ __device__ __forceinline__ void consume_page(uint32_t sbase, const StageOffsets&
     if (pos0 + 2 * c + 1 >= len_eff) t[1] = -INFINITY;
     if (pos0 + 8 + 2 * c >= len_eff) t[2] = -INFINITY;
     if (pos0 + 9 + 2 * c >= len_eff) t[3] = -INFINITY;
+    if (kWts) {  // a masked token's scale may be anything
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (pos0 + 8 * (k >> 1) + 2 * c + (k & 1) >= len_eff) vk[k] = 0.f;
+    }
   }
   if (kWts && srow != nullptr) {
     *reinterpret_cast<float2*>(srow + 2 * c) = make_float2(t[0], t[1]);

@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(kGW * 32) decode_generic_kernel(const GenericP
             l[g] = l[g] * alpha + pr;
 #pragma unroll
             for (int j = 0; j < kDpl; ++j) acc[g][j] *= alpha;
-            ps[g * 64 + lane] = pr * vsc;
+            ps[g * 64 + lane] = kWts && !valid ? 0.f : pr * vsc;  // a masked token's scale may be anything
           }
         }
         __syncwarp();

@@ -7,7 +7,10 @@ part r that all heads share.  ``LatentKVCache`` holds them in pages;
 * ``LatentKVCache.append`` writes new tokens,
 * ``latent_attention_cuda`` is the absorbed form for decoding: the queries are multiplied
   into the latent space by the caller (q_latent = q_nope W_uk of the head), the result comes
-  back as a latent that the caller multiplies by W_uv.
+  back as a latent that the caller multiplies by W_uv;
+* ``latent_prefill_attention_cuda`` is the expanded form for prompts, over every head's keys
+  and values as the caller expanded them (``append(..., return_held=True)`` gives the latents
+  that the cache stands for).
 
 The reference has no counterpart.
 """
@@ -207,6 +210,58 @@ def latent_attention_cuda(q_latent: torch.Tensor, q_rope: torch.Tensor, cache: L
         a.workspace, a.workspace_bytes = ws.data_ptr(), need.value
         _lib.check(lib.fs_latent_attention(C.byref(a), stream_of(device)), "fs_latent_attention")
     return out.squeeze(1) if single else out
+
+
+def latent_prefill_attention_cuda(q: torch.Tensor, kv: torch.Tensor, k_rope: torch.Tensor, q_offsets: torch.Tensor,
+                                  k_offsets: torch.Tensor, *, sm_scale: Optional[float] = None,
+                                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Expanded latent attention of packed prompts, causal, aligned at the end.
+
+    q [Nq, H, dn + dr]; kv [Nk, H, dn + dv], every head's key part and value expanded from the
+    latents; k_rope [Nk, dr], the rotary key that all heads share (fp16 or bf16, one dtype).
+    Request b's queries are rows q_offsets[b] : q_offsets[b + 1] of q, its keys and values rows
+    k_offsets[b] : k_offsets[b + 1] (int64 [B + 1] on the device, ascending); its query i of nq
+    sees keys j <= i + nk - nq, so a chunk of new tokens sees a cached prefix and, in order,
+    itself; a query that sees no key gives zeros.  dn and dv 64 or 128, dr 32 or 64 (dr is read
+    from k_rope, dn from q).  Returns out [Nq, H, dv]; a given ``out`` keeps the rows that no
+    request covers, otherwise those are zeros.  sm_scale defaults to 1 / sqrt(dn + dr)."""
+    require_cuda(q, "q")
+    if q.ndim != 3 or kv.ndim != 3 or k_rope.ndim != 2:
+        raise ValueError("q must be [rows, heads, dim], kv [rows, heads, dim] and k_rope [rows, dim]")
+    nq, h, dq = (int(x) for x in q.shape)
+    nk, dr = int(k_rope.shape[0]), int(k_rope.shape[1])
+    dn = dq - dr
+    dv = int(kv.shape[2]) - dn
+    if int(kv.shape[0]) != nk or int(kv.shape[1]) != h or h <= 0:
+        raise ValueError("kv must have k_rope's rows and q's heads")
+    if dn not in (64, 128) or dv not in (64, 128) or dr not in ROPE_DIMS:
+        raise ValueError("nope and value dims must be 64 or 128, the rope dim 32 or 64")
+    if q.dtype not in (torch.float16, torch.bfloat16) or kv.dtype != q.dtype or k_rope.dtype != q.dtype:
+        raise ValueError("q, kv and k_rope must be fp16 or bf16, all of one dtype")
+    device = q.device
+    if any(t.device != device for t in (kv, k_rope, q_offsets, k_offsets)):
+        raise RuntimeError("q, kv, k_rope and the offsets must be on one CUDA device")
+    if q_offsets.ndim != 1 or tuple(q_offsets.shape) != tuple(k_offsets.shape) or int(q_offsets.shape[0]) < 2:
+        raise ValueError("q_offsets and k_offsets must be [batch + 1]")
+    if out is not None:
+        if tuple(out.shape) != (nq, h, dv) or out.dtype != q.dtype or not out.is_contiguous() or out.data_ptr() % 16:
+            raise ValueError("out must be a contiguous, 16-byte aligned [Nq, H, dv] tensor of q's dtype")
+        if out.device != device:
+            raise RuntimeError("out must be on q's CUDA device")
+    qc, kvc, rc = _aligned(q), _aligned(kv), _aligned(k_rope)
+    qo, ko = _i64(q_offsets), _i64(k_offsets)
+    with torch.cuda.device(device):
+        if out is None:
+            out = torch.zeros((nq, h, dv), dtype=q.dtype, device=device)
+        a = _lib.FsLatentPrefillArgs()
+        a.q, a.kv, a.k_rope, a.out = qc.data_ptr(), kvc.data_ptr(), rc.data_ptr(), out.data_ptr()
+        a.q_offsets, a.k_offsets = qo.data_ptr(), ko.data_ptr()
+        a.q_rows, a.k_rows = nq, nk
+        a.dtype, a.batch, a.heads = _dtype(q), int(qo.shape[0]) - 1, h
+        a.nope_dim, a.rope_dim, a.value_dim = dn, dr, dv
+        a.sm_scale = 1.0 / math.sqrt(dq) if sm_scale is None else float(sm_scale)
+        _lib.check(_lib.load().fs_latent_prefill(C.byref(a), stream_of(device)), "fs_latent_prefill")
+    return out
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:

@@ -253,6 +253,30 @@ typedef struct FsLatentArgs {
 int fs_latent_workspace_size(const FsLatentArgs* args, size_t* bytes);
 int fs_latent_attention(const FsLatentArgs* args, void* stream);
 
+/* Expanded latent attention for prompts: every head's keys and values, expanded from the
+ * latents by the caller, with one rotary key for all heads; `batch` requests packed one
+ * behind the other, request b's queries in rows q_offsets[b] .. q_offsets[b + 1] of q and its
+ * keys in rows k_offsets[b] .. of kv and k_rope; causal and aligned at the end: query i of nq
+ * sees the keys j <= i + nk - nq (none: zeros).
+ *   q [q_rows, heads, nope_dim + rope_dim]   kv [k_rows, heads, nope_dim + value_dim] (the
+ *   key's own part, then the value)   k_rope [k_rows, rope_dim]   out [q_rows, heads, value_dim]
+ * all dtype FS_F16 or FS_BF16, contiguous, 16-byte aligned; offsets int64 [batch + 1] on the
+ * device, ascending (offsets outside the rows are cut to them).  Rows of out that no request
+ * covers are left as they were.  nope_dim and value_dim 64 / 128, rope_dim 32 / 64; fewer
+ * than 2^30 rows. */
+typedef struct FsLatentPrefillArgs {
+  const void* q;
+  const void* kv;
+  const void* k_rope;
+  void* out;
+  const int64_t* q_offsets;
+  const int64_t* k_offsets;
+  int64_t q_rows, k_rows;
+  int32_t dtype, batch, heads, nope_dim, rope_dim, value_dim;
+  float sm_scale;
+} FsLatentPrefillArgs;
+int fs_latent_prefill(const FsLatentPrefillArgs* args, void* stream);
+
 /* Log-sum-exp merge of n_parts partial results (split-K partials, or per-GPU
  * shards gathered over NVLink).  Part i's O is o_parts + i*S ([rows, head_dim] fp32)
  * and its LSE lse_parts + i*S' ([rows] fp32), where S = part_stride and S' =

@@ -254,6 +254,21 @@ def test_captured_graphs_share_nothing():
         assert torch.allclose(w, 3 * ref_w, rtol=1e-6)
 
 
+@pytest.mark.parametrize("d,dtype", [(128, torch.float16), (64, torch.bfloat16)])
+def test_nothing_behind_the_length_is_used(d, dtype):
+    cache = make_cache(2, 2, d, [100, 39], 16, "symmetric", seed=20)
+    q = torch.randn((2, 4, d), generator=torch.Generator().manual_seed(12)).to(dtype).cuda()
+    w = torch.zeros((cache.k_quant.values.shape[0], 2, 16), device="cuda")
+    ref = check(q, cache, w)
+    for i, n in enumerate((100, 39)):
+        page = cache.block_table[i, n // 16]
+        cache.k_quant.scale[page, :, n % 16:] = float("nan")
+        cache.v_quant.scale[page, :, n % 16:] = float("inf")
+    w2 = torch.zeros_like(w)
+    out = fs().paged_quant_attention_weights_cuda(q, cache, w2)
+    assert torch.equal(out, ref) and torch.equal(w, w2)
+
+
 def test_refusals():
     cache = make_cache(1, 2, 128, [40], 16, "affine", seed=19)
     pages = cache.k_quant.values.shape[0]

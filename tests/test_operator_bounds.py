@@ -15,7 +15,8 @@ HEADER = Path(__file__).resolve().parents[1] / "include" / "flashspec_b200.h"
 def layouts():
     from flashspec_b200 import _lib
 
-    return {"FsEvictArgs": _lib.FsEvictArgs}
+    return {"FsEvictArgs": _lib.FsEvictArgs, "FsLatentAppendArgs": _lib.FsLatentAppendArgs,
+            "FsLatentArgs": _lib.FsLatentArgs, "FsLatentPrefillArgs": _lib.FsLatentPrefillArgs}
 
 
 def test_struct_layouts_match_c(tmp_path):
@@ -106,3 +107,59 @@ def test_evict_workspace():
     a.table_cols, a.max_seq_len = 393216 // 16 + 16, 393216 + 256
     assert lib.fs_evict_workspace_size(C.byref(a), C.byref(n)) == 0 and n.value == 2 * 4 * (393216 + 256) * 4
     assert lib.fs_evict_tokens(C.byref(a), None) == 4  # FS_ERR_WORKSPACE
+
+
+def latent_args():
+    from flashspec_b200 import _lib
+
+    a = _lib.FsLatentArgs()
+    a.q = a.q_rope = a.out = a.values = a.scale = a.ropes = a.block_table = a.lengths = 4096
+    a.batch, a.tokens, a.heads, a.latent_dim, a.rope_dim, a.page_size = 2, 1, 16, 512, 64, 64
+    a.table_cols, a.max_seq_len, a.num_pages, a.sm_scale = 4, 256, 10, 0.1
+    return a
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(q=None), 1), (dict(lengths=None), 1), (dict(tokens=0), 1), (dict(heads=0), 1), (dict(num_pages=0), 1),
+    (dict(dtype=2), 2), (dict(latent_dim=192), 2), (dict(rope_dim=16), 2), (dict(page_size=48), 2),
+    (dict(batch=4097), 2), (dict(tokens=1 << 17), 2), (dict(table_cols=1 << 26), 2), (dict(values=4104), 5),
+    (dict(q=4098), 5), (dict(scale=4097), 5)])
+def test_latent_attention_refuses(change, status):
+    from flashspec_b200 import _lib
+
+    a, n = latent_args(), C.c_size_t(0)
+    for k, v in change.items():
+        setattr(a, k, v)
+    assert _lib.load().fs_latent_attention(C.byref(a), None) == status
+    assert _lib.load().fs_latent_workspace_size(C.byref(a), C.byref(n)) == status
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(latent=None), 1), (dict(new_lengths=None), 1), (dict(new_lengths=4096), 1), (dict(tokens=0), 1),
+    (dict(dtype=2), 2), (dict(latent_dim=64), 2), (dict(held=4097), 5)])
+def test_latent_append_refuses(change, status):
+    from flashspec_b200 import _lib
+
+    a = _lib.FsLatentAppendArgs()
+    a.latent = a.rope = a.values = a.scale = a.ropes = a.block_table = a.lengths = 4096
+    a.new_lengths = 8192
+    a.batch, a.tokens, a.latent_dim, a.rope_dim, a.page_size, a.table_cols, a.num_pages = 1, 1, 512, 64, 64, 1, 1
+    for k, v in change.items():
+        setattr(a, k, v)
+    assert _lib.load().fs_latent_append(C.byref(a), None) == status
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(q=None), 1), (dict(kv=None), 1), (dict(q_offsets=None), 1), (dict(batch=0), 1), (dict(heads=0), 1),
+    (dict(q_rows=-1), 1), (dict(dtype=2), 2), (dict(nope_dim=96), 2), (dict(rope_dim=128), 2), (dict(value_dim=32), 2),
+    (dict(k_rope=4098), 5), (dict(out=4104), 5), (dict(k_rows=1 << 30), 2), (dict(q_rows=0), 0)])
+def test_latent_prefill_refuses(change, status):
+    from flashspec_b200 import _lib
+
+    a = _lib.FsLatentPrefillArgs()
+    a.q = a.kv = a.k_rope = a.out = a.q_offsets = a.k_offsets = 4096
+    a.q_rows = a.k_rows = 10
+    a.batch, a.heads, a.nope_dim, a.rope_dim, a.value_dim = 1, 2, 128, 64, 128
+    for k, v in change.items():
+        setattr(a, k, v)
+    assert _lib.load().fs_latent_prefill(C.byref(a), None) == status
