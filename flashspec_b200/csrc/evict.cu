@@ -41,7 +41,7 @@ constexpr int kBins = 2048;
 constexpr int kSelMaxCluster = 8;
 // keys of one CTA held in shared memory at most (192 KB); longer rows keep them in the workspace
 constexpr int kSelSmemKeys = 48 * 1024;
-constexpr int kSelKeysPerCta = 4096;  // keys a CTA should have before the row gets a larger cluster
+constexpr int kEvictFill = 296;  // CTAs that keep the GPU busy: two on each of 148 SMs
 
 struct EvictParams {
   const int64_t* table;
@@ -58,6 +58,7 @@ struct EvictParams {
   int64_t num_pages, max_seq_len;
   int Hkv, cols, page, D, budget, recent, sinks;
   int chunk_cap;  // keys of one CTA at most
+  int vec;        // pages of whole groups of four tokens, weights 16-byte aligned
   int sym;
 };
 
@@ -112,7 +113,7 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* warp_sums, 
 // kSmem: the keys live in shared memory, else in the workspace (each CTA in its own part).
 template <bool kSmem>
 __global__ void __launch_bounds__(kSelThreads) select_tokens_kernel(const EvictParams p) {
-  extern __shared__ uint32_t sel_smem[];
+  extern __shared__ __align__(16) uint32_t sel_smem[];
   __shared__ __align__(16) uint32_t hist[kBins];
   __shared__ uint32_t warp_sums[kSelThreads / 32];
   __shared__ uint32_t found[2];   // bin of the K-th key, keys above that bin
@@ -133,10 +134,26 @@ __global__ void __launch_bounds__(kSelThreads) select_tokens_kernel(const EvictP
   const int chunk = (n + 4 * C - 1) / (4 * C) * 4;  // <= chunk_cap
   const int c0 = min(rank * chunk, n), c1 = min(c0 + chunk, n);
   uint32_t* keys = kSmem ? sel_smem : p.keys + (size_t)blockIdx.x * p.chunk_cap;
-  for (int i = c0 + tid; i < c1; i += kSelThreads) {
-    const int lp = i / p.page;
-    const int64_t phys = page_at(p, b, lp);
-    keys[i - c0] = phys < 0 ? 0u : key_of(p.weights[(phys * p.Hkv + h) * p.page + (i - lp * p.page)]);
+  if (p.vec) {
+    // four positions of one page a thread, four independent groups in flight
+#pragma unroll 4
+    for (int i = c0 + 4 * tid; i < c1; i += 4 * kSelThreads) {
+      const int lp = i / p.page;
+      const int64_t phys = page_at(p, b, lp);
+      uint4 k = make_uint4(0u, 0u, 0u, 0u);
+      if (phys >= 0) {
+        const float4 w = *reinterpret_cast<const float4*>(p.weights + (phys * p.Hkv + h) * p.page + (i - lp * p.page));
+        k = make_uint4(key_of(w.x), key_of(w.y), key_of(w.z), key_of(w.w));
+      }
+      *reinterpret_cast<uint4*>(keys + (i - c0)) = k;  // the chunk is padded to whole groups
+    }
+  } else {
+#pragma unroll 4
+    for (int i = c0 + tid; i < c1; i += kSelThreads) {
+      const int lp = i / p.page;
+      const int64_t phys = page_at(p, b, lp);
+      keys[i - c0] = phys < 0 ? 0u : key_of(p.weights[(phys * p.Hkv + h) * p.page + (i - lp * p.page)]);
+    }
   }
 
   // ---- the K-th largest key T of the contested range, and how many equal to T stay
@@ -243,25 +260,124 @@ __global__ void __launch_bounds__(kSelThreads) select_tokens_kernel(const EvictP
   }
   // ---- no tokens behind the kept ones: positions -1, weights zero
   for (int i = count + rank * kSelThreads + tid; i < p.budget; i += C * kSelThreads) kept[i] = -1;
-  for (int64_t i = count + rank * kSelThreads + tid; i < cap; i += C * kSelThreads) {
-    const int64_t lp = i / p.page, phys = page_at(p, b, (int)lp);
-    if (phys >= 0) p.weights_out[(phys * p.Hkv + h) * p.page + (i - lp * p.page)] = 0.f;
+  if (p.vec) {  // whole groups of four behind the one that `count` falls into
+    for (int64_t i = (count & ~3) + 4 * (rank * kSelThreads + tid); i < cap; i += 4 * C * kSelThreads) {
+      const int lp = (int)(i / p.page);
+      const int64_t phys = page_at(p, b, lp);
+      if (phys < 0) continue;
+      float* dst = p.weights_out + (phys * p.Hkv + h) * p.page + (i - (int64_t)lp * p.page);
+      if (i >= count) {
+        *reinterpret_cast<float4*>(dst) = make_float4(0.f, 0.f, 0.f, 0.f);
+      } else {
+        for (int j = 0; j < 4; ++j)
+          if (i + j >= count) dst[j] = 0.f;
+      }
+    }
+  } else {
+    for (int64_t i = count + rank * kSelThreads + tid; i < cap; i += C * kSelThreads) {
+      const int lp = (int)(i / p.page);
+      const int64_t phys = page_at(p, b, lp);
+      if (phys >= 0) p.weights_out[(phys * p.Hkv + h) * p.page + (i - (int64_t)lp * p.page)] = 0.f;
+    }
   }
   cluster.sync();  // no CTA leaves while its counts may still be read
 }
 
-constexpr int kMoveWarps = 16;
+constexpr int kMoveWarps = 8;
 
-// One page of K or V in a warp's registers: kCh 16-byte chunks a lane, chunk c of lane l
-// being bytes [16 (32 c + l), ...) of the page's [page, D] block.
+// One page of K or V on its way through a warp: kCh 16-byte chunks a lane, chunk c of lane l
+// being bytes [16 (32 c + l), ...) of the page's [page, D] block.  The sources (page of the
+// pool and row in it, -1: zeros) are looked up a round ahead, behind the data loads of the
+// round before.
 template <int kCh, bool kSym>
-struct PageRegs {
-  uint4 raw[kCh];
-  float scale[kSym ? 1 : kCh];  // affine: scale and zero point of each chunk's source block
-  int16_t zero[kSym ? 1 : kCh];
-  float tok_scale[2];  // symmetric: scales of tokens `lane` and `lane + 32`
-  int64_t dst;         // block index of the destination, -1: nothing to write
+struct PageMove {
+  int sp[kCh], sr[kCh];              // source of each chunk
+  int tp[kSym ? 2 : 1], tr[kSym ? 2 : 1];  // symmetric: source of tokens `lane` and `lane + 32`
+  int dst;                           // page of the pool, -1: nothing to write
+
+  __device__ __forceinline__ void plan(const EvictParams& p, int b, const int32_t* kept, int pg, int npg, int lane) {
+    dst = -1;
+    if (pg >= npg) return;
+    const int rows = min(p.page, p.budget - pg * p.page);  // kept tokens of the page
+    bool stays = true;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int t = lane + 32 * u;
+      int src = -1;
+      if (t < rows) {
+        src = kept[pg * p.page + t];
+        stays = stays && src == pg * p.page + t;
+      }
+      if (kSym) tp[u] = src;
+    }
+    if (__all_sync(0xffffffffu, stays)) return;
+    dst = (int)page_at(p, b, pg);
+#pragma unroll
+    for (int c = 0; c < kCh; ++c) {
+      const int e = 16 * (32 * c + lane), t = e / p.D;
+      sp[c] = -1;
+      if (e < p.page * p.D && t < rows) {
+        const int src = kept[pg * p.page + t], lp = src / p.page;
+        sp[c] = (int)page_at(p, b, lp);
+        sr[c] = src - lp * p.page;
+      }
+    }
+    if (kSym) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (tp[u] < 0) continue;
+        const int lp = tp[u] / p.page;
+        tr[u] = tp[u] - lp * p.page;
+        tp[u] = (int)page_at(p, b, lp);
+      }
+    }
+  }
 };
+
+// 16 codes through (u - zp) * scale and the destination's rounding, bit for bit as dequant16
+// followed by quantize16_fast, with one multiplication for the two.  With x = RN(d s),
+// d = u - zp exact, the code is rint(clamp(RN(RN(x / S) + Z))).  ta = RN(d RN(s RN(1/S)) + Z)
+// is within |d s / S| (3 2^-24) + ulp(ta) / 2 of it; where ta lies in [0, 255] |d s / S| <
+// 511, so that is below 1.2e-4, and a ta farther than 2^-12 from a half-integer has the same
+// rint (and clamps the same way).  The others, 0.05% of them, take the exact path.
+__device__ __forceinline__ uint4 requantize16(uint4 raw, float scale, int16_t zp, float ratio, QParams q) {
+  const float base = __fadd_rn(8388608.0f, (float)zp);
+  const uint32_t w4[4] = {raw.x ^ 0x80808080u, raw.y ^ 0x80808080u, raw.z ^ 0x80808080u, raw.w ^ 0x80808080u};
+  constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23
+  uint32_t w[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    uint32_t bits[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float d = __fsub_rn(__uint_as_float(__byte_perm(w4[k], 0x4B000000u, 0x7540 | j)), base);
+      const float tc = fminf(fmaxf(__fmaf_rn(d, ratio, q.zp), 0.0f), 255.0f);
+      const float r = __fadd_rn(tc, kMagic);
+      const float off = __fsub_rn(tc, __fsub_rn(r, kMagic));
+      bits[j] = __float_as_uint(r);  // low byte = rint(tc)
+      if (fabsf(off) >= 0.5f - 2.44140625e-4f)
+        bits[j] = (uint32_t)(uint8_t)quantize_one_exact(__fmul_rn(d, scale), q) ^ 0x80u;
+    }
+    const uint32_t lo = __byte_perm(bits[0], bits[1], 0x0040), hi = __byte_perm(bits[2], bits[3], 0x0040);
+    w[k] = __byte_perm(lo, hi, 0x5410) ^ 0x80808080u;
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Smallest and largest byte of 16 codes, as the unsigned codes u = value + 128.  (u - zp)
+// times a positive scale is monotone, rounding included, so these give the chunk's extremes.
+__device__ __forceinline__ void minmax16(uint4 raw, int& lo, int& hi) {
+  const uint32_t w4[4] = {raw.x ^ 0x80808080u, raw.y ^ 0x80808080u, raw.z ^ 0x80808080u, raw.w ^ 0x80808080u};
+  uint32_t mn = 0x00ff00ffu, mx = 0u;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t a = w4[k] & 0x00ff00ffu, b = (w4[k] >> 8) & 0x00ff00ffu;
+    mn = __vimin3_u16x2(mn, a, b);
+    mx = __vimax3_u16x2(mx, a, b);
+  }
+  lo = min((int)(mn & 0xffffu), (int)(mn >> 16));
+  hi = max((int)(mx & 0xffffu), (int)(mx >> 16));
+}
 
 template <int kCh, int kPages, bool kSym>
 __global__ void __launch_bounds__(kMoveWarps * 32) move_tokens_kernel(const EvictParams p) {
@@ -277,75 +393,63 @@ __global__ void __launch_bounds__(kMoveWarps * 32) move_tokens_kernel(const Evic
   float* scale = p.scale[kv];
   int16_t* zero = p.zero[kv];
   const int per_round = C * kMoveWarps * kPages;
+  const int pg0 = (rank * kMoveWarps + warp) * kPages;
+  PageMove<kCh, kSym> mv[kPages];
+#pragma unroll
+  for (int q = 0; q < kPages; ++q) mv[q].plan(p, b, kept, pg0 + q, npg, lane);
   for (int r0 = 0; r0 < npg; r0 += per_round) {
-    PageRegs<kCh, kSym> regs[kPages];
+    uint4 raw[kPages][kCh];
+    float sc[kPages][kSym ? 2 : kCh];  // affine: of each chunk's source block; symmetric: of two tokens
+    int16_t zp[kPages][kSym ? 1 : kCh];
+    int64_t dst[kPages];
 #pragma unroll
     for (int q = 0; q < kPages; ++q) {
-      PageRegs<kCh, kSym>& g = regs[q];
-      const int pg = r0 + (rank * kMoveWarps + warp) * kPages + q;
-      g.dst = -1;
-      if (pg >= npg) continue;
-      const int rows = min(page, p.budget - pg * page);  // kept tokens of the page
-      bool stays = true;
-      for (int t = lane; t < rows; t += 32) stays = stays && kept[pg * page + t] == pg * page + t;
-      const int64_t phys = page_at(p, b, pg);
-      if (__all_sync(0xffffffffu, stays) || phys < 0) continue;
-      g.dst = phys * p.Hkv + h;
+      const PageMove<kCh, kSym>& m = mv[q];
+      dst[q] = m.dst < 0 ? -1 : (int64_t)m.dst * p.Hkv + h;
+      if (m.dst < 0) continue;
 #pragma unroll
       for (int c = 0; c < kCh; ++c) {
-        const int e = 16 * (32 * c + lane), t = e / D;
-        g.raw[c] = make_uint4(0u, 0u, 0u, 0u);
-        if (!kSym) g.scale[c] = 0.f, g.zero[c] = 128;  // an absent token dequantizes to 0
-        if (e < E && t < rows) {
-          const int src = kept[pg * page + t], lp = src / page;
-          const int64_t sp = page_at(p, b, lp);
-          if (sp >= 0) {
-            const int64_t blk = sp * p.Hkv + h;
-            g.raw[c] = *reinterpret_cast<const uint4*>(values + blk * E + (src - lp * page) * D + (e - t * D));
-            if (!kSym) g.scale[c] = scale[blk], g.zero[c] = zero[blk];
-          }
+        const int e = 16 * (32 * c + lane);
+        raw[q][c] = make_uint4(0u, 0u, 0u, 0u);
+        if (!kSym) sc[q][c] = 0.f, zp[q][c] = 128;  // an absent token dequantizes to 0
+        if (m.sp[c] >= 0) {
+          const int64_t blk = (int64_t)m.sp[c] * p.Hkv + h;
+          raw[q][c] = *reinterpret_cast<const uint4*>(values + blk * E + m.sr[c] * D + e % D);
+          if (!kSym) sc[q][c] = scale[blk], zp[q][c] = zero[blk];
         }
       }
       if (kSym) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int t = lane + 32 * u;
-          g.tok_scale[u] = 1.0e-8f;
-          if (t < rows) {
-            const int src = kept[pg * page + t], lp = src / page;
-            const int64_t sp = page_at(p, b, lp);
-            if (sp >= 0) g.tok_scale[u] = scale[(sp * p.Hkv + h) * page + (src - lp * page)];
-          }
-        }
+        for (int u = 0; u < 2; ++u)
+          sc[q][u] = m.tp[u] >= 0 ? scale[((int64_t)m.tp[u] * p.Hkv + h) * page + m.tr[u]] : 1.0e-8f;
       }
     }
+#pragma unroll
+    for (int q = 0; q < kPages; ++q) mv[q].plan(p, b, kept, r0 + per_round + pg0 + q, npg, lane);
     cluster.sync();  // all sources of this round are in registers
 #pragma unroll
     for (int q = 0; q < kPages; ++q) {
-      const PageRegs<kCh, kSym>& g = regs[q];
-      if (g.dst < 0) continue;
+      if (dst[q] < 0) continue;
+      int8_t* out = values + dst[q] * E;
       if (kSym) {
 #pragma unroll
         for (int c = 0; c < kCh; ++c) {
           const int e = 16 * (32 * c + lane);
-          if (e < E) *reinterpret_cast<uint4*>(values + g.dst * E + e) = g.raw[c];
+          if (e < E) *reinterpret_cast<uint4*>(out + e) = raw[q][c];
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u)
-          if (lane + 32 * u < page) scale[g.dst * page + lane + 32 * u] = g.tok_scale[u];
+          if (lane + 32 * u < page) scale[dst[q] * page + lane + 32 * u] = sc[q][u];
         continue;
       }
-      float mn = INFINITY, mx = -INFINITY, v[16];
+      float mn = INFINITY, mx = -INFINITY;
 #pragma unroll
       for (int c = 0; c < kCh; ++c) {
         if (16 * (32 * c + lane) >= E) continue;
-        dequant16(make_int4((int)g.raw[c].x, (int)g.raw[c].y, (int)g.raw[c].z, (int)g.raw[c].w), g.scale[c],
-                  g.zero[c], v);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          mn = fminf(mn, v[j]);
-          mx = fmaxf(mx, v[j]);
-        }
+        int lo, hi;
+        minmax16(raw[q][c], lo, hi);
+        mn = fminf(mn, dequant_one((int8_t)(lo - 128), sc[q][c], zp[q][c]));
+        mx = fmaxf(mx, dequant_one((int8_t)(hi - 128), sc[q][c], zp[q][c]));
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
@@ -353,27 +457,32 @@ __global__ void __launch_bounds__(kMoveWarps * 32) move_tokens_kernel(const Evic
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
       }
       const QParams qp = qparams_from_range(mn, mx);
+      const float rcp = __frcp_rn(qp.scale);
 #pragma unroll
       for (int c = 0; c < kCh; ++c) {
         const int e = 16 * (32 * c + lane);
-        if (e >= E) continue;
-        dequant16(make_int4((int)g.raw[c].x, (int)g.raw[c].y, (int)g.raw[c].z, (int)g.raw[c].w), g.scale[c],
-                  g.zero[c], v);
-        *reinterpret_cast<uint4*>(values + g.dst * E + e) = quantize16_fast(v, qp);
+        if (e < E)
+          *reinterpret_cast<uint4*>(out + e) =
+              requantize16(raw[q][c], sc[q][c], zp[q][c], __fmul_rn(sc[q][c], rcp), qp);
       }
       if (lane == 0) {
-        scale[g.dst] = qp.scale;
-        zero[g.dst] = (int16_t)qp.zp;
+        scale[dst[q]] = qp.scale;
+        zero[dst[q]] = (int16_t)qp.zp;
       }
     }
   }
 }
 
-// Cluster of a row of `tokens` positions, and the keys of one of its CTAs.
-static int select_cluster(int64_t tokens, int* chunk_cap) {
+// Cluster of a row of `tokens` positions, and the keys of one of its CTAs.  Rows that alone
+// fill the GPU take one CTA each; few long rows are spread, down to 2048 keys a CTA.
+static int select_cluster(int64_t tokens, int64_t rows, int* chunk_cap) {
   int C = 1;
-  while (C < kSelMaxCluster && tokens > (int64_t)C * kSelKeysPerCta) C *= 2;
+  while (C < kSelMaxCluster && rows * C < kEvictFill && tokens > (int64_t)C * 2048) C *= 2;
   *chunk_cap = (int)((tokens + 4 * C - 1) / (4 * C) * 4);
+  while (C < kSelMaxCluster && *chunk_cap > kSelSmemKeys) {  // keep the keys in shared memory
+    C *= 2;
+    *chunk_cap = (int)((tokens + 4 * C - 1) / (4 * C) * 4);
+  }
   return C;
 }
 
@@ -393,6 +502,7 @@ static int evict_check(const FsEvictArgs* a) {
   if (a->page_size <= 0 || a->page_size > 64 || a->head_dim <= 0 || a->head_dim % 16 ||
       a->page_size * (a->head_dim + 16) > 12 * 1024)
     return FS_ERR_UNSUPPORTED;
+  if (a->num_pages >= (1ll << 31)) return FS_ERR_UNSUPPORTED;
   if ((int64_t)a->batch * a->kv_heads * 2 * kSelMaxCluster >= (1ll << 31)) return FS_ERR_UNSUPPORTED;
   if ((int64_t)a->table_cols * a->page_size >= (1ll << 31) - 4 * kSelThreads) return FS_ERR_UNSUPPORTED;
   if ((reinterpret_cast<uintptr_t>(a->k_values) | reinterpret_cast<uintptr_t>(a->v_values)) & 15)
@@ -409,7 +519,7 @@ static int64_t evict_tokens_at_most(const FsEvictArgs* a) {
 
 static size_t evict_workspace(const FsEvictArgs* a) {
   int chunk = 0;
-  const int C = select_cluster(evict_tokens_at_most(a), &chunk);
+  const int C = select_cluster(evict_tokens_at_most(a), (int64_t)a->batch * a->kv_heads, &chunk);
   return chunk <= kSelSmemKeys ? 0 : (size_t)a->batch * a->kv_heads * C * chunk * 4;
 }
 
@@ -442,14 +552,14 @@ static int launch_move(const FsEvictArgs* a, const EvictParams& p, void* stream)
   const int npg = (a->budget + a->page_size - 1) / a->page_size;
   const int64_t rows = (int64_t)a->batch * a->kv_heads * 2;
   auto go = [&](auto kernel, int pages) {
-    // as many CTAs as one round of the row's pages takes, so that few rounds wait for each other
+    // few rows are spread over clusters, up to one round of their pages
     int C = 1;
-    while (C < 8 && npg > C * kMoveWarps * pages) C *= 2;
+    while (C < 8 && rows * C < 2 * kEvictFill && npg > C * kMoveWarps * pages) C *= 2;
     return launch_cluster(kernel, "token move kernel launch", rows, C, kMoveWarps * 32, 0, p, stream);
   };
-  if (chunks <= 1) return go(move_tokens_kernel<1, 4, kSym>, 4);
-  if (chunks <= 2) return go(move_tokens_kernel<2, 4, kSym>, 4);
-  if (chunks <= 4) return go(move_tokens_kernel<4, 2, kSym>, 2);
+  if (chunks <= 1) return go(move_tokens_kernel<1, 2, kSym>, 2);
+  if (chunks <= 2) return go(move_tokens_kernel<2, 2, kSym>, 2);
+  if (chunks <= 4) return go(move_tokens_kernel<4, kSym ? 2 : 1, kSym>, kSym ? 2 : 1);
   if (chunks <= 8) return go(move_tokens_kernel<8, 1, kSym>, 1);
   if (chunks <= 16) return go(move_tokens_kernel<16, 1, kSym>, 1);
   return go(move_tokens_kernel<24, 1, kSym>, 1);
@@ -496,7 +606,8 @@ int fs_evict_tokens(const FsEvictArgs* a, void* stream) {
   p.recent = a->recent;
   p.sinks = a->sinks;
   p.sym = a->kv_format == FS_KV_SYMMETRIC;
-  const int C = select_cluster(evict_tokens_at_most(a), &p.chunk_cap);
+  p.vec = a->page_size % 4 == 0 && ((reinterpret_cast<uintptr_t>(a->weights) | reinterpret_cast<uintptr_t>(a->weights_out)) & 15) == 0;
+  const int C = select_cluster(evict_tokens_at_most(a), (int64_t)a->batch * a->kv_heads, &p.chunk_cap);
   const int64_t rows = (int64_t)a->batch * a->kv_heads;
   int st;
   if (need > 0) {
