@@ -43,6 +43,12 @@ constexpr int kSelMaxCluster = 8;
 constexpr int kSelSmemKeys = 48 * 1024;
 constexpr int kEvictFill = 296;  // CTAs that keep the GPU busy: two on each of 148 SMs
 
+// Division by a page's tokens or a head's dims: a shift where it is a power of two.
+struct Divisor {
+  int d, shift;  // shift < 0: not a power of two
+  __device__ __forceinline__ int quot(int x) const { return shift >= 0 ? x >> shift : x / d; }
+};
+
 struct EvictParams {
   const int64_t* table;
   const int64_t* lengths;
@@ -56,6 +62,7 @@ struct EvictParams {
   float* scale[2];
   int16_t* zero[2];
   int64_t num_pages, max_seq_len;
+  Divisor by_page, by_dim;
   int Hkv, cols, page, D, budget, recent, sinks;
   int chunk_cap;  // keys of one CTA at most
   int vec;        // pages of whole groups of four tokens, weights 16-byte aligned
@@ -121,16 +128,17 @@ __global__ void __launch_bounds__(kSelThreads) select_tokens_kernel(const EvictP
   cg::cluster_group cluster = cg::this_cluster();
   const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int row = blockIdx.x / C, b = row / p.Hkv, h = row % p.Hkv;
-  const int tid = threadIdx.x;
-  const int64_t cap = (int64_t)p.cols * p.page;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int cap = p.cols * p.page;
   const int n = (int)live_tokens(p, b);
   const int count = min(n, p.budget);
   if (h == 0 && rank == 0 && tid == 0) p.new_lengths[b] = count;
   int32_t* kept = p.kept + (size_t)row * p.budget;
-  const int lo = n > p.budget ? p.sinks : 0, hi = n > p.budget ? n - p.recent : 0;  // the contested range
-  const int K = n > p.budget ? p.budget - p.sinks - p.recent : 0;
+  const bool cut = n > p.budget;
+  const int lo = p.sinks, hi = n - p.recent;  // the contested range of a row that is cut
+  const int K = cut ? p.budget - p.sinks - p.recent : 0;
 
-  // ---- the row's weights, as keys of positions [c0, c1)
+  // ---- the row's weights, as keys of positions [c0, c1); the chunk is padded to groups of four
   const int chunk = (n + 4 * C - 1) / (4 * C) * 4;  // <= chunk_cap
   const int c0 = min(rank * chunk, n), c1 = min(c0 + chunk, n);
   uint32_t* keys = kSmem ? sel_smem : p.keys + (size_t)blockIdx.x * p.chunk_cap;
@@ -138,41 +146,44 @@ __global__ void __launch_bounds__(kSelThreads) select_tokens_kernel(const EvictP
     // four positions of one page a thread, four independent groups in flight
 #pragma unroll 4
     for (int i = c0 + 4 * tid; i < c1; i += 4 * kSelThreads) {
-      const int lp = i / p.page;
+      const int lp = p.by_page.quot(i);
       const int64_t phys = page_at(p, b, lp);
       uint4 k = make_uint4(0u, 0u, 0u, 0u);
       if (phys >= 0) {
         const float4 w = *reinterpret_cast<const float4*>(p.weights + (phys * p.Hkv + h) * p.page + (i - lp * p.page));
         k = make_uint4(key_of(w.x), key_of(w.y), key_of(w.z), key_of(w.w));
       }
-      *reinterpret_cast<uint4*>(keys + (i - c0)) = k;  // the chunk is padded to whole groups
+      *reinterpret_cast<uint4*>(keys + (i - c0)) = k;
     }
   } else {
 #pragma unroll 4
     for (int i = c0 + tid; i < c1; i += kSelThreads) {
-      const int lp = i / p.page;
+      const int lp = p.by_page.quot(i);
       const int64_t phys = page_at(p, b, lp);
       keys[i - c0] = phys < 0 ? 0u : key_of(p.weights[(phys * p.Hkv + h) * p.page + (i - lp * p.page)]);
     }
   }
 
-  // ---- the K-th largest key T of the contested range, and how many equal to T stay
-  uint32_t T = 0xffffffffu, quota = 0;  // kept: key > T, and the first `quota` keys == T
-  const bool contest = K > 0;
-  if (contest) {
+  if (cut && K > 0) {
+    // ---- the K-th largest key T of the contested range, and how many equal to T stay
     uint32_t prefix = 0, need = (uint32_t)K;
     const int a0 = max(c0, lo), a1 = min(c1, hi);
 #pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
       const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
-      for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0u;
+      *reinterpret_cast<uint4*>(hist + 4 * tid) = make_uint4(0u, 0u, 0u, 0u);
       __syncthreads();
-      for (int i = a0 + tid; i < a1; i += kSelThreads) {
-        const uint32_t k = keys[i - c0];
-        if (pass == 0 || (k >> (shift + bits)) == prefix) atomicAdd(hist + ((k >> shift) & ((1u << bits) - 1)), 1u);
+#pragma unroll 2
+      for (int i = c0 + 4 * tid; i < c1; i += 4 * kSelThreads) {
+        const uint4 k4 = *reinterpret_cast<const uint4*>(keys + (i - c0));
+        const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (i + j >= a0 && i + j < a1 && (pass == 0 || (k[j] >> (shift + bits)) == prefix))
+            atomicAdd(hist + ((k[j] >> shift) & ((1u << bits) - 1)), 1u);
       }
       cluster.sync();  // every CTA's histogram is complete
-      // thread t sums bins [4t, 4t + 4) from the top over the cluster
+      // thread t sums bins [top, top + 4) over the cluster, the highest bins first
       const int top = kBins - 4 * (tid + 1);
       uint32_t v[4] = {0, 0, 0, 0};
       for (int r = 0; r < C; ++r) {
@@ -196,91 +207,106 @@ __global__ void __launch_bounds__(kSelThreads) select_tokens_kernel(const EvictP
       prefix = (prefix << bits) | found[0];
       need -= found[1];
     }
-    T = prefix;
-    quota = need;
+    const uint32_t T = prefix, quota = need;  // kept: key > T, and the first `quota` keys == T
+
+    // ---- each warp counts a contiguous part of the chunk, then numbers what it keeps
+    const int part = (chunk + 128 * (kSelThreads / 32) - 1) / (128 * (kSelThreads / 32)) * 128;
+    const int w0 = min(c0 + warp * part, c1), w1 = min(w0 + part, c1);
     uint32_t above = 0, equal = 0;
-    for (int i = a0 + tid; i < a1; i += kSelThreads) {
-      const uint32_t k = keys[i - c0];
-      above += k > T;
-      equal += k == T;
+    for (int i = w0 + 4 * lane; i < w1; i += 128) {
+      const uint4 k4 = *reinterpret_cast<const uint4*>(keys + (i - c0));
+      const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool in = i + j >= a0 && i + j < a1;
+        above += in && k[j] > T;
+        equal += in && k[j] == T;
+      }
     }
-    uint32_t total;
-    block_scan(above, warp_sums, &total);
-    if (tid == 0) counts[0] = total;
-    block_scan(equal, warp_sums, &total);
-    if (tid == 0) counts[1] = total;
-  }
-  cluster.sync();  // counts are written; every weight of the row has been read
-  uint32_t base_above = 0, base_equal = 0;
-  if (contest) {
+    above = __reduce_add_sync(0xffffffffu, above);
+    equal = __reduce_add_sync(0xffffffffu, equal);
+    uint32_t n_above, n_equal;
+    const uint32_t at_above = block_scan(lane == 31 ? above : 0u, warp_sums, &n_above);
+    const uint32_t at_equal = block_scan(lane == 31 ? equal : 0u, warp_sums, &n_equal);
+    // before this warp: the scan at the previous warp's last lane
+    uint32_t base_above = __shfl_sync(0xffffffffu, at_above, 31) - above;
+    uint32_t base_equal = __shfl_sync(0xffffffffu, at_equal, 31) - equal;
+    if (tid == 0) counts[0] = n_above, counts[1] = n_equal;
+    cluster.sync();  // counts are written
     for (int r = 0; r < rank; ++r) {
       const uint32_t* c = cluster.map_shared_rank(counts, r);
       base_above += c[0];
       base_equal += c[1];
     }
+    for (int i0 = w0; i0 < w1; i0 += 128) {
+      const int i = i0 + 4 * lane;
+      uint32_t k[4] = {0u, 0u, 0u, 0u}, packed = 0;  // above in the low half, equal in the high half
+      if (i < w1) {
+        const uint4 k4 = *reinterpret_cast<const uint4*>(keys + (i - c0));
+        k[0] = k4.x, k[1] = k4.y, k[2] = k4.z, k[3] = k4.w;
+      }
+      bool gt[4], eq[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool in = i + j >= a0 && i + j < a1;
+        gt[j] = in && k[j] > T;
+        eq[j] = in && k[j] == T;
+        packed += (gt[j] ? 1u : 0u) + (eq[j] ? 0x10000u : 0u);
+      }
+      if (!__any_sync(0xffffffffu, packed != 0u)) continue;
+      uint32_t incl = packed;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+      }
+      const uint32_t sum = __shfl_sync(0xffffffffu, incl, 31), at = incl - packed;
+      uint32_t a = base_above + (at & 0xffffu), e = base_equal + (at >> 16);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (gt[j] || (eq[j] && e < quota)) kept[lo + (int)(a + min(e, quota))] = i + j;
+        a += gt[j];
+        e += eq[j];
+      }
+      base_above += sum & 0xffffu;
+      base_equal += sum >> 16;
+    }
   }
+  // ---- the tokens that are kept anyway, and nothing behind them
+  for (int i = rank * kSelThreads + tid; i < p.budget; i += C * kSelThreads) {
+    if (!cut)
+      kept[i] = i < n ? i : -1;
+    else if (i < p.sinks)
+      kept[i] = i;
+    else if (i >= p.budget - p.recent)
+      kept[i] = n - (p.budget - i);
+  }
+  cluster.sync();  // `kept` is complete; every weight of the row has been read
 
-  // ---- number the kept tokens in order; four consecutive positions a thread
-  auto put = [&](int dst, int pos, uint32_t key) {
-    kept[dst] = pos;
-    const int lp = dst / p.page;
-    const int64_t phys = page_at(p, b, lp);
-    if (phys >= 0) p.weights_out[(phys * p.Hkv + h) * p.page + (dst - lp * p.page)] = weight_of(key);
+  // ---- the kept tokens' weights at their new places, zeros at the others
+  auto weight_at = [&](int dst) -> float {
+    if (dst >= count) return 0.f;
+    const int src = kept[dst], r = src / chunk;
+    const uint32_t* k = kSmem ? cluster.map_shared_rank(sel_smem, r) : p.keys + (size_t)(blockIdx.x - rank + r) * p.chunk_cap;
+    return weight_of(k[src - r * chunk]);
   };
-  for (int t0 = c0; t0 < c1; t0 += 4 * kSelThreads) {
-    const int i0 = t0 + 4 * tid;
-    uint32_t key[4], packed = 0;  // above in the low half, equal in the high half (<= 2048 each)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = i0 + j;
-      key[j] = i < c1 ? keys[i - c0] : 0u;
-      if (contest && i < c1 && i >= lo && i < hi) packed += key[j] > T ? 1u : key[j] == T ? 0x10000u : 0u;
-    }
-    uint32_t total = 0, at = 0;
-    if (contest) at = block_scan(packed, warp_sums, &total) - packed;
-    uint32_t above = base_above + (at & 0xffffu), equal = base_equal + (at >> 16);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = i0 + j;
-      if (i >= c1) continue;
-      if (n <= p.budget || i < lo) {
-        put(i, i, key[j]);
-      } else if (i >= hi) {
-        put(p.budget - (n - i), i, key[j]);
-      } else if (contest && key[j] > T) {
-        put(lo + (int)(above + min(equal, quota)), i, key[j]);
-        ++above;
-      } else if (contest && key[j] == T) {
-        if (equal < quota) put(lo + (int)(above + equal), i, key[j]);
-        ++equal;
-      }
-    }
-    base_above += total & 0xffffu;
-    base_equal += total >> 16;
-  }
-  // ---- no tokens behind the kept ones: positions -1, weights zero
-  for (int i = count + rank * kSelThreads + tid; i < p.budget; i += C * kSelThreads) kept[i] = -1;
-  if (p.vec) {  // whole groups of four behind the one that `count` falls into
-    for (int64_t i = (count & ~3) + 4 * (rank * kSelThreads + tid); i < cap; i += 4 * C * kSelThreads) {
-      const int lp = (int)(i / p.page);
+  if (p.vec) {
+    for (int i = 4 * (rank * kSelThreads + tid); i < cap; i += 4 * C * kSelThreads) {
+      const int lp = p.by_page.quot(i);
       const int64_t phys = page_at(p, b, lp);
-      if (phys < 0) continue;
-      float* dst = p.weights_out + (phys * p.Hkv + h) * p.page + (i - (int64_t)lp * p.page);
-      if (i >= count) {
-        *reinterpret_cast<float4*>(dst) = make_float4(0.f, 0.f, 0.f, 0.f);
-      } else {
-        for (int j = 0; j < 4; ++j)
-          if (i + j >= count) dst[j] = 0.f;
-      }
+      const float4 w = make_float4(weight_at(i), weight_at(i + 1), weight_at(i + 2), weight_at(i + 3));
+      if (phys >= 0)
+        *reinterpret_cast<float4*>(p.weights_out + (phys * p.Hkv + h) * p.page + (i - lp * p.page)) = w;
     }
   } else {
-    for (int64_t i = count + rank * kSelThreads + tid; i < cap; i += C * kSelThreads) {
-      const int lp = (int)(i / p.page);
+    for (int i = rank * kSelThreads + tid; i < cap; i += C * kSelThreads) {
+      const int lp = p.by_page.quot(i);
       const int64_t phys = page_at(p, b, lp);
-      if (phys >= 0) p.weights_out[(phys * p.Hkv + h) * p.page + (i - (int64_t)lp * p.page)] = 0.f;
+      const float w = weight_at(i);
+      if (phys >= 0) p.weights_out[(phys * p.Hkv + h) * p.page + (i - lp * p.page)] = w;
     }
   }
-  cluster.sync();  // no CTA leaves while its counts may still be read
+  cluster.sync();  // no CTA leaves while its keys and counts may still be read
 }
 
 constexpr int kMoveWarps = 8;
@@ -314,10 +340,10 @@ struct PageMove {
     dst = (int)page_at(p, b, pg);
 #pragma unroll
     for (int c = 0; c < kCh; ++c) {
-      const int e = 16 * (32 * c + lane), t = e / p.D;
+      const int e = 16 * (32 * c + lane), t = p.by_dim.quot(e);
       sp[c] = -1;
       if (e < p.page * p.D && t < rows) {
-        const int src = kept[pg * p.page + t], lp = src / p.page;
+        const int src = kept[pg * p.page + t], lp = p.by_page.quot(src);
         sp[c] = (int)page_at(p, b, lp);
         sr[c] = src - lp * p.page;
       }
@@ -326,7 +352,7 @@ struct PageMove {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         if (tp[u] < 0) continue;
-        const int lp = tp[u] / p.page;
+        const int lp = p.by_page.quot(tp[u]);
         tr[u] = tp[u] - lp * p.page;
         tp[u] = (int)page_at(p, b, lp);
       }
@@ -414,7 +440,7 @@ __global__ void __launch_bounds__(kMoveWarps * 32) move_tokens_kernel(const Evic
         if (!kSym) sc[q][c] = 0.f, zp[q][c] = 128;  // an absent token dequantizes to 0
         if (m.sp[c] >= 0) {
           const int64_t blk = (int64_t)m.sp[c] * p.Hkv + h;
-          raw[q][c] = *reinterpret_cast<const uint4*>(values + blk * E + m.sr[c] * D + e % D);
+          raw[q][c] = *reinterpret_cast<const uint4*>(values + blk * E + m.sr[c] * D + (e - p.by_dim.quot(e) * D));
           if (!kSym) sc[q][c] = scale[blk], zp[q][c] = zero[blk];
         }
       }
@@ -484,6 +510,13 @@ static int select_cluster(int64_t tokens, int64_t rows, int* chunk_cap) {
     *chunk_cap = (int)((tokens + 4 * C - 1) / (4 * C) * 4);
   }
   return C;
+}
+
+static Divisor divisor(int d) {
+  Divisor x{d, -1};
+  if ((d & (d - 1)) == 0)
+    for (x.shift = 0; (1 << x.shift) < d;) ++x.shift;
+  return x;
 }
 
 static int evict_check(const FsEvictArgs* a) {
@@ -605,6 +638,8 @@ int fs_evict_tokens(const FsEvictArgs* a, void* stream) {
   p.budget = a->budget;
   p.recent = a->recent;
   p.sinks = a->sinks;
+  p.by_page = divisor(a->page_size);
+  p.by_dim = divisor(a->head_dim);
   p.sym = a->kv_format == FS_KV_SYMMETRIC;
   p.vec = a->page_size % 4 == 0 && ((reinterpret_cast<uintptr_t>(a->weights) | reinterpret_cast<uintptr_t>(a->weights_out)) & 15) == 0;
   const int C = select_cluster(evict_tokens_at_most(a), (int64_t)a->batch * a->kv_heads, &p.chunk_cap);
