@@ -40,6 +40,7 @@
 #include "common.h"
 #include "generic.h"
 #include "ptx.cuh"
+#include "tensor_map.h"
 #include "weights.h"
 #include "xwords.cuh"
 
@@ -1640,23 +1641,6 @@ static int resident_ctas(int device, int shape) {
     per_sm = 1;
   cached[shape][device] = per_sm * device_sm_count(device);
   return cached[shape][device];
-}
-
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(ptr);
-  });
-  return fn;
 }
 
 // View of an int8 KV array as rows of 128 bytes; one box = one 16-row page block,

@@ -309,7 +309,12 @@ __global__ void __launch_bounds__(kSelThreads) select_tokens_kernel(const EvictP
   cluster.sync();  // no CTA leaves while its keys and counts may still be read
 }
 
-constexpr int kMoveWarps = 8;
+
+// Affine pages of up to four chunks a lane: registers for 28 resident warps an SM.
+template <int kCh, int kWarps, bool kSym>
+constexpr int move_min_blocks() {
+  return kCh <= 4 && !kSym ? 28 / kWarps : 1;
+}
 
 // One page of K or V on its way through a warp: kCh 16-byte chunks a lane, chunk c of lane l
 // being bytes [16 (32 c + l), ...) of the page's [page, D] block.  The sources (page of the
@@ -360,53 +365,82 @@ struct PageMove {
   }
 };
 
+// Byte j of an XOR-ed word (a code u) as the float 2^23 + u.
+__device__ __forceinline__ float code_float(uint32_t w, int j) {
+  return __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7540 | j));
+}
+
 // 16 codes through (u - zp) * scale and the destination's rounding, bit for bit as dequant16
-// followed by quantize16_fast, with one multiplication for the two.  With x = RN(d s),
-// d = u - zp exact, the code is rint(clamp(RN(RN(x / S) + Z))).  ta = RN(d RN(s RN(1/S)) + Z)
-// is within |d s / S| (3 2^-24) + ulp(ta) / 2 of it; where ta lies in [0, 255] |d s / S| <
-// 511, so that is below 1.2e-4, and a ta farther than 2^-12 from a half-integer has the same
-// rint (and clamps the same way).  The others, 0.05% of them, take the exact path.
+// followed by quantize16_fast, with one multiplication for the two.  With d = u - zp exact the
+// code is rint(clamp(t)), t = RN(RN(RN(d s) / S) + Z); here ta = RN(d RN(s RN(1/S)) + Z).
+// Where ta lies in [0, 255], |d s / S| <= 255 (1 + 2^-15), each side is off from d s / S + Z by
+// two roundings of it (255 * 2^-23) and half an ulp of 255 (2^-17): together less than 7.7e-5.
+// So a ta farther than 2^-13 (1.2e-4) from a half-integer has the same rint, and one outside
+// [0, 255] clamps the same way.  The others, 0.025% of them, take the exact path.
+constexpr float kNearHalf = 0.5f - 1.220703125e-4f;
+
+// Out of line: the codes of a chunk that has one near a half-integer, those by the format's
+// own steps.
+static __device__ __noinline__ uint4 requantize16_careful(uint4 raw, float scale, float base, float ratio, float to_scale,
+                                                          float to_zero) {
+  const QParams q{to_scale, to_zero};
+  uint32_t w4[4] = {raw.x ^ 0x80808080u, raw.y ^ 0x80808080u, raw.z ^ 0x80808080u, raw.w ^ 0x80808080u};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    uint32_t out = 0u;
+#pragma unroll 1
+    for (int j = 0; j < 4; ++j) {
+      const float d = __fsub_rn(__uint_as_float(0x4B000000u | ((w4[k] >> (8 * j)) & 0xffu)), base);
+      const float tc = fminf(fmaxf(__fmaf_rn(d, ratio, q.zp), 0.0f), 255.0f);
+      uint32_t code = (uint32_t)rintf(tc);
+      if (fabsf(__fsub_rn(tc, rintf(tc))) >= kNearHalf)
+        code = (uint32_t)((int)quantize_one(__fmul_rn(d, scale), q) + 128);
+      out |= code << (8 * j);
+    }
+    w4[k] = out ^ 0x80808080u;
+  }
+  return make_uint4(w4[0], w4[1], w4[2], w4[3]);
+}
+
 __device__ __forceinline__ uint4 requantize16(uint4 raw, float scale, int16_t zp, float ratio, QParams q) {
   const float base = __fadd_rn(8388608.0f, (float)zp);
   const uint32_t w4[4] = {raw.x ^ 0x80808080u, raw.y ^ 0x80808080u, raw.z ^ 0x80808080u, raw.w ^ 0x80808080u};
   constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23
   uint32_t w[4];
+  float worst = 0.f;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     uint32_t bits[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float d = __fsub_rn(__uint_as_float(__byte_perm(w4[k], 0x4B000000u, 0x7540 | j)), base);
-      const float tc = fminf(fmaxf(__fmaf_rn(d, ratio, q.zp), 0.0f), 255.0f);
+      const float ta = __fmaf_rn(__fsub_rn(code_float(w4[k], j), base), ratio, q.zp);
+      const float tc = fminf(fmaxf(ta, 0.0f), 255.0f);
       const float r = __fadd_rn(tc, kMagic);
-      const float off = __fsub_rn(tc, __fsub_rn(r, kMagic));
+      worst = fmaxf(worst, fabsf(__fsub_rn(tc, __fsub_rn(r, kMagic))));
       bits[j] = __float_as_uint(r);  // low byte = rint(tc)
-      if (fabsf(off) >= 0.5f - 2.44140625e-4f)
-        bits[j] = (uint32_t)(uint8_t)quantize_one_exact(__fmul_rn(d, scale), q) ^ 0x80u;
     }
     const uint32_t lo = __byte_perm(bits[0], bits[1], 0x0040), hi = __byte_perm(bits[2], bits[3], 0x0040);
     w[k] = __byte_perm(lo, hi, 0x5410) ^ 0x80808080u;
   }
+  if (worst >= kNearHalf) return requantize16_careful(raw, scale, base, ratio, q.scale, q.zp);
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Smallest and largest byte of 16 codes, as the unsigned codes u = value + 128.  (u - zp)
-// times a positive scale is monotone, rounding included, so these give the chunk's extremes.
-__device__ __forceinline__ void minmax16(uint4 raw, int& lo, int& hi) {
+// Smallest and largest of 16 codes u, as floats 2^23 + u.  (u - zp) times a positive scale is
+// monotone, rounding included, so they give the chunk's extremes.
+__device__ __forceinline__ void minmax16(uint4 raw, float& lo, float& hi) {
   const uint32_t w4[4] = {raw.x ^ 0x80808080u, raw.y ^ 0x80808080u, raw.z ^ 0x80808080u, raw.w ^ 0x80808080u};
-  uint32_t mn = 0x00ff00ffu, mx = 0u;
+  lo = hi = code_float(w4[0], 0);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const uint32_t a = w4[k] & 0x00ff00ffu, b = (w4[k] >> 8) & 0x00ff00ffu;
-    mn = __vimin3_u16x2(mn, a, b);
-    mx = __vimax3_u16x2(mx, a, b);
+  for (int j = 1; j < 16; ++j) {
+    const float f = code_float(w4[j >> 2], j & 3);
+    lo = fminf(lo, f);
+    hi = fmaxf(hi, f);
   }
-  lo = min((int)(mn & 0xffffu), (int)(mn >> 16));
-  hi = max((int)(mx & 0xffffu), (int)(mx >> 16));
 }
 
-template <int kCh, int kPages, bool kSym>
-__global__ void __launch_bounds__(kMoveWarps * 32) move_tokens_kernel(const EvictParams p) {
+template <int kCh, int kPages, int kWarps, bool kSym>
+__global__ void __launch_bounds__(kWarps * 32, move_min_blocks<kCh, kWarps, kSym>()) move_tokens_kernel(const EvictParams p) {
   cg::cluster_group cluster = cg::this_cluster();
   const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int item = blockIdx.x / C, kv = item & 1, row = item >> 1, b = row / p.Hkv, h = row % p.Hkv;
@@ -418,8 +452,8 @@ __global__ void __launch_bounds__(kMoveWarps * 32) move_tokens_kernel(const Evic
   int8_t* values = p.values[kv];
   float* scale = p.scale[kv];
   int16_t* zero = p.zero[kv];
-  const int per_round = C * kMoveWarps * kPages;
-  const int pg0 = (rank * kMoveWarps + warp) * kPages;
+  const int per_round = C * kWarps * kPages;
+  const int pg0 = (rank * kWarps + warp) * kPages;
   PageMove<kCh, kSym> mv[kPages];
 #pragma unroll
   for (int q = 0; q < kPages; ++q) mv[q].plan(p, b, kept, pg0 + q, npg, lane);
@@ -450,50 +484,53 @@ __global__ void __launch_bounds__(kMoveWarps * 32) move_tokens_kernel(const Evic
           sc[q][u] = m.tp[u] >= 0 ? scale[((int64_t)m.tp[u] * p.Hkv + h) * page + m.tr[u]] : 1.0e-8f;
       }
     }
+    cluster.barrier_arrive();  // this warp's sources of the round are read
 #pragma unroll
     for (int q = 0; q < kPages; ++q) mv[q].plan(p, b, kept, r0 + per_round + pg0 + q, npg, lane);
-    cluster.sync();  // all sources of this round are in registers
+    QParams qp[kPages];
+    if (!kSym) {  // the new codes, in place of the old ones, while the others arrive
+#pragma unroll
+      for (int q = 0; q < kPages; ++q) {
+        if (dst[q] < 0) continue;
+        float mn = INFINITY, mx = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < kCh; ++c) {
+          if (16 * (32 * c + lane) >= E) continue;
+          float lo, hi;
+          minmax16(raw[q][c], lo, hi);
+          const float base = __fadd_rn(8388608.0f, (float)zp[q][c]);
+          mn = fminf(mn, __fmul_rn(__fsub_rn(lo, base), sc[q][c]));
+          mx = fmaxf(mx, __fmul_rn(__fsub_rn(hi, base), sc[q][c]));
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+          mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        }
+        qp[q] = qparams_from_range(mn, mx);
+        const float rcp = __frcp_rn(qp[q].scale);
+#pragma unroll
+        for (int c = 0; c < kCh; ++c)
+          raw[q][c] = requantize16(raw[q][c], sc[q][c], zp[q][c], __fmul_rn(sc[q][c], rcp), qp[q]);
+      }
+    }
+    cluster.barrier_wait();  // all sources of the round are read
 #pragma unroll
     for (int q = 0; q < kPages; ++q) {
       if (dst[q] < 0) continue;
       int8_t* out = values + dst[q] * E;
-      if (kSym) {
-#pragma unroll
-        for (int c = 0; c < kCh; ++c) {
-          const int e = 16 * (32 * c + lane);
-          if (e < E) *reinterpret_cast<uint4*>(out + e) = raw[q][c];
-        }
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-          if (lane + 32 * u < page) scale[dst[q] * page + lane + 32 * u] = sc[q][u];
-        continue;
-      }
-      float mn = INFINITY, mx = -INFINITY;
-#pragma unroll
-      for (int c = 0; c < kCh; ++c) {
-        if (16 * (32 * c + lane) >= E) continue;
-        int lo, hi;
-        minmax16(raw[q][c], lo, hi);
-        mn = fminf(mn, dequant_one((int8_t)(lo - 128), sc[q][c], zp[q][c]));
-        mx = fmaxf(mx, dequant_one((int8_t)(hi - 128), sc[q][c], zp[q][c]));
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      }
-      const QParams qp = qparams_from_range(mn, mx);
-      const float rcp = __frcp_rn(qp.scale);
 #pragma unroll
       for (int c = 0; c < kCh; ++c) {
         const int e = 16 * (32 * c + lane);
-        if (e < E)
-          *reinterpret_cast<uint4*>(out + e) =
-              requantize16(raw[q][c], sc[q][c], zp[q][c], __fmul_rn(sc[q][c], rcp), qp);
+        if (e < E) *reinterpret_cast<uint4*>(out + e) = raw[q][c];
       }
-      if (lane == 0) {
-        scale[dst[q]] = qp.scale;
-        zero[dst[q]] = (int16_t)qp.zp;
+      if (kSym) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          if (lane + 32 * u < page) scale[dst[q] * page + lane + 32 * u] = sc[q][u];
+      } else if (lane == 0) {
+        scale[dst[q]] = qp[q].scale;
+        zero[dst[q]] = (int16_t)qp[q].zp;
       }
     }
   }
@@ -579,23 +616,29 @@ static int launch_cluster(Kernel kernel, const char* what, int64_t rows, int clu
   return FS_OK;
 }
 
+// Rows that fill the GPU by themselves take one CTA of four warps each (few warps wait for
+// each other, no long tail); fewer rows are spread over clusters of CTAs of eight warps, up to
+// one round of their pages.
+template <int kCh, int kPages, bool kSym>
+static int launch_move_chunks(const FsEvictArgs* a, const EvictParams& p, void* stream) {
+  const int npg = (a->budget + a->page_size - 1) / a->page_size;
+  const int64_t rows = (int64_t)a->batch * a->kv_heads * 2;
+  const char* what = "token move kernel launch";
+  if (rows >= 2 * kEvictFill) return launch_cluster(move_tokens_kernel<kCh, kPages, 4, kSym>, what, rows, 1, 128, 0, p, stream);
+  int C = 1;
+  while (C < 8 && rows * C < 2 * kEvictFill && npg > C * 8 * kPages) C *= 2;
+  return launch_cluster(move_tokens_kernel<kCh, kPages, 8, kSym>, what, rows, C, 256, 0, p, stream);
+}
+
 template <bool kSym>
 static int launch_move(const FsEvictArgs* a, const EvictParams& p, void* stream) {
   const int chunks = (a->page_size * a->head_dim + 511) / 512;
-  const int npg = (a->budget + a->page_size - 1) / a->page_size;
-  const int64_t rows = (int64_t)a->batch * a->kv_heads * 2;
-  auto go = [&](auto kernel, int pages) {
-    // few rows are spread over clusters, up to one round of their pages
-    int C = 1;
-    while (C < 8 && rows * C < 2 * kEvictFill && npg > C * kMoveWarps * pages) C *= 2;
-    return launch_cluster(kernel, "token move kernel launch", rows, C, kMoveWarps * 32, 0, p, stream);
-  };
-  if (chunks <= 1) return go(move_tokens_kernel<1, 2, kSym>, 2);
-  if (chunks <= 2) return go(move_tokens_kernel<2, 2, kSym>, 2);
-  if (chunks <= 4) return go(move_tokens_kernel<4, kSym ? 2 : 1, kSym>, kSym ? 2 : 1);
-  if (chunks <= 8) return go(move_tokens_kernel<8, 1, kSym>, 1);
-  if (chunks <= 16) return go(move_tokens_kernel<16, 1, kSym>, 1);
-  return go(move_tokens_kernel<24, 1, kSym>, 1);
+  if (chunks <= 1) return launch_move_chunks<1, 2, kSym>(a, p, stream);
+  if (chunks <= 2) return launch_move_chunks<2, 2, kSym>(a, p, stream);
+  if (chunks <= 4) return launch_move_chunks<4, kSym ? 2 : 1, kSym>(a, p, stream);
+  if (chunks <= 8) return launch_move_chunks<8, 1, kSym>(a, p, stream);
+  if (chunks <= 16) return launch_move_chunks<16, 1, kSym>(a, p, stream);
+  return launch_move_chunks<24, 1, kSym>(a, p, stream);
 }
 
 }  // namespace fsb

@@ -9,16 +9,16 @@
 //
 // latent_attention_kernel.  Rows (t, h) of a request are cut into blocks of up to 16, 32 or
 // 64; the flattened list of (request, row block, tile of 64 tokens) is cut into equal
-// contiguous shares, one per CTA (lengths are read on the device).  A CTA keeps three tiles
-// in flight with cp.async.  Per tile:
+// contiguous shares, one per CTA (lengths are read on the device).  Warp 0 keeps three tiles
+// in flight with TMA (128-byte swizzle; page lookups run a tile ahead).  Per tile:
 //   1. S = Q C^T on the int8 tensor cores, straight from the stored bytes: q is held as
 //      16-bit fixed point in two signed bytes (error max|q| 2^-16 of a row), two exact
-//      MMAs; the rotary part on 16-bit MMAs.  The eight warps split rows, dims and tokens
-//      (kMT x kKS x kTS), so q stays in registers; their partial sums meet in shared memory.
+//      MMAs; the rotary part on 16-bit MMAs.  The warps split rows, dims and tokens (kMT x
+//      kKS x kTS), so q stays in registers; their partial sums meet in shared memory.
 //   2. softmax: running maximum m of score + log2(scale) and sum of 2^(score - m) per row in
 //      fp32; P = 2^(score - m) * scale in fp16, scaled by 2^14 to use its range whatever the
 //      scale (the largest P is 2^14).
-//   3. O += P C: each warp owns dc / 8 dims of all rows.  A byte becomes the exact fp16
+//   3. O += P C: each warp owns dc / 16 dims of all rows.  A byte becomes the exact fp16
 //      integer (XOR and byte permute against 0x64 exponent bytes, minus 1152).
 // A share that holds a whole (request, row block) writes the output; others leave normalised
 // (O, LSE) partials that latent_merge_kernel joins.
@@ -34,6 +34,7 @@
 #include "../../include/flashspec_b200.h"
 #include "common.h"
 #include "ptx.cuh"
+#include "tensor_map.h"
 
 namespace fsb {
 
@@ -113,27 +114,24 @@ __global__ void __launch_bounds__(kAppendWarps * 32) latent_append_kernel(const 
 // absorbed attention
 // ---------------------------------------------------------------------------------
 
-constexpr int kLatThreads = 256;
-constexpr int kLatWarps = 8;
 constexpr int kTile = 64;  // tokens
 constexpr int kLatStages = 3;
 constexpr int kSPad = 72;  // floats a row of partial scores
 constexpr int kPPad = 72;  // halves a row of P
 constexpr int kLatMaxBatch = 4096;
 constexpr float kPTop = 16384.f;
+constexpr uint64_t kLatTimeoutNs = 2000000000ull;
 
 struct LatentParams {
   const uint16_t* q;       // [B, T, H, dc]
   const uint16_t* q_rope;  // [B, T, H, dr]
-  const int8_t* values;    // [P, page, dc]
   const float* scale;      // [P, page]
-  const uint16_t* ropes;   // [P, page, dr]
   const int64_t* table;
   const int64_t* lengths;
-  uint16_t* out;  // [B, T, H, dc]
-  float* part_o;  // [ctas][2][rows of a block][dc]
+  uint16_t* out;    // [B, T, H, dc]
+  float* part_o;    // [ctas][2][rows of a block][dc]
   float* part_lse;  // [ctas][2][rows of a block], log2 domain
-  int* prefix;  // [B + 1] tiles before each request (row blocks not counted)
+  int* prefix;      // [B + 1] tiles before each request (row blocks not counted)
   uint32_t* status;
   int64_t num_pages, max_seq_len;
   float scale_log2;  // sm_scale * log2(e)
@@ -144,39 +142,43 @@ __device__ __forceinline__ int latent_len(const LatentParams& p, int b) {
   return (int)max((int64_t)0, min(min(p.lengths[b], p.max_seq_len), (int64_t)p.cols * p.page));
 }
 
-// Bank swizzle of the 16-byte chunks of a row: rows r and r + 1 differ by 4 chunks (two rows
-// of four chunks are read together), eight rows by eight different amounts.
-__device__ __forceinline__ int lat_swz(int row) { return ((row & 1) << 2) | ((row >> 1) & 3); }
+// Column n of a tile's scores is token lat_token(n): inside each group of eight, even columns
+// are tokens 0-3 and odd ones 4-7.  The two rows that a quarter warp reads together then
+// differ in bit 2, so the 128-byte swizzle puts their four chunks on different banks.
+__device__ __forceinline__ int lat_token(int n) { return (n & ~7) | ((n >> 1) & 3) | ((n & 1) << 2); }
 
 template <int kDC, int kDR, int kMT>
 struct LatentShape {
+  static constexpr int kWarps = kDC >= 256 ? 16 : 8;
+  static constexpr int kThreads = 32 * kWarps;
   static constexpr int kRows = 16 * kMT;
   // warps = kMT row groups x kKS slices of the dims (64 at least) x kTS token groups
-  static constexpr int kKS = (8 / kMT) < (kDC / 64) ? (8 / kMT) : (kDC / 64);
-  static constexpr int kTS = 8 / (kMT * kKS);
-  static constexpr int kSlice = kDC / kKS;        // dims of a warp's QK slice
-  static constexpr int kQSteps = kSlice / 32;     // int8 MMA steps
-  static constexpr int kNT = kTile / 8 / kTS;     // n-tiles of 8 tokens a warp
-  static constexpr int kRSteps = kDR / 16;        // rotary MMA steps, dealt to the slices
+  static constexpr int kMaxKS = kMT == 1 ? 8 : 4;
+  static constexpr int kKS = kMaxKS < kDC / 64 ? kMaxKS : kDC / 64;
+  static constexpr int kTS = kWarps / (kMT * kKS);
+  static constexpr int kSlice = kDC / kKS;     // dims of a warp's QK slice
+  static constexpr int kQSteps = kSlice / 32;  // int8 MMA steps
+  static constexpr int kNT = kTile / 8 / kTS;  // n-tiles of 8 tokens a warp
+  static constexpr int kRSteps = kDR / 16;     // rotary MMA steps, dealt to the slices
   static constexpr int kRPer = (kRSteps + kKS - 1) / kKS;
-  static constexpr int kDW = kDC / 8;             // dims of a warp's O
-  static constexpr int kOT = kDW / 8;             // n-tiles of O
-  static constexpr int kTPR = kLatThreads / kRows;  // softmax threads a row
-  static constexpr int kSeg = kTile / 4 / kTPR;     // groups of four tokens a softmax thread
+  static constexpr int kDW = kDC / kWarps;     // dims of a warp's O
+  static constexpr int kOT = kDW / 8;          // n-tiles of O
+  static constexpr int kTPR = kThreads / kRows;  // softmax threads a row
+  static constexpr int kGV = kTile / kTPR < 4 ? kTile / kTPR : 4;  // columns a softmax thread reads together
+  static constexpr int kSeg = kTile / kTPR / kGV;
   static constexpr int kValBytes = kTile * kDC, kRopeBytes = kTile * kDR * 2;
-  static constexpr int kStage = kValBytes + kRopeBytes + kTile * 4;
+  static constexpr int kStage = (kValBytes + kRopeBytes + kTile * 4 + 1023) / 1024 * 1024;
   static constexpr int kSBytes = kKS * kRows * kSPad * 4;
   static constexpr int kPBytes = kRows * kPPad * 2;
   static constexpr int kOffS = kLatStages * kStage;
   static constexpr int kOffP = kOffS + kSBytes;
-  static constexpr int kOffMisc = kOffP + kPBytes;  // alpha [rows], qscale [rows], lam [tile], prefix
-  static constexpr int kMiscFloats = 2 * kRows + kTile;
-  static constexpr __host__ __device__ int smem(int batch) { return kOffMisc + kMiscFloats * 4 + (batch + 1) * 4; }
+  static constexpr int kOffMisc = kOffP + kPBytes;  // alpha [rows], qscale [rows], scale and lam [tile], prefix
+  static constexpr int kMiscFloats = 2 * kRows + 2 * kTile;
+  static_assert(kTS >= 1 && kMT * kKS * kTS == kWarps, "every warp has a part of the scores");
+  static constexpr __host__ __device__ int smem(int batch) {
+    return 1024 /* alignment */ + kOffMisc + kMiscFloats * 4 + (batch + 1) * 4;
+  }
 };
-
-__device__ __forceinline__ void lat_cp16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
 
 __device__ __forceinline__ void mma_16816_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                                uint32_t b0, uint32_t b1) {
@@ -192,9 +194,10 @@ __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t& r0, uint32_t& r
 }
 
 // Tiles before each request, into pre[0 .. B] (shared memory); every thread calls it.
+template <int kThreads>
 __device__ __forceinline__ void latent_prefix(const LatentParams& p, int* pre) {
   const int tid = threadIdx.x, lane = tid & 31;
-  for (int r = tid; r < p.B; r += kLatThreads) pre[r + 1] = (latent_len(p, r) + kTile - 1) / kTile;
+  for (int r = tid; r < p.B; r += kThreads) pre[r + 1] = (latent_len(p, r) + kTile - 1) / kTile;
   __syncthreads();
   if (tid < 32) {
     int carry = 0;
@@ -213,35 +216,49 @@ __device__ __forceinline__ void latent_prefix(const LatentParams& p, int* pre) {
   __syncthreads();
 }
 
-// Share k of C of n flat tiles starts here.
+// n flat tiles on C = min(CTAs, n) shares, none of them empty; share k starts here.
 __device__ __forceinline__ int64_t latent_share(int64_t n, int k, int C) { return n * k / C; }
 
 template <int kDC, int kDR, int kMT, bool kBf16>
-__global__ void __launch_bounds__(kLatThreads, 1) latent_attention_kernel(const LatentParams p) {
+__global__ void __launch_bounds__(LatentShape<kDC, kDR, kMT>::kThreads, 1)
+    latent_attention_kernel(const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_r,
+                            const LatentParams p) {
   using L = LatentShape<kDC, kDR, kMT>;
-  extern __shared__ __align__(1024) uint8_t lat_smem[];
-  const uint32_t smem_s = smem_u32(lat_smem);
+  extern __shared__ uint8_t lat_raw[];
+  __shared__ alignas(8) uint64_t s_full[kLatStages];
+  __shared__ uint32_t s_pages[kLatStages];  // which of a tile's pages are there, one bit each
+  const uint32_t raw_s = smem_u32(lat_raw);
+  const uint32_t smem_s = (raw_s + 1023u) & ~1023u;
+  uint8_t* lat_smem = lat_raw + (smem_s - raw_s);
   float* s_part = reinterpret_cast<float*>(lat_smem + L::kOffS);  // [kKS][rows][kSPad]
   __half* s_p = reinterpret_cast<__half*>(lat_smem + L::kOffP);   // [rows][kPPad]
   float* s_alpha = reinterpret_cast<float*>(lat_smem + L::kOffMisc);
   float* s_qscale = s_alpha + L::kRows;
-  float* s_lam = s_qscale + L::kRows;
+  float* s_scale = s_qscale + L::kRows;  // by column, -1 where there is no token
+  float* s_lam = s_scale + kTile;        // by column, log2 of it
   int* pre = reinterpret_cast<int*>(s_lam + kTile);
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, c = lane & 3;
   const int mt = warp % kMT, ks = (warp / kMT) % L::kKS, ts = warp / (kMT * L::kKS);
 
-  latent_prefix(p, pre);
+  if (tid == 0) {
+    for (int i = 0; i < kLatStages; ++i) mbar_init(smem_u32(&s_full[i]), 1);
+    fence_mbar_init();
+    fence_proxy_async_smem();
+  }
+  latent_prefix<L::kThreads>(p, pre);
   if (blockIdx.x == 0)
-    for (int r = tid; r <= p.B; r += kLatThreads) p.prefix[r] = pre[r];
+    for (int r = tid; r <= p.B; r += L::kThreads) p.prefix[r] = pre[r];
   const int64_t total = (int64_t)pre[p.B] * p.row_blocks;
-  const int64_t f_begin = latent_share(total, blockIdx.x, gridDim.x);
-  const int64_t f_end = latent_share(total, blockIdx.x + 1, gridDim.x);
+  const int C = (int)min((int64_t)gridDim.x, total);
+  if ((int)blockIdx.x >= C) return;
+  const int64_t f_begin = latent_share(total, blockIdx.x, C), f_end = latent_share(total, blockIdx.x + 1, C);
   bool first = true;
+  uint32_t issued = 0, used = 0;  // tiles put into the ring and taken out of it, over all pieces
 
-  // softmax thread: row and its token groups
-  const int srow = tid / L::kTPR, sj = tid % L::kTPR;
+  const int srow = tid / L::kTPR, sj = tid % L::kTPR;  // softmax thread: row and its columns
+  const int box_rows = min(p.page, kTile), per_tile = kTile / box_rows;  // pages (or halves of one) a tile
 
   for (int64_t f = f_begin; f < f_end;) {
     // ---- the piece: tiles [t0, t1) of row block rb of request b
@@ -251,8 +268,8 @@ __global__ void __launch_bounds__(kLatThreads, 1) latent_attention_kernel(const 
       if ((int64_t)pre[mid] * p.row_blocks <= f) lo = mid; else hi = mid;
     }
     const int b = lo, nt = pre[b + 1] - pre[b];
-    const int64_t off = f - (int64_t)pre[b] * p.row_blocks;
-    const int rb = (int)(off / nt), t0 = (int)(off % nt);
+    const int off = (int)(f - (int64_t)pre[b] * p.row_blocks);
+    const int rb = off / nt, t0 = off - rb * nt;
     const int t1 = (int)min((int64_t)nt, t0 + (f_end - f));
     f += t1 - t0;
     const int len = latent_len(p, b);
@@ -261,62 +278,47 @@ __global__ void __launch_bounds__(kLatThreads, 1) latent_attention_kernel(const 
     const uint16_t* qrb = p.q_rope + ((size_t)b * p.R + row0) * kDR;
     const int64_t* trow = p.table + (size_t)b * p.cols;
 
-    // ---- tile loader: values, rotary parts and scales of tile t into stage t % kLatStages
-    auto load_tile = [&](int t) {
-      const int st = t % kLatStages;
-      const uint32_t base = smem_s + st * L::kStage;
-      const int tok0 = t * kTile;
-      constexpr int kVC = kDC / 16, kRC = kDR / 8;  // 16-byte chunks of a row
-#pragma unroll
-      for (int i = tid; i < kTile * kVC; i += kLatThreads) {
-        const int r = i / kVC, ch = i % kVC, tok = tok0 + r;
-        if (tok < len) {
-          const int lp = tok / p.page;
-          const int64_t phys = trow[lp];
-          if (phys >= 0 && phys < p.num_pages)
-            lat_cp16(base + r * kDC + ((ch ^ lat_swz(r)) << 4),
-                     p.values + ((size_t)phys * p.page + (tok - lp * p.page)) * kDC + 16 * ch);
-        }
+    // ---- producer (warp 0): page lookups run a tile ahead of the copies
+    auto lookup = [&](int t) -> int64_t {  // lane i: the pool page of part i of tile t, -1: none
+      const int tok = t * kTile + lane * box_rows;
+      if (t >= t1 || lane >= per_tile || tok >= len) return -1;
+      const int64_t phys = trow[tok / p.page];
+      if (phys >= p.num_pages) {
+        if (p.status != nullptr) atomicOr(p.status, FS_DEV_BAD_PAGE);
+        return -1;
       }
-#pragma unroll
-      for (int i = tid; i < kTile * kRC; i += kLatThreads) {
-        const int r = i / kRC, ch = i % kRC, tok = tok0 + r;
-        if (tok < len) {
-          const int lp = tok / p.page;
-          const int64_t phys = trow[lp];
-          if (phys >= 0 && phys < p.num_pages)
-            lat_cp16(base + L::kValBytes + r * kDR * 2 + ((ch ^ (lat_swz(r) & (kRC - 1))) << 4),
-                     p.ropes + ((size_t)phys * p.page + (tok - lp * p.page)) * kDR + 8 * ch);
-        }
-      }
-      if (tid < kTile) {  // a token that is not there gets scale -1
-        const int tok = tok0 + tid;
-        const uint32_t dst = base + L::kValBytes + L::kRopeBytes + 4 * tid;
-        int64_t phys = -1;
-        int lp = 0;
-        if (tok < len) {
-          lp = tok / p.page;
-          phys = trow[lp];
-          if (phys >= p.num_pages) {
-            if (p.status != nullptr) atomicOr(p.status, FS_DEV_BAD_PAGE);
-            phys = -1;
-          }
-        }
-        if (phys >= 0)
-          cp_async_4(dst, p.scale + (size_t)phys * p.page + (tok - lp * p.page));
-        else
-          asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst), "f"(-1.f) : "memory");
-      }
+      return phys;
     };
-
+    auto issue = [&](int t, int64_t phys) {  // tile t into the ring
+      const int st = (int)(issued % kLatStages);
+      const uint32_t base = smem_s + st * L::kStage, bar = smem_u32(&s_full[st]);
+      const uint32_t there = __ballot_sync(0xffffffffu, phys >= 0);
+      if (lane == 0) {
+        s_pages[st] = there;
+        mbar_arrive_expect_tx(bar, (uint32_t)__popc(there) * box_rows * (kDC + 2 * kDR + 4));
+      }
+      __syncwarp();
+      if (phys >= 0) {
+        const int r = lane * box_rows, in_page = (t * kTile + r) % p.page;
+        const int64_t row = phys * p.page + in_page;
+        const uint64_t policy = l2_policy_evict_first();
+#pragma unroll
+        for (int j = 0; j < kDC / 128; ++j)
+          tma_load_2d(base + j * (kTile * 128) + r * 128, &map_v, 128 * j, (int32_t)row, bar, policy);
+        tma_load_2d(base + L::kValBytes + r * 2 * kDR, &map_r, 0, (int32_t)row, bar, policy);
+        bulk_load(base + L::kValBytes + L::kRopeBytes + 4 * r, p.scale + row, (uint32_t)(4 * box_rows), bar);
+      }
+      ++issued;
+    };
+    int64_t next_phys = -1;
     __syncthreads();  // the previous piece is done with the stages and the row state
-    load_tile(t0);
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    if (t0 + 1 < t1) load_tile(t0 + 1);
-    asm volatile("cp.async.commit_group;" ::: "memory");
+    if (warp == 0) {
+      for (int i = 0; i < kLatStages - 1 && t0 + i < t1; ++i) issue(t0 + i, lookup(t0 + i));
+      next_phys = lookup(t0 + kLatStages - 1);
+    }
 
     // ---- q as 16-bit fixed point: row scales, then this warp's fragments
-    for (int r = warp; r < L::kRows; r += kLatWarps) {
+    for (int r = warp; r < L::kRows; r += L::kWarps) {
       float amax = 0.f;
       bool bad = false;
       if (r < rows) {
@@ -390,28 +392,25 @@ __global__ void __launch_bounds__(kLatThreads, 1) latent_attention_kernel(const 
         for (int k = 0; k < 4; ++k) acc[i][j][k] = 0.f;
     float m_run = -1.0e30f, l_run = 0.f;
     // tokens that this softmax thread's row sees: query t sees the first len - T + t + 1
-    const int limit = len - p.T + 1 + (row0 + srow) / p.H;
+    const int limit = min(len, len - p.T + 1 + (row0 + srow) / p.H);
 
-    for (int t = t0; t < t1; ++t) {
-      asm volatile("cp.async.wait_group 1;" ::: "memory");
-      __syncthreads();  // tile t is here; every warp is done with tile t - 1
-      if (t + 2 < t1) load_tile(t + 2);
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      const uint32_t base = smem_s + (t % kLatStages) * L::kStage;
+    for (int t = t0; t < t1; ++t, ++used) {
+      const int st = (int)(used % kLatStages);
+      const uint32_t base = smem_s + st * L::kStage;
       const float* tok_scale =
-          reinterpret_cast<const float*>(lat_smem + (t % kLatStages) * L::kStage + L::kValBytes + L::kRopeBytes);
-      if (tid < kTile) s_lam[tid] = fmaxf(lg2_approx(fmaxf(tok_scale[tid], 0.f)), -100.f);
+          reinterpret_cast<const float*>(lat_smem + st * L::kStage + L::kValBytes + L::kRopeBytes);
+      const bool here = mbar_wait_bounded(smem_u32(&s_full[st]), (used / kLatStages) & 1u, kLatTimeoutNs);
 
       // ---- 1. partial scores of this warp's rows, dims and tokens
+      const int prow = lat_token(g);  // row of column g of a group
 #pragma unroll
       for (int n = 0; n < L::kNT; ++n) {
-        const int tok = (ts * L::kNT + n) * 8;
+        const int col = (ts * L::kNT + n) * 8, brow = col + prow;
         int sh[4] = {0, 0, 0, 0}, sl[4] = {0, 0, 0, 0};
-        const int brow = tok + g;
 #pragma unroll
         for (int j2 = 0; j2 < L::kQSteps / 2; ++j2) {
-          const int ch = (ks * L::kSlice + 64 * j2) / 16 + c;
-          const uint4 kv = lds128(base + brow * kDC + ((ch ^ lat_swz(brow)) << 4));
+          const int d16 = (ks * L::kSlice + 64 * j2) / 16 + c;  // 16-byte chunk of the row
+          const uint4 kv = lds128(base + (d16 >> 3) * (kTile * 128) + brow * 128 + (((d16 & 7) ^ prow) << 4));
           mma_16832_s8(sh, qhi[2 * j2][0], qhi[2 * j2][1], qhi[2 * j2][2], qhi[2 * j2][3], kv.x, kv.y);
           mma_16832_s8(sl, qlo[2 * j2][0], qlo[2 * j2][1], qlo[2 * j2][2], qlo[2 * j2][3], kv.x, kv.y);
           mma_16832_s8(sh, qhi[2 * j2 + 1][0], qhi[2 * j2 + 1][1], qhi[2 * j2 + 1][2], qhi[2 * j2 + 1][3], kv.z, kv.w);
@@ -422,10 +421,9 @@ __global__ void __launch_bounds__(kLatThreads, 1) latent_attention_kernel(const 
         for (int i = 0; i < L::kRPer; ++i) {
           const int s = ks + i * L::kKS;
           if (s < L::kRSteps) {
-            constexpr int kRC = kDR / 8;
             const int ch = 2 * s + (c >> 1);
-            const uint32_t at = base + L::kValBytes + brow * kDR * 2 + ((ch ^ (lat_swz(brow) & (kRC - 1))) << 4) + 8 * (c & 1);
-            const float2 w = lds64f(at);
+            const int swz = kDR == 64 ? prow : (prow >> 1) & 3;  // the 128- or 64-byte swizzle
+            const float2 w = lds64f(base + L::kValBytes + brow * kDR * 2 + ((ch ^ swz) << 4) + 8 * (c & 1));
             const uint32_t b0 = __float_as_uint(w.x), b1 = __float_as_uint(w.y);
             if (kBf16)
               mma_16816_bf16(rp, qr[i][0], qr[i][1], qr[i][2], qr[i][3], b0, b1);
@@ -433,40 +431,64 @@ __global__ void __launch_bounds__(kLatThreads, 1) latent_attention_kernel(const 
               mma_16816(rp, qr[i][0], qr[i][1], qr[i][2], qr[i][3], b0, b1);
           }
         }
-        const float2 sc = *reinterpret_cast<const float2*>(tok_scale + tok + 2 * c);
-        float* dst = s_part + ((size_t)ks * L::kRows + 16 * mt + g) * kSPad + tok + 2 * c;
+        const float sc0 = tok_scale[col + c], sc1 = tok_scale[col + c + 4];  // columns 2c and 2c + 1
+        float* dst = s_part + ((size_t)ks * L::kRows + 16 * mt + g) * kSPad + col + 2 * c;
 #pragma unroll
-        for (int r2 = 0; r2 < 2; ++r2) {
-          const float x0 = fmaf(256.f, (float)sh[2 * r2], (float)sl[2 * r2]) * (fq[r2] * sc.x);
-          const float x1 = fmaf(256.f, (float)sh[2 * r2 + 1], (float)sl[2 * r2 + 1]) * (fq[r2] * sc.y);
+        for (int r2 = 0; r2 < 2; ++r2) {  // at most 256 dims: 256 hi + lo stays within 31 bits
+          const float x0 = (float)((sh[2 * r2] << 8) + sl[2 * r2]) * (fq[r2] * sc0);
+          const float x1 = (float)((sh[2 * r2 + 1] << 8) + sl[2 * r2 + 1]) * (fq[r2] * sc1);
           *reinterpret_cast<float2*>(dst + 8 * r2 * kSPad) =
               make_float2(fmaf(rp[2 * r2], p.scale_log2, x0), fmaf(rp[2 * r2 + 1], p.scale_log2, x1));
         }
       }
-      __syncthreads();
+      if (tid < kTile) {
+        const int tok = lat_token(tid);
+        const bool there = t * kTile + tok < len && ((s_pages[st] >> (tok / box_rows)) & 1u);
+        const float sc = there ? tok_scale[tok] : -1.f;
+        s_scale[tid] = sc;
+        s_lam[tid] = fmaxf(lg2_approx(fmaxf(sc, 0.f)), -100.f);
+      }
+      if (__syncthreads_or(here ? 0 : 1)) {  // a copy that never came: give up, outputs are invalid
+        if (tid == 0 && p.status != nullptr) atomicOr(p.status, FS_DEV_TIMEOUT);
+        return;
+      }
+      // every warp is done with tile t - 1: its stage takes tile t + kLatStages - 1
+      if (warp == 0 && t + kLatStages - 1 < t1) {
+        issue(t + kLatStages - 1, next_phys);
+        next_phys = lookup(t + kLatStages);
+      }
 
-      // ---- 2. softmax of row srow, four tokens at a time
-      float z[L::kSeg][4];
+      // ---- 2. softmax of row srow
+      float z[L::kSeg][L::kGV], sc[L::kSeg][L::kGV];
       float mx = -INFINITY;
 #pragma unroll
       for (int i = 0; i < L::kSeg; ++i) {
-        const int tk = 4 * (sj + L::kTPR * i);
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        const int n0 = L::kGV * (sj + L::kTPR * i);
+        float v[L::kGV], lm[L::kGV];
+        auto load = [&](const float* src, float (&dst)[L::kGV]) {
+          if (L::kGV == 4) {
+            const float4 x = *reinterpret_cast<const float4*>(src);
+            dst[0] = x.x, dst[1] = x.y, dst[L::kGV - 2] = x.z, dst[L::kGV - 1] = x.w;
+          } else {
+            const float2 x = *reinterpret_cast<const float2*>(src);
+            dst[0] = x.x, dst[1] = x.y;
+          }
+        };
+        load(s_part + (size_t)srow * kSPad + n0, v);
 #pragma unroll
-        for (int k2 = 0; k2 < L::kKS; ++k2) {
-          const float4 x = *reinterpret_cast<const float4*>(s_part + ((size_t)k2 * L::kRows + srow) * kSPad + tk);
-          v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+        for (int k2 = 1; k2 < L::kKS; ++k2) {
+          float x[L::kGV];
+          load(s_part + ((size_t)k2 * L::kRows + srow) * kSPad + n0, x);
+#pragma unroll
+          for (int k = 0; k < L::kGV; ++k) v[k] += x[k];
         }
-        const float vv[4] = {v.x, v.y, v.z, v.w};
-        const float4 sc = *reinterpret_cast<const float4*>(tok_scale + tk);
-        const float scs[4] = {sc.x, sc.y, sc.z, sc.w};
-        const float4 lm = *reinterpret_cast<const float4*>(s_lam + tk);
-        const float lms[4] = {lm.x, lm.y, lm.z, lm.w};
+        load(s_scale + n0, sc[i]);
+        load(s_lam + n0, lm);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const bool seen = t * kTile + tk + k < limit && !(scs[k] < 0.f);
-          z[i][k] = seen ? vv[k] : -INFINITY;
-          mx = fmaxf(mx, z[i][k] + lms[k]);
+        for (int k = 0; k < L::kGV; ++k) {
+          const bool seen = t * kTile + lat_token(n0 + k) < limit && !(sc[i][k] < 0.f);
+          z[i][k] = seen ? v[k] : -INFINITY;
+          mx = fmaxf(mx, z[i][k] + lm[k]);
         }
       }
 #pragma unroll
@@ -477,20 +499,16 @@ __global__ void __launch_bounds__(kLatThreads, 1) latent_attention_kernel(const 
       l_run *= alpha;
 #pragma unroll
       for (int i = 0; i < L::kSeg; ++i) {
-        const int tk = 4 * (sj + L::kTPR * i);
-        const float4 sc = *reinterpret_cast<const float4*>(tok_scale + tk);
-        const float scs[4] = {sc.x, sc.y, sc.z, sc.w};
-        float pr[4];
+        float pr[L::kGV];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < L::kGV; ++k) {
           const float e = ex2_approx(z[i][k] - m_new);
           l_run += e;
-          pr[k] = e * (scs[k] * kPTop);
+          pr[k] = e * (sc[i][k] * kPTop);
         }
-        uint2 w;
-        w.x = pack_half2(pr[0], pr[1]);
-        w.y = pack_half2(pr[2], pr[3]);
-        *reinterpret_cast<uint2*>(s_p + srow * kPPad + tk) = w;
+        __half* dst = s_p + srow * kPPad + L::kGV * (sj + L::kTPR * i);
+#pragma unroll
+        for (int k = 0; k < L::kGV; k += 2) *reinterpret_cast<uint32_t*>(dst + k) = pack_half2(pr[k], pr[k + 1]);
       }
       if (sj == 0) s_alpha[srow] = alpha;
       __syncthreads();
@@ -524,19 +542,19 @@ __global__ void __launch_bounds__(kLatThreads, 1) latent_attention_kernel(const 
         for (int i = 0; i < kMT; ++i)
           ldsm_x4(p_s + ((16 * i + (lane & 15)) * kPPad + 16 * kk + 8 * (lane >> 4)) * 2, pa[i][0], pa[i][1], pa[i][2],
                   pa[i][3]);
-        // matrices of a transposed load: (tokens 0-7 | 8-15 of the step) x (chunk ch | ch + 1)
+        // matrices of a transposed load: (columns 0-7 | 8-15 of the step) x (chunk ch | ch + 1)
         constexpr int kChunks = L::kDW / 16;
         static_assert(kChunks >= 1, "a warp owns whole 16-dim chunks");
-        const int r = 16 * kk + (lane & 7) + 8 * ((lane >> 3) & 1);
+        const int in8 = lat_token(lane & 7), r = 16 * kk + 8 * ((lane >> 3) & 1) + in8;
 #pragma unroll
         for (int ch0 = 0; ch0 < kChunks; ch0 += 2) {
           uint32_t v[4];
-          // with one chunk a warp (dc = 128) the second pair of matrices repeats the first
+          // with one chunk a warp the second pair of matrices repeats the first
           const int ch = warp * kChunks + ch0 + (kChunks > 1 ? (lane >> 4) : 0);
-          ldsm_x4_trans(base + r * kDC + ((ch ^ lat_swz(r)) << 4), v[0], v[1], v[2], v[3]);
+          ldsm_x4_trans(base + (ch >> 3) * (kTile * 128) + r * 128 + (((ch & 7) ^ in8) << 4), v[0], v[1], v[2], v[3]);
 #pragma unroll
           for (int u = 0; u < (kChunks > 1 ? 2 : 1); ++u) {
-            // bytes [token 2c: dims 2g, 2g + 1][token 2c + 1: the same]; even dims form one
+            // bytes [column 2c: dims 2g, 2g + 1][column 2c + 1: the same]; even dims form one
             // n-tile, odd dims the next
             const uint32_t x0 = v[2 * u] ^ 0x80808080u, x1 = v[2 * u + 1] ^ 0x80808080u;
             const __half2 base2 = __half2half2(__ushort_as_half((unsigned short)0x6480));  // 1152
@@ -555,7 +573,6 @@ __global__ void __launch_bounds__(kLatThreads, 1) latent_attention_kernel(const 
         }
       }
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
 
     // ---- close the piece: normalise
     float l = l_run;
@@ -597,81 +614,75 @@ __global__ void __launch_bounds__(kLatThreads, 1) latent_attention_kernel(const 
 }
 
 // Joins the partials of each (request, row block) that several shares hold, and writes zeros
-// for requests without tokens.  One CTA per (request, row block, 4 rows); a warp a row.
-constexpr int kMergeWarps = 4;
+// for requests without tokens.  One CTA a row, four dims a thread; the weights of up to
+// kMergeChunk shares at a time are formed together, then their rows are added up.
+constexpr int kMergeChunk = 128;
 
-__global__ void __launch_bounds__(kMergeWarps * 32) latent_merge_kernel(const LatentParams p, int block_rows, int dc,
-                                                                       int ctas) {
-  const int groups = (block_rows + kMergeWarps - 1) / kMergeWarps;
-  const int grp = blockIdx.x % groups, item = blockIdx.x / groups, rb = item % p.row_blocks, b = item / p.row_blocks;
-  const int lane = threadIdx.x & 31;
-  const int r = grp * kMergeWarps + (threadIdx.x >> 5), row = rb * block_rows + r;
-  if (r >= block_rows || row >= p.R) return;
+__global__ void __launch_bounds__(128) latent_merge_kernel(const LatentParams p, int block_rows, int dc, int ctas) {
+  __shared__ float s_w[kMergeChunk];
+  __shared__ float s_max[4];
+  cudaGridDependencySynchronize();  // launched early: the shares' results are there now
+  const int row = blockIdx.x % p.R, b = blockIdx.x / p.R, rb = row / block_rows, r = row - rb * block_rows;
+  const int tid = threadIdx.x, threads = blockDim.x;
   const int nt = p.prefix[b + 1] - p.prefix[b];
-  uint16_t* out = p.out + ((size_t)b * p.R + row) * dc;
+  uint16_t* out = p.out + ((size_t)b * p.R + row) * dc + 4 * tid;
   if (nt == 0) {
-    for (int d = 4 * lane; d < dc; d += 128) *reinterpret_cast<uint2*>(out + d) = make_uint2(0u, 0u);
+    *reinterpret_cast<uint2*>(out) = make_uint2(0u, 0u);
     return;
   }
   const int64_t total = (int64_t)p.prefix[p.B] * p.row_blocks;
+  const int C = (int)min((int64_t)ctas, total);
   const int64_t f0 = (int64_t)p.prefix[b] * p.row_blocks + (int64_t)rb * nt, f1 = f0 + nt;
   // the share that holds flat tile f: the last one that starts at or before it
   auto owner = [&](int64_t f) -> int {
-    int k = (int)min((int64_t)ctas - 1, (f + 1) * ctas / total);
-    while (k > 0 && latent_share(total, k, ctas) > f) --k;
-    while (k + 1 < ctas && latent_share(total, k + 1, ctas) <= f) ++k;
+    int k = (int)min((int64_t)C - 1, (f + 1) * C / total);
+    while (k > 0 && latent_share(total, k, C) > f) --k;
     return k;
   };
   const int k0 = owner(f0), k1 = owner(f1 - 1);
   if (k0 == k1) return;  // one share wrote the output itself
-  // the first share's piece is its first one only if the share starts in this row block
-  auto slot = [&](int k) -> size_t {
-    const bool is_first = k > k0 || latent_share(total, k, ctas) >= f0;
-    return ((size_t)k * 2 + (is_first ? 0 : 1)) * block_rows + r;
-  };
+  // a share's first piece is in slot 0; the first share's piece is a later one where the
+  // share starts before this row block
+  const size_t late = latent_share(total, k0, C) < f0 ? 1 : 0;
+  auto slot = [&](int k) -> size_t { return ((size_t)k * 2 + (k == k0 ? late : 0)) * block_rows + r; };
   float M = -INFINITY;
   bool nan = false;
-  for (int k = k0 + lane; k <= k1; k += 32) {
-    if (latent_share(total, k, ctas) == latent_share(total, k + 1, ctas)) continue;  // an empty share
+  for (int k = k0 + tid; k <= k1; k += threads) {
     const float x = p.part_lse[slot(k)];
     nan |= isnan(x);
     M = fmaxf(M, x);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  if (__any_sync(0xffffffffu, nan)) M = __int_as_float(0x7fc00000);
+  if ((tid & 31) == 0) s_max[tid >> 5] = M;
+  nan = __syncthreads_or(nan ? 1 : 0) != 0;
+  for (int i = 0; i < threads / 32; ++i) M = fmaxf(M, s_max[i]);
+  if (nan) M = __int_as_float(0x7fc00000);
   float W = 0.f;
-  float4 acc[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   if (M != -INFINITY) {
-    for (int k = k0; k <= k1; ++k) {
-      if (latent_share(total, k, ctas) == latent_share(total, k + 1, ctas)) continue;
-      const size_t s = slot(k);
-      const float w = exp2f(p.part_lse[s] - M);
-      W += w;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int d = 4 * lane + 128 * j;
-        if (d >= dc) break;
-        const float4 v = *reinterpret_cast<const float4*>(p.part_o + s * dc + d);
-        acc[j].x = fmaf(w, v.x, acc[j].x);
-        acc[j].y = fmaf(w, v.y, acc[j].y);
-        acc[j].z = fmaf(w, v.z, acc[j].z);
-        acc[j].w = fmaf(w, v.w, acc[j].w);
+    for (int c0 = k0; c0 <= k1; c0 += kMergeChunk) {
+      const int n = min(kMergeChunk, k1 + 1 - c0);
+      __syncthreads();
+      for (int i = tid; i < n; i += threads) s_w[i] = exp2f(p.part_lse[slot(c0 + i)] - M);
+      __syncthreads();
+#pragma unroll 8
+      for (int i = 0; i < n; ++i) {
+        const float w = s_w[i];
+        const float4 v = *reinterpret_cast<const float4*>(p.part_o + slot(c0 + i) * dc + 4 * tid);
+        W += w;
+        acc.x = fmaf(w, v.x, acc.x);
+        acc.y = fmaf(w, v.y, acc.y);
+        acc.z = fmaf(w, v.z, acc.z);
+        acc.w = fmaf(w, v.w, acc.w);
       }
     }
   }
   const float inv = W > 0.f ? 1.f / W : (W == 0.f ? 0.f : W);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int d = 4 * lane + 128 * j;
-    if (d >= dc) break;
-    uint2 w;
-    w.x = (uint32_t)lat_b16(acc[j].x * inv, p.bf16) | ((uint32_t)lat_b16(acc[j].y * inv, p.bf16) << 16);
-    w.y = (uint32_t)lat_b16(acc[j].z * inv, p.bf16) | ((uint32_t)lat_b16(acc[j].w * inv, p.bf16) << 16);
-    *reinterpret_cast<uint2*>(out + d) = w;
-  }
+  uint2 w;
+  w.x = (uint32_t)lat_b16(acc.x * inv, p.bf16) | ((uint32_t)lat_b16(acc.y * inv, p.bf16) << 16);
+  w.y = (uint32_t)lat_b16(acc.z * inv, p.bf16) | ((uint32_t)lat_b16(acc.w * inv, p.bf16) << 16);
+  *reinterpret_cast<uint2*>(out) = w;
 }
 
 // ---------------------------------------------------------------------------------
@@ -692,16 +703,17 @@ static int latent_check(const FsLatentArgs* a) {
     return FS_ERR_INVALID_ARGUMENT;
   if (a->dtype != FS_F16 && a->dtype != FS_BF16) return FS_ERR_UNSUPPORTED;
   if (!latent_dims_ok(a->latent_dim, a->rope_dim, a->page_size) || a->batch > kLatMaxBatch) return FS_ERR_UNSUPPORTED;
-  if ((int64_t)a->tokens * a->heads > (1 << 20)) return FS_ERR_UNSUPPORTED;
+  if ((int64_t)a->tokens * a->heads > (1 << 20) || (int64_t)a->tokens * a->heads * a->batch >= (1ll << 31))
+    return FS_ERR_UNSUPPORTED;
+  if (a->num_pages * a->page_size >= (1ll << 31) || a->num_pages >= (1ll << 31)) return FS_ERR_UNSUPPORTED;
   if ((int64_t)a->table_cols * a->page_size >= (1ll << 31) - kTile) return FS_ERR_UNSUPPORTED;
   // flat tiles are counted in 32 bits before the row blocks
   const int64_t longest = std::min<int64_t>(a->max_seq_len, (int64_t)a->table_cols * a->page_size);
   if ((longest / kTile + 1) * a->batch >= (1ll << 31)) return FS_ERR_UNSUPPORTED;
   if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->q_rope) |
        reinterpret_cast<uintptr_t>(a->values) | reinterpret_cast<uintptr_t>(a->ropes) |
-       reinterpret_cast<uintptr_t>(a->out)) & 15)
+       reinterpret_cast<uintptr_t>(a->scale) | reinterpret_cast<uintptr_t>(a->out)) & 15)
     return FS_ERR_ALIGNMENT;
-  if (reinterpret_cast<uintptr_t>(a->scale) & 3) return FS_ERR_ALIGNMENT;
   return FS_OK;
 }
 
@@ -725,34 +737,48 @@ static LatentPlan latent_plan(const FsLatentArgs* a, int device) {
 }
 
 template <int kDC, int kDR, int kMT>
-static int launch_latent(const LatentParams& p, const LatentPlan& pl, void* stream) {
+static int launch_latent(const FsLatentArgs* a, const LatentParams& p, const LatentPlan& pl, void* stream) {
   using L = LatentShape<kDC, kDR, kMT>;
   static_assert(L::smem(kLatMaxBatch) <= 227 * 1024, "shared memory of a CTA");
-  const int smem = L::smem(p.B);
+  CUtensorMap map_v, map_r;
+  const uint64_t rows = (uint64_t)a->num_pages * a->page_size;
+  const uint32_t box_rows = (uint32_t)std::min(a->page_size, kTile);
+  if (int st = make_byte_map(&map_v, a->values, rows, kDC, box_rows, 128); st != FS_OK) return st;
+  if (int st = make_byte_map(&map_r, a->ropes, rows, 2 * kDR, box_rows, 2 * kDR); st != FS_OK) return st;
   auto kernel = p.bf16 ? latent_attention_kernel<kDC, kDR, kMT, true> : latent_attention_kernel<kDC, kDR, kMT, false>;
   if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::smem(kLatMaxBatch));
       e != cudaSuccess)
     return fail_cuda("shared-memory limit of the latent attention kernel", e);
-  kernel<<<pl.ctas, kLatThreads, smem, reinterpret_cast<cudaStream_t>(stream)>>>(p);
+  kernel<<<pl.ctas, L::kThreads, L::smem(p.B), reinterpret_cast<cudaStream_t>(stream)>>>(map_v, map_r, p);
   if (int st = launch_status("latent attention kernel launch"); st != FS_OK) return st;
-  const int64_t blocks = (int64_t)p.B * p.row_blocks * ((L::kRows + kMergeWarps - 1) / kMergeWarps);
-  latent_merge_kernel<<<(unsigned)blocks, kMergeWarps * 32, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
-      p, L::kRows, kDC, pl.ctas);
-  return launch_status("latent merge kernel launch");
+  // the merge is launched while the shares still run and waits for them on the device
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(p.B * p.R));
+  cfg.blockDim = dim3(kDC / 4);
+  cfg.stream = reinterpret_cast<cudaStream_t>(stream);
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (cudaError_t e = cudaLaunchKernelEx(&cfg, latent_merge_kernel, p, L::kRows, kDC, pl.ctas); e != cudaSuccess)
+    return fail_cuda("latent merge kernel launch", e);
+  return FS_OK;
 }
 
 template <int kDC, int kDR>
-static int launch_latent_rows(const LatentParams& p, const LatentPlan& pl, void* stream) {
+static int launch_latent_rows(const FsLatentArgs* a, const LatentParams& p, const LatentPlan& pl, void* stream) {
   switch (pl.mt) {
-    case 1: return launch_latent<kDC, kDR, 1>(p, pl, stream);
-    case 2: return launch_latent<kDC, kDR, 2>(p, pl, stream);
-    default: return launch_latent<kDC, kDR, 4>(p, pl, stream);
+    case 1: return launch_latent<kDC, kDR, 1>(a, p, pl, stream);
+    case 2: return launch_latent<kDC, kDR, 2>(a, p, pl, stream);
+    default: return launch_latent<kDC, kDR, 4>(a, p, pl, stream);
   }
 }
 
 template <int kDC>
-static int launch_latent_rope(const LatentParams& p, const LatentPlan& pl, int dr, void* stream) {
-  return dr == 64 ? launch_latent_rows<kDC, 64>(p, pl, stream) : launch_latent_rows<kDC, 32>(p, pl, stream);
+static int launch_latent_rope(const FsLatentArgs* a, const LatentParams& p, const LatentPlan& pl, void* stream) {
+  return a->rope_dim == 64 ? launch_latent_rows<kDC, 64>(a, p, pl, stream)
+                           : launch_latent_rows<kDC, 32>(a, p, pl, stream);
 }
 
 }  // namespace fsb
@@ -819,14 +845,11 @@ int fs_latent_attention(const FsLatentArgs* a, void* stream) {
   const LatentPlan pl = latent_plan(a, device);
   if (a->workspace == nullptr || a->workspace_bytes < pl.o + pl.lse + pl.prefix) return FS_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(a->workspace) & 255) return FS_ERR_ALIGNMENT;
-  if ((int64_t)a->batch * pl.row_blocks * 16 >= (1ll << 31)) return FS_ERR_UNSUPPORTED;
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
   LatentParams p{};
   p.q = static_cast<const uint16_t*>(a->q);
   p.q_rope = static_cast<const uint16_t*>(a->q_rope);
-  p.values = a->values;
   p.scale = a->scale;
-  p.ropes = static_cast<const uint16_t*>(a->ropes);
   p.table = a->block_table;
   p.lengths = a->lengths;
   p.out = static_cast<uint16_t*>(a->out);
@@ -846,9 +869,9 @@ int fs_latent_attention(const FsLatentArgs* a, void* stream) {
   p.cols = a->table_cols;
   p.bf16 = a->dtype == FS_BF16;
   switch (a->latent_dim) {
-    case 128: return launch_latent_rope<128>(p, pl, a->rope_dim, stream);
-    case 256: return launch_latent_rope<256>(p, pl, a->rope_dim, stream);
-    default: return launch_latent_rope<512>(p, pl, a->rope_dim, stream);
+    case 128: return launch_latent_rope<128>(a, p, pl, stream);
+    case 256: return launch_latent_rope<256>(a, p, pl, stream);
+    default: return launch_latent_rope<512>(a, p, pl, stream);
   }
 }
 
