@@ -9,8 +9,8 @@
 //
 // latent_attention_kernel.  Rows (t, h) of a request are cut into blocks of up to 16, 32 or
 // 64; the flattened list of (request, row block, tile of 64 tokens) is cut into equal
-// contiguous shares, one per CTA (lengths are read on the device).  Warp 0 keeps three tiles
-// in flight with TMA (128-byte swizzle; page lookups run a tile ahead).  Per tile:
+// contiguous shares, one per CTA (lengths are read on the device).  Warp 0 keeps two or three
+// tiles in flight with TMA (128-byte swizzle; page lookups run a tile ahead).  Per tile:
 //   1. S = Q C^T on the int8 tensor cores, straight from the stored bytes: q is held as
 //      16-bit fixed point in two signed bytes (error max|q| 2^-16 of a row), two exact
 //      MMAs; the rotary part on 16-bit MMAs.  The warps split rows, dims and tokens (kMT x
@@ -18,7 +18,7 @@
 //   2. softmax: running maximum m of score + log2(scale) and sum of 2^(score - m) per row in
 //      fp32; P = 2^(score - m) * scale in fp16, scaled by 2^14 to use its range whatever the
 //      scale (the largest P is 2^14).
-//   3. O += P C: each warp owns dc / 16 dims of all rows.  A byte becomes the exact fp16
+//   3. O += P C: each warp owns its part of the dims, of all rows.  A byte becomes the exact fp16
 //      integer (XOR and byte permute against 0x64 exponent bytes, minus 1152).
 // A share that holds a whole (request, row block) writes the output; others leave normalised
 // (O, LSE) partials that latent_merge_kernel joins.
@@ -115,7 +115,6 @@ __global__ void __launch_bounds__(kAppendWarps * 32) latent_append_kernel(const 
 // ---------------------------------------------------------------------------------
 
 constexpr int kTile = 64;  // tokens
-constexpr int kLatStages = 3;
 constexpr int kSPad = 72;  // floats a row of partial scores
 constexpr int kPPad = 72;  // halves a row of P
 constexpr int kLatMaxBatch = 4096;
@@ -149,11 +148,15 @@ __device__ __forceinline__ int lat_token(int n) { return (n & ~7) | ((n >> 1) & 
 
 template <int kDC, int kDR, int kMT>
 struct LatentShape {
-  static constexpr int kWarps = kDC >= 256 ? 16 : 8;
+  // One 16-row block: two CTAs of 8 warps an SM, whose phases overlap; more rows: one CTA of
+  // 16 warps (the scores' partial sums and O would not fit twice).
+  static constexpr int kCtas = kMT == 1 ? 2 : 1;
+  static constexpr int kStages = kMT == 1 ? 2 : 3;
+  static constexpr int kWarps = kMT > 1 && kDC >= 256 ? 16 : 8;
   static constexpr int kThreads = 32 * kWarps;
   static constexpr int kRows = 16 * kMT;
   // warps = kMT row groups x kKS slices of the dims (64 at least) x kTS token groups
-  static constexpr int kMaxKS = kMT == 1 ? 8 : 4;
+  static constexpr int kMaxKS = 4;
   static constexpr int kKS = kMaxKS < kDC / 64 ? kMaxKS : kDC / 64;
   static constexpr int kTS = kWarps / (kMT * kKS);
   static constexpr int kSlice = kDC / kKS;     // dims of a warp's QK slice
@@ -170,7 +173,7 @@ struct LatentShape {
   static constexpr int kStage = (kValBytes + kRopeBytes + kTile * 4 + 1023) / 1024 * 1024;
   static constexpr int kSBytes = kKS * kRows * kSPad * 4;
   static constexpr int kPBytes = kRows * kPPad * 2;
-  static constexpr int kOffS = kLatStages * kStage;
+  static constexpr int kOffS = kStages * kStage;
   static constexpr int kOffP = kOffS + kSBytes;
   static constexpr int kOffMisc = kOffP + kPBytes;  // alpha [rows], qscale [rows], scale and lam [tile], prefix
   static constexpr int kMiscFloats = 2 * kRows + 2 * kTile;
@@ -220,13 +223,13 @@ __device__ __forceinline__ void latent_prefix(const LatentParams& p, int* pre) {
 __device__ __forceinline__ int64_t latent_share(int64_t n, int k, int C) { return n * k / C; }
 
 template <int kDC, int kDR, int kMT, bool kBf16>
-__global__ void __launch_bounds__(LatentShape<kDC, kDR, kMT>::kThreads, 1)
+__global__ void __launch_bounds__(LatentShape<kDC, kDR, kMT>::kThreads, LatentShape<kDC, kDR, kMT>::kCtas)
     latent_attention_kernel(const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_r,
                             const LatentParams p) {
   using L = LatentShape<kDC, kDR, kMT>;
   extern __shared__ uint8_t lat_raw[];
-  __shared__ alignas(8) uint64_t s_full[kLatStages];
-  __shared__ uint32_t s_pages[kLatStages];  // which of a tile's pages are there, one bit each
+  __shared__ alignas(8) uint64_t s_full[L::kStages];
+  __shared__ uint32_t s_pages[L::kStages];  // which of a tile's pages are there, one bit each
   const uint32_t raw_s = smem_u32(lat_raw);
   const uint32_t smem_s = (raw_s + 1023u) & ~1023u;
   uint8_t* lat_smem = lat_raw + (smem_s - raw_s);
@@ -243,7 +246,7 @@ __global__ void __launch_bounds__(LatentShape<kDC, kDR, kMT>::kThreads, 1)
   const int mt = warp % kMT, ks = (warp / kMT) % L::kKS, ts = warp / (kMT * L::kKS);
 
   if (tid == 0) {
-    for (int i = 0; i < kLatStages; ++i) mbar_init(smem_u32(&s_full[i]), 1);
+    for (int i = 0; i < L::kStages; ++i) mbar_init(smem_u32(&s_full[i]), 1);
     fence_mbar_init();
     fence_proxy_async_smem();
   }
@@ -290,7 +293,7 @@ __global__ void __launch_bounds__(LatentShape<kDC, kDR, kMT>::kThreads, 1)
       return phys;
     };
     auto issue = [&](int t, int64_t phys) {  // tile t into the ring
-      const int st = (int)(issued % kLatStages);
+      const int st = (int)(issued % L::kStages);
       const uint32_t base = smem_s + st * L::kStage, bar = smem_u32(&s_full[st]);
       const uint32_t there = __ballot_sync(0xffffffffu, phys >= 0);
       if (lane == 0) {
@@ -313,8 +316,8 @@ __global__ void __launch_bounds__(LatentShape<kDC, kDR, kMT>::kThreads, 1)
     int64_t next_phys = -1;
     __syncthreads();  // the previous piece is done with the stages and the row state
     if (warp == 0) {
-      for (int i = 0; i < kLatStages - 1 && t0 + i < t1; ++i) issue(t0 + i, lookup(t0 + i));
-      next_phys = lookup(t0 + kLatStages - 1);
+      for (int i = 0; i < L::kStages - 1 && t0 + i < t1; ++i) issue(t0 + i, lookup(t0 + i));
+      next_phys = lookup(t0 + L::kStages - 1);
     }
 
     // ---- q as 16-bit fixed point: row scales, then this warp's fragments
@@ -395,15 +398,15 @@ __global__ void __launch_bounds__(LatentShape<kDC, kDR, kMT>::kThreads, 1)
     const int limit = min(len, len - p.T + 1 + (row0 + srow) / p.H);
 
     for (int t = t0; t < t1; ++t, ++used) {
-      const int st = (int)(used % kLatStages);
+      const int st = (int)(used % L::kStages);
       const uint32_t base = smem_s + st * L::kStage;
       const float* tok_scale =
           reinterpret_cast<const float*>(lat_smem + st * L::kStage + L::kValBytes + L::kRopeBytes);
-      const bool here = mbar_wait_bounded(smem_u32(&s_full[st]), (used / kLatStages) & 1u, kLatTimeoutNs);
+      const bool here = mbar_wait_bounded(smem_u32(&s_full[st]), (used / L::kStages) & 1u, kLatTimeoutNs);
 
       // ---- 1. partial scores of this warp's rows, dims and tokens
       const int prow = lat_token(g);  // row of column g of a group
-#pragma unroll
+#pragma unroll 2
       for (int n = 0; n < L::kNT; ++n) {
         const int col = (ts * L::kNT + n) * 8, brow = col + prow;
         int sh[4] = {0, 0, 0, 0}, sl[4] = {0, 0, 0, 0};
@@ -452,10 +455,10 @@ __global__ void __launch_bounds__(LatentShape<kDC, kDR, kMT>::kThreads, 1)
         if (tid == 0 && p.status != nullptr) atomicOr(p.status, FS_DEV_TIMEOUT);
         return;
       }
-      // every warp is done with tile t - 1: its stage takes tile t + kLatStages - 1
-      if (warp == 0 && t + kLatStages - 1 < t1) {
-        issue(t + kLatStages - 1, next_phys);
-        next_phys = lookup(t + kLatStages);
+      // every warp is done with tile t - 1: its stage takes tile t + L::kStages - 1
+      if (warp == 0 && t + L::kStages - 1 < t1) {
+        issue(t + L::kStages - 1, next_phys);
+        next_phys = lookup(t + L::kStages);
       }
 
       // ---- 2. softmax of row srow
@@ -537,23 +540,19 @@ __global__ void __launch_bounds__(LatentShape<kDC, kDR, kMT>::kThreads, 1)
       const uint32_t p_s = smem_s + L::kOffP;
 #pragma unroll
       for (int kk = 0; kk < kTile / 16; ++kk) {
-        uint32_t pa[kMT][4];
-#pragma unroll
-        for (int i = 0; i < kMT; ++i)
-          ldsm_x4(p_s + ((16 * i + (lane & 15)) * kPPad + 16 * kk + 8 * (lane >> 4)) * 2, pa[i][0], pa[i][1], pa[i][2],
-                  pa[i][3]);
         // matrices of a transposed load: (columns 0-7 | 8-15 of the step) x (chunk ch | ch + 1)
         constexpr int kChunks = L::kDW / 16;
-        static_assert(kChunks >= 1, "a warp owns whole 16-dim chunks");
+        static_assert(kChunks == 1 || kChunks % 2 == 0, "a warp owns whole pairs of 16-dim chunks, or one chunk");
+        constexpr int kPair = kChunks > 1 ? 2 : 1;
         const int in8 = lat_token(lane & 7), r = 16 * kk + 8 * ((lane >> 3) & 1) + in8;
 #pragma unroll
         for (int ch0 = 0; ch0 < kChunks; ch0 += 2) {
-          uint32_t v[4];
+          uint32_t v[4], bf[kPair][4];
           // with one chunk a warp the second pair of matrices repeats the first
           const int ch = warp * kChunks + ch0 + (kChunks > 1 ? (lane >> 4) : 0);
           ldsm_x4_trans(base + (ch >> 3) * (kTile * 128) + r * 128 + (((ch & 7) ^ in8) << 4), v[0], v[1], v[2], v[3]);
 #pragma unroll
-          for (int u = 0; u < (kChunks > 1 ? 2 : 1); ++u) {
+          for (int u = 0; u < kPair; ++u) {
             // bytes [column 2c: dims 2g, 2g + 1][column 2c + 1: the same]; even dims form one
             // n-tile, odd dims the next
             const uint32_t x0 = v[2 * u] ^ 0x80808080u, x1 = v[2 * u + 1] ^ 0x80808080u;
@@ -563,11 +562,17 @@ __global__ void __launch_bounds__(LatentShape<kDC, kDR, kMT>::kThreads, 1)
               const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&h), base2);
               return *reinterpret_cast<const uint32_t*>(&d);
             };
-            const uint32_t e0 = cvt(x0, 0x4240u), e1 = cvt(x1, 0x4240u), o0 = cvt(x0, 0x4341u), o1 = cvt(x1, 0x4341u);
+            bf[u][0] = cvt(x0, 0x4240u), bf[u][1] = cvt(x1, 0x4240u);
+            bf[u][2] = cvt(x0, 0x4341u), bf[u][3] = cvt(x1, 0x4341u);
+          }
 #pragma unroll
-            for (int i = 0; i < kMT; ++i) {
-              mma_16816(acc[i][2 * (ch0 + u)], pa[i][0], pa[i][1], pa[i][2], pa[i][3], e0, e1);
-              mma_16816(acc[i][2 * (ch0 + u) + 1], pa[i][0], pa[i][1], pa[i][2], pa[i][3], o0, o1);
+          for (int i = 0; i < kMT; ++i) {
+            uint32_t pa[4];
+            ldsm_x4(p_s + ((16 * i + (lane & 15)) * kPPad + 16 * kk + 8 * (lane >> 4)) * 2, pa[0], pa[1], pa[2], pa[3]);
+#pragma unroll
+            for (int u = 0; u < kPair; ++u) {
+              mma_16816(acc[i][2 * (ch0 + u)], pa[0], pa[1], pa[2], pa[3], bf[u][0], bf[u][1]);
+              mma_16816(acc[i][2 * (ch0 + u) + 1], pa[0], pa[1], pa[2], pa[3], bf[u][2], bf[u][3]);
             }
           }
         }
@@ -728,7 +733,7 @@ static LatentPlan latent_plan(const FsLatentArgs* a, int device) {
   pl.mt = R <= 16 ? 1 : R <= 32 ? 2 : 4;
   const int rows = 16 * pl.mt;
   pl.row_blocks = (R + rows - 1) / rows;
-  pl.ctas = device_sm_count(device);
+  pl.ctas = device_sm_count(device) * (pl.mt == 1 ? 2 : 1);  // LatentShape::kCtas on every SM
   auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
   pl.o = up((size_t)pl.ctas * 2 * rows * a->latent_dim * 4);
   pl.lse = up((size_t)pl.ctas * 2 * rows * 4);
@@ -739,7 +744,7 @@ static LatentPlan latent_plan(const FsLatentArgs* a, int device) {
 template <int kDC, int kDR, int kMT>
 static int launch_latent(const FsLatentArgs* a, const LatentParams& p, const LatentPlan& pl, void* stream) {
   using L = LatentShape<kDC, kDR, kMT>;
-  static_assert(L::smem(kLatMaxBatch) <= 227 * 1024, "shared memory of a CTA");
+  static_assert(L::smem(kLatMaxBatch) <= 227 * 1024 && L::kCtas * (L::smem(1024) + 1024) <= 228 * 1024, "shared memory of a CTA");
   CUtensorMap map_v, map_r;
   const uint64_t rows = (uint64_t)a->num_pages * a->page_size;
   const uint32_t box_rows = (uint32_t)std::min(a->page_size, kTile);
