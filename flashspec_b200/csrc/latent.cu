@@ -152,11 +152,11 @@ struct LatentShape {
   // 16 warps (the scores' partial sums and O would not fit twice).
   static constexpr int kCtas = kMT == 1 ? 2 : 1;
   static constexpr int kStages = kMT == 1 ? 2 : 3;
-  static constexpr int kWarps = kMT > 1 && kDC >= 256 ? 16 : 8;
+  static constexpr int kWarps = kMT == 2 && kDC >= 256 ? 16 : 8;
   static constexpr int kThreads = 32 * kWarps;
   static constexpr int kRows = 16 * kMT;
   // warps = kMT row groups x kKS slices of the dims (64 at least) x kTS token groups
-  static constexpr int kMaxKS = 4;
+  static constexpr int kMaxKS = kWarps / kMT < 4 ? kWarps / kMT : 4;
   static constexpr int kKS = kMaxKS < kDC / 64 ? kMaxKS : kDC / 64;
   static constexpr int kTS = kWarps / (kMT * kKS);
   static constexpr int kSlice = kDC / kKS;     // dims of a warp's QK slice
@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(LatentShape<kDC, kDR, kMT>::kThreads, LatentSh
 
       // ---- 1. partial scores of this warp's rows, dims and tokens
       const int prow = lat_token(g);  // row of column g of a group
-#pragma unroll 2
+#pragma unroll 4
       for (int n = 0; n < L::kNT; ++n) {
         const int col = (ts * L::kNT + n) * 8, brow = col + prow;
         int sh[4] = {0, 0, 0, 0}, sl[4] = {0, 0, 0, 0};
