@@ -19,7 +19,7 @@ LIB = PKG / "libflashspec_b200.so"
 SOURCES = ["decode.cu", "decode_generic.cu", "quant.cu", "noalloc.cu", "exchange.cu", "probe.cu", "tree.cu",
            "weights.cu", "evict.cu", "latent.cu", "latent_prefill.cu"]
 HEADERS = ["ptx.cuh", "common.h", "generic.h", "weights.h", "xwords.cuh",
-           "quant_math.cuh", "tensor_map.h"]
+           "quant_math.cuh", "tensor_map.h", "tcgen05.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-O2", f"-I{ROOT / 'include'}"]
 

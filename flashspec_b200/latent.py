@@ -214,7 +214,8 @@ def latent_attention_cuda(q_latent: torch.Tensor, q_rope: torch.Tensor, cache: L
 
 def latent_prefill_attention_cuda(q: torch.Tensor, kv: torch.Tensor, k_rope: torch.Tensor, q_offsets: torch.Tensor,
                                   k_offsets: torch.Tensor, *, sm_scale: Optional[float] = None,
-                                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                                  out: Optional[torch.Tensor] = None,
+                                  device_status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Expanded latent attention of packed prompts, causal, aligned at the end.
 
     q [Nq, H, dn + dr]; kv [Nk, H, dn + dv], every head's key part and value expanded from the
@@ -260,6 +261,7 @@ def latent_prefill_attention_cuda(q: torch.Tensor, kv: torch.Tensor, k_rope: tor
         a.dtype, a.batch, a.heads = _dtype(q), int(qo.shape[0]) - 1, h
         a.nope_dim, a.rope_dim, a.value_dim = dn, dr, dv
         a.sm_scale = 1.0 / math.sqrt(dq) if sm_scale is None else float(sm_scale)
+        a.device_status = device_status.data_ptr() if device_status is not None else None
         _lib.check(_lib.load().fs_latent_prefill(C.byref(a), stream_of(device)), "fs_latent_prefill")
     return out
 
