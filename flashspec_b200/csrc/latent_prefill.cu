@@ -272,13 +272,26 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       tmem_ld32(sb + 64 * half, raw[0]);
       tmem_ld32(sb + 64 * half + 32, raw[1]);
       tmem_wait_ld();
-      float x[64], mx = -INFINITY;
+      // tiles that every query sees whole keep the raw scores (the scale joins in the exponent's
+      // FMA); edge tiles are scaled and masked here
+      float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      if (edge) {
+        const int seen = limit - j0 - 64 * half;  // this thread's keys 0 .. seen
 #pragma unroll
-      for (int k = 0; k < 64; ++k) {
-        x[k] = __uint_as_float(raw[k >> 5][k & 31]) * p.scale_log2;
-        if (edge && j0 + 64 * half + k > limit) x[k] = -INFINITY;
-        mx = fmaxf(mx, x[k]);
+        for (int k = 0; k < 64; ++k) {
+          const float x = k > seen ? -INFINITY : __uint_as_float(raw[k >> 5][k & 31]) * p.scale_log2;
+          raw[k >> 5][k & 31] = __float_as_uint(x);
+          m4[k & 3] = fmaxf(m4[k & 3], x);
+        }
+      } else if (p.scale_log2 >= 0.f) {
+#pragma unroll
+        for (int k = 0; k < 64; ++k) m4[k & 3] = fmaxf(m4[k & 3], __uint_as_float(raw[k >> 5][k & 31]));
+      } else {
+#pragma unroll
+        for (int k = 0; k < 64; ++k) m4[k & 3] = fmaxf(m4[k & 3], -__uint_as_float(raw[k >> 5][k & 31]));
       }
+      const float mul = edge ? 1.f : p.scale_log2;
+      float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * fabsf(mul);
       s_half[st][half][row] = mx;
       if (any_of(!ok)) {  // after it, both halves have read their scores
         ok = false;
@@ -298,22 +311,27 @@ __global__ void __launch_bounds__(kPreThreads, 1)
           const uint32_t ob = tmem + lanes + L::kTmemO + half * (kDV / 2);
 #pragma unroll
           for (int c = 0; c < kDV / 64; ++c) {
-            tmem_ld32(ob + 32 * c, raw[0]);
+            uint32_t o[32];
+            tmem_ld32(ob + 32 * c, o);
             tmem_wait_ld();
 #pragma unroll
-            for (int k = 0; k < 32; ++k) raw[0][k] = __float_as_uint(__uint_as_float(raw[0][k]) * alpha);
-            tmem_st32(ob + 32 * c, raw[0]);
+            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+            tmem_st32(ob + 32 * c, o);
           }
         }
         m_ref = m_new;
       }
+      float l4[4] = {0.f, 0.f, 0.f, 0.f};
+      uint32_t packed[32];
 #pragma unroll
       for (int k = 0; k < 32; ++k) {
-        const float p0 = ex2_approx(x[2 * k] - m_ref), p1 = ex2_approx(x[2 * k + 1] - m_ref);
-        l += p0 + p1;
-        raw[0][k] = pre_pack<kBf16>(p0, p1);
+        const float p0 = ex2_approx(fmaf(__uint_as_float(raw[k >> 4][(2 * k) & 31]), mul, -m_ref));
+        const float p1 = ex2_approx(fmaf(__uint_as_float(raw[k >> 4][(2 * k + 1) & 31]), mul, -m_ref));
+        l4[k & 3] += p0 + p1;
+        packed[k] = pre_pack<kBf16>(p0, p1);
       }
-      tmem_st32(sb + 32 * half, raw[0]);
+      l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+      tmem_st32(sb + 32 * half, packed);
       if (edge) {
         constexpr uint16_t kExp = kBf16 ? 0x7f80 : 0x7c00;
         ok = pre_wait(&bars.v_full[st], (j >> 1) & 1, &s_abort) && ok;
