@@ -5,22 +5,23 @@
 //   score(i, h, j) = sm_scale * (q[i, h, :dn] . kv[j, h, :dn] + q[i, h, dn:] . k_rope[j])
 //   out[i, h]      = sum_j softmax_j(score) kv[j, h, dn:]
 //
-// A CTA takes 128 queries of one head and walks the keys in tiles of 128.  Roles:
-//   warp 0      TMA: Q once, then K (the head's own chunks and the shared rotary one, side by
-//               side, so it is never copied per head) and V tiles, two of each in flight
-//   warp 1      tcgen05.mma: S = Q K^T into one of two TMEM buffers, O += P V with P read
-//               from TMEM; S of the next tile is issued before P V of this one, so the tensor
-//               cores work while the softmax of a tile runs
-//   warps 4-11  softmax: two threads a row, 64 keys each (they meet over the row's maximum).
-//               P goes back to TMEM in 16 bits over the scores.  The reference maximum moves
-//               only when the true one is past it by more than 2^8 (P then stays below 256,
-//               sums are in fp32, and O is rescaled seldom instead of once a tile).
-// Bound by the tensor cores for long prompts: a tile is 128 x 128 x (dn + dr + dv) MACs.
+// A CTA takes 256 queries of one head, as two blocks of 128, and walks the keys in tiles of
+// 96.  (With 128 queries a CTA the K and V tiles, 80 KB per 128 keys, came out of L2 at 6.8
+// TB/s and bound the kernel: 220 us at the packed prompts; tiles of 96 keys let two K and two
+// V tiles fit beside the queries.)  Roles:
+//   warp 0      TMA: the queries once, then K (the head's own chunks and the shared rotary
+//               one, side by side, so it is never copied per head) and V tiles
+//   warp 1      tcgen05.mma: S = Q K^T into TMEM, O += P V with P read from TMEM
+//   warps 4-7   softmax of the first block, one thread a row; warps 8-11 of the second
+// The blocks do not wait for each other: the tensor cores work on one's tile while the other
+// forms exponentials.  P goes back to TMEM in 16 bits over the scores.  The reference maximum
+// moves only when the true one is past it by more than 2^8 (P then stays below 256, sums are
+// in fp32, and O is rescaled seldom instead of once a tile).
 //
 // A value that is not finite must not reach queries that do not see its key (0 * inf is NaN).
-// Only tiles on the causal edge are seen by some of a CTA's queries and not by others (and
+// Only tiles on the causal edge are seen by some of a block's queries and not by others (and
 // only they may hold rows of the next request): there such values are set to zero and the
-// first key that has one is noted per dim; the queries that see that key get NaN.
+// first key that has one is noted per dim; the CTA's queries that see that key get NaN.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -38,10 +39,11 @@
 namespace fsb {
 
 constexpr int kPreThreads = 384;
-constexpr int kPreSoft = 256;  // softmax threads (warps 4 .. 11)
-constexpr int kPreQ = 128;     // queries of a CTA
-constexpr int kPreK = 128;     // keys of a tile
-constexpr int kChunk = kPreK * 128;  // bytes of a 64-element chunk of a tile: 128 rows of 128 bytes
+constexpr int kPreSoft = 128;  // threads of a softmax group
+constexpr int kPreQ = 128;     // queries of a block, two blocks a CTA
+constexpr int kPreK = 96;      // keys of a tile
+constexpr int kQChunk = kPreQ * 128;  // bytes of a 64-element chunk: rows of 128 bytes
+constexpr int kChunk = kPreK * 128;
 constexpr float kPreSlack = 8.f;     // log2 of what the true maximum may be past the reference
 constexpr uint64_t kPreTimeoutNs = 2000000000ull;
 
@@ -60,14 +62,14 @@ struct PrefillShape {
   static constexpr int kDQ = kDN + kDR;
   static constexpr int kQKChunks = kDN / 64 + 1;  // the last one is the rotary part, 32 or 64 wide
   static constexpr int kVChunks = kDV / 64;
-  static constexpr int kQ = 0, kK = kQKChunks * kChunk, kV = kK + 2 * kQKChunks * kChunk;
+  static constexpr int kQ = 0, kK = 2 * kQKChunks * kQChunk, kV = kK + 2 * kQKChunks * kChunk;
   static constexpr int kSmem = kV + 2 * kVChunks * kChunk + 1024;  // 1024: alignment
-  // TMEM columns: two score buffers (P over their first half) and O
-  static constexpr uint32_t kTmemS = 0, kTmemO = 2 * kPreK, kTmemCols = 512;
+  // TMEM columns of a block: scores (P over their first half), and O
+  static constexpr uint32_t kTmemS = 0, kTmemO = 256, kTmemStep = 128, kTmemCols = 512;
 };
 
 struct PreBars {
-  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], pv_done;
+  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], pv_done[2];
 };
 
 template <bool kBf16>
@@ -111,7 +113,6 @@ __global__ void __launch_bounds__(kPreThreads, 1)
   __shared__ int s_find[2];
   __shared__ volatile int s_abort;
   __shared__ uint32_t s_tmem;
-  __shared__ float s_half[2][2][kPreQ];  // [tile parity][half][row]: maxima, and sums at the end
   __shared__ int s_bad[kDV];             // per dim: first key of an edge tile whose value is not finite
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int h = blockIdx.x % p.H;
@@ -123,7 +124,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       int64_t lo;
       int n = 0;
       if (base + lane < p.B) pre_range(p.q_off, base + lane, p.nq, lo, n);
-      int x = (n + kPreQ - 1) / kPreQ;
+      int x = (n + 2 * kPreQ - 1) / (2 * kPreQ);
       const int mine = x;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -150,8 +151,8 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       mbar_init(smem_u32(&bars.v_empty[i]), 1);
       mbar_init(smem_u32(&bars.s_full[i]), 1);
       mbar_init(smem_u32(&bars.p_ready[i]), kPreSoft);
+      mbar_init(smem_u32(&bars.pv_done[i]), 1);
     }
-    mbar_init(smem_u32(&bars.pv_done), 1);
     s_abort = 0;
     fence_mbar_init();
     fence_proxy_async_smem();
@@ -172,11 +173,14 @@ __global__ void __launch_bounds__(kPreThreads, 1)
   int nq, nk;
   pre_range(p.q_off, b, p.nq, q0, nq);
   pre_range(p.k_off, b, p.nk, k0, nk);
-  const int i0 = s_find[1] * kPreQ;             // first query of the tile, within the request
-  const int rows = min(kPreQ, nq - i0);
-  const int shift = nk - nq;                    // query i sees keys j <= i + shift
-  const int last = min(nk, i0 + rows + shift);  // keys that any of the tile's queries sees
-  const int tiles = last > 0 ? (last + kPreK - 1) / kPreK : 0;
+  const int i0 = s_find[1] * 2 * kPreQ;  // first query of the CTA, within the request
+  const int shift = nk - nq;             // query i sees keys j <= i + shift
+  // key tiles that any query of block g sees
+  auto tiles_of = [&](int g) -> int {
+    const int first = i0 + g * kPreQ, rows = min(kPreQ, nq - first), last = rows > 0 ? min(nk, first + rows + shift) : 0;
+    return last > 0 ? (last + kPreK - 1) / kPreK : 0;
+  };
+  const int n0 = tiles_of(0), n1 = tiles_of(1), tiles = max(n0, n1);
 
   if (warp == 0) {
     // ================================ TMA ==================================
@@ -188,8 +192,10 @@ __global__ void __launch_bounds__(kPreThreads, 1)
             "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"((int)y), "r"(smem_u32(bar))
             : "memory");
       };
-      mbar_arrive_expect_tx(smem_u32(&bars.q_full), L::kQKChunks * kChunk);
-      for (int c = 0; c < L::kQKChunks; ++c) load(smem + L::kQ + c * kChunk, &map_q, h * L::kDQ + 64 * c, q0 + i0, &bars.q_full);
+      mbar_arrive_expect_tx(smem_u32(&bars.q_full), 2 * L::kQKChunks * kQChunk);
+      for (int c = 0; c < 2 * L::kQKChunks; ++c)  // block 0's chunks, then block 1's (rows behind the last read as zero)
+        load(smem + L::kQ + c * kQChunk, &map_q, h * L::kDQ + 64 * (c % L::kQKChunks),
+             q0 + i0 + (c / L::kQKChunks) * kPreQ, &bars.q_full);
       for (int j = 0; j < tiles; ++j) {
         const int st = j & 1;
         const uint32_t ph = ((j >> 1) & 1) ^ 1;  // the stage's previous use is over (none: passes)
@@ -211,48 +217,166 @@ __global__ void __launch_bounds__(kPreThreads, 1)
     if (lane == 0 && tiles > 0) {
       constexpr uint32_t kIdS = mma_idesc(kPreQ, kPreK, kBf16, false);
       constexpr uint32_t kIdO = mma_idesc(kPreQ, kDV, kBf16, true);
-      auto scores = [&](int j) {  // S of tile j
-        const uint32_t kb = smem + L::kK + (j & 1) * L::kQKChunks * kChunk;
-        const uint32_t d = tmem + L::kTmemS + (j & 1) * kPreK;
+      constexpr uint32_t kHi = mma_desc_hi_sw128(1024);
+      const uint32_t q_lo = mma_desc_lo(smem + L::kQ, 0), k_lo = mma_desc_lo(smem + L::kK, 0);
+      const uint32_t v_lo = mma_desc_lo(smem + L::kV, kChunk);
+      auto scores = [&](int g, int j) {  // S of block g and tile j
+        const uint32_t q = q_lo + g * (L::kQKChunks * kQChunk / 16), k = k_lo + (j & 1) * (L::kQKChunks * kChunk / 16);
+        const uint32_t d = tmem + L::kTmemS + g * L::kTmemStep;
 #pragma unroll
-        for (int s = 0; s < L::kDQ / 16; ++s) {  // 16 dims a step: 32 bytes of a chunk's rows
-          const uint32_t off = (s >> 2) * kChunk + (s & 3) * 32;
-          mma_ss(d, mma_desc_sw128(smem + L::kQ + off, 0, 1024), mma_desc_sw128(kb + off, 0, 1024), kIdS, s > 0);
-        }
-        mma_commit(smem_u32(&bars.s_full[j & 1]));
-        mma_commit(smem_u32(&bars.k_empty[j & 1]));
+        for (int s = 0; s < L::kDQ / 16; ++s)  // 16 dims a step: 32 bytes of a chunk's rows
+          mma_ss(d, mma_desc(q + ((s >> 2) * kQChunk + (s & 3) * 32) / 16, kHi),
+                 mma_desc(k + ((s >> 2) * kChunk + (s & 3) * 32) / 16, kHi), kIdS, s > 0);
+        mma_commit(smem_u32(&bars.s_full[g]));
       };
       bool ok = pre_wait(&bars.q_full, 0, &s_abort) && pre_wait(&bars.k_full[0], 0, &s_abort);
       tcgen05_fence_after();
-      if (ok) scores(0);
+      if (ok) {
+        if (n0 > 0) scores(0, 0);
+        if (n1 > 0) scores(1, 0);
+        mma_commit(smem_u32(&bars.k_empty[0]));
+      }
       for (int j = 0; j < tiles && ok; ++j) {
         const int st = j & 1;
-        if (j + 1 < tiles) {
-          ok = pre_wait(&bars.k_full[st ^ 1], ((j + 1) >> 1) & 1, &s_abort);
-          tcgen05_fence_after();
+        const uint32_t v = v_lo + st * (L::kVChunks * kChunk / 16);
+        ok = pre_wait(&bars.v_full[st], (j >> 1) & 1, &s_abort);
+        if (ok && j + 1 < tiles) ok = pre_wait(&bars.k_full[st ^ 1], ((j + 1) >> 1) & 1, &s_abort);
+        for (int g = 0; g < 2 && ok; ++g) {
+          const int n = g == 0 ? n0 : n1;
+          if (j >= n) continue;
+          ok = pre_wait(&bars.p_ready[g], j & 1, &s_abort);
           if (!ok) break;
-          scores(j + 1);
-        }
-        ok = pre_wait(&bars.p_ready[st], (j >> 1) & 1, &s_abort) && pre_wait(&bars.v_full[st], (j >> 1) & 1, &s_abort);
-        if (!ok) break;
-        tcgen05_fence_after();
-        const uint32_t vb = smem + L::kV + st * L::kVChunks * kChunk, a = tmem + L::kTmemS + st * kPreK;
+          tcgen05_fence_after();
+          const uint32_t a = tmem + L::kTmemS + g * L::kTmemStep, d = tmem + L::kTmemO + g * L::kTmemStep;
 #pragma unroll
-        for (int s = 0; s < kPreK / 16; ++s)  // 16 keys a step: 8 columns of P, 16 rows of V
-          mma_ts(tmem + L::kTmemO, a + 8 * s, mma_desc_sw128(vb + s * 16 * 128, kChunk, 1024), kIdO, j > 0 || s > 0);
+          for (int s = 0; s < kPreK / 16; ++s)  // 16 keys a step: 8 columns of P, 16 rows of V
+            mma_ts(d, a + 8 * s, mma_desc(v + s * (16 * 128 / 16), kHi), kIdO, j > 0 || s > 0);
+          if (j + 1 == n) mma_commit(smem_u32(&bars.pv_done[g]));
+          if (j + 1 < n) scores(g, j + 1);  // over the P that was just read
+        }
         mma_commit(smem_u32(&bars.v_empty[st]));
-        mma_commit(smem_u32(&bars.pv_done));
+        mma_commit(smem_u32(&bars.k_empty[st ^ 1]));
       }
     }
   } else if (warp >= 4) {
     // ============================== softmax ================================
-    const int half = (warp - 4) >> 2, row = (warp & 3) * 32 + lane, st_tid = tid - 128;
+    const int grp = (warp - 4) >> 2, row = (warp & 3) * 32 + lane, grp_tid = tid & (kPreSoft - 1);
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const int limit = i0 + row + shift;  // last key that this row sees
+    const int first = i0 + grp * kPreQ, rows = min(kPreQ, nq - first), n = grp == 0 ? n0 : n1;
+    const int limit = first + row + shift;  // last key that this row sees
+    const uint32_t sb = tmem + lanes + L::kTmemS + grp * L::kTmemStep;
+    const uint32_t ob = tmem + lanes + L::kTmemO + grp * L::kTmemStep;
     float m_ref = -1.0e30f, l = 0.f;
-    // a wait that gave up is shared at the next barrier, where all 256 threads leave together
     bool any_bad = false, ok = true;
-    auto any_of = [](bool x) -> bool {  // OR over the softmax threads; also orders their shared memory
+    for (int j = 0; j < n; ++j) {
+      const int j0 = j * kPreK;
+      ok = pre_wait(&bars.s_full[grp], j & 1, &s_abort);
+      if (!__all_sync(0xffffffffu, ok)) {
+        ok = false;
+        break;
+      }
+      tcgen05_fence_after();
+      const bool edge = j0 + kPreK > first + shift + 1;  // some of the block's queries do not see the whole tile
+      uint32_t raw[kPreK / 32][32];
+#pragma unroll
+      for (int c = 0; c < kPreK / 32; ++c) tmem_ld32(sb + 32 * c, raw[c]);
+      tmem_wait_ld();
+      // tiles that every query sees whole keep the raw scores (the scale joins in the exponent's
+      // FMA); edge tiles are scaled and masked here
+      float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      if (edge) {
+        const int seen = limit - j0;  // this row's keys 0 .. seen
+#pragma unroll
+        for (int k = 0; k < kPreK; ++k) {
+          const float x = k > seen ? -INFINITY : __uint_as_float(raw[k >> 5][k & 31]) * p.scale_log2;
+          raw[k >> 5][k & 31] = __float_as_uint(x);
+          m4[k & 3] = fmaxf(m4[k & 3], x);
+        }
+      } else if (p.scale_log2 >= 0.f) {
+#pragma unroll
+        for (int k = 0; k < kPreK; ++k) m4[k & 3] = fmaxf(m4[k & 3], __uint_as_float(raw[k >> 5][k & 31]));
+      } else {
+#pragma unroll
+        for (int k = 0; k < kPreK; ++k) m4[k & 3] = fmaxf(m4[k & 3], -__uint_as_float(raw[k >> 5][k & 31]));
+      }
+      const float mul = edge ? 1.f : p.scale_log2;
+      const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * fabsf(mul);
+      // a row's first maximum is its reference; later ones only when far past it
+      const bool move = mx > m_ref + (m_ref == -1.0e30f ? 0.f : kPreSlack);
+      if (__any_sync(0xffffffffu, move)) {
+        const float m_new = move ? mx : m_ref;
+        if (j > 0) {  // O is there (its MMAs were issued before this tile's): bring it to the new reference
+          const float alpha = ex2_approx(m_ref - m_new);
+          l *= alpha;
+#pragma unroll
+          for (int c = 0; c < kDV / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld16(ob + 16 * c, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+            tmem_st16(ob + 16 * c, o);
+          }
+        }
+        m_ref = m_new;
+      }
+      float l4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < kPreK / 32; ++c) {
+        uint32_t packed[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const float p0 = ex2_approx(fmaf(__uint_as_float(raw[c][2 * k]), mul, -m_ref));
+          const float p1 = ex2_approx(fmaf(__uint_as_float(raw[c][2 * k + 1]), mul, -m_ref));
+          l4[k & 3] += p0 + p1;
+          packed[k] = pre_pack<kBf16>(p0, p1);
+        }
+        tmem_st16(sb + 16 * c, packed);
+      }
+      l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+      if (edge) {
+        constexpr uint16_t kExp = kBf16 ? 0x7f80 : 0x7c00;
+        ok = pre_wait(&bars.v_full[j & 1], (j >> 1) & 1, &s_abort);
+        uint8_t* vb = smem_p + L::kV + (j & 1) * L::kVChunks * kChunk;
+#pragma unroll 2
+        for (int i = grp_tid; i < L::kVChunks * kPreK * 8; i += kPreSoft) {
+          uint4* at = reinterpret_cast<uint4*>(vb + 16 * i);  // [chunk][key][16-byte unit]
+          const uint4 v = *at;
+          uint32_t w[4] = {v.x, v.y, v.z, v.w};
+          bool here = false;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            // an exponent of all ones carries out of its field when its lowest bit is added
+            constexpr uint32_t kLow = kBf16 ? 0x00800080u : 0x04000400u, kMask = kBf16 ? 0x7f807f80u : 0x7c007c00u;
+            here |= (((w[k] & kMask) + kLow) & 0x80008000u) != 0u;
+          }
+          if (here) {
+            const int ch = i / (kPreK * 8), r = (i >> 3) % kPreK, u = i & 7;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const uint16_t e = (uint16_t)(w[k >> 1] >> (16 * (k & 1)));
+              if ((e & kExp) == kExp) {
+                atomicMin(s_bad + 64 * ch + 8 * (u ^ (r & 7)) + k, j0 + r);
+                w[k >> 1] &= (k & 1) ? 0x0000ffffu : 0xffff0000u;
+              }
+            }
+            *at = make_uint4(w[0], w[1], w[2], w[3]);
+            any_bad = true;
+          }
+        }
+        fence_proxy_async_smem();  // the MMA reads V through the async proxy
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+      }
+      tmem_wait_st();
+      tcgen05_fence_before();
+      mbar_arrive(smem_u32(&bars.p_ready[grp]));
+    }
+    if (n > 0 && ok) ok = pre_wait(&bars.pv_done[grp], 0, &s_abort);
+    __syncwarp();
+    auto any_of = [](bool x) -> bool {  // OR over both groups; also orders their shared memory
       uint32_t r;
       asm volatile(
           "{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n bar.red.or.pred q, 1, 256, p;\n selp.b32 %0, 1, 0, q;\n}\n"
@@ -261,143 +385,39 @@ __global__ void __launch_bounds__(kPreThreads, 1)
           : "memory");
       return r != 0;
     };
-    for (int j = 0; j < tiles; ++j) {
-      const int st = j & 1, j0 = j * kPreK;
-      ok = pre_wait(&bars.s_full[st], (j >> 1) & 1, &s_abort) && ok;
-      __syncwarp();
-      tcgen05_fence_after();
-      const uint32_t sb = tmem + lanes + L::kTmemS + st * kPreK;
-      const bool edge = j0 + kPreK > i0 + shift + 1;  // some of the CTA's queries do not see the whole tile
-      uint32_t raw[2][32];
-      tmem_ld32(sb + 64 * half, raw[0]);
-      tmem_ld32(sb + 64 * half + 32, raw[1]);
-      tmem_wait_ld();
-      // tiles that every query sees whole keep the raw scores (the scale joins in the exponent's
-      // FMA); edge tiles are scaled and masked here
-      float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      if (edge) {
-        const int seen = limit - j0 - 64 * half;  // this thread's keys 0 .. seen
-#pragma unroll
-        for (int k = 0; k < 64; ++k) {
-          const float x = k > seen ? -INFINITY : __uint_as_float(raw[k >> 5][k & 31]) * p.scale_log2;
-          raw[k >> 5][k & 31] = __float_as_uint(x);
-          m4[k & 3] = fmaxf(m4[k & 3], x);
-        }
-      } else if (p.scale_log2 >= 0.f) {
-#pragma unroll
-        for (int k = 0; k < 64; ++k) m4[k & 3] = fmaxf(m4[k & 3], __uint_as_float(raw[k >> 5][k & 31]));
-      } else {
-#pragma unroll
-        for (int k = 0; k < 64; ++k) m4[k & 3] = fmaxf(m4[k & 3], -__uint_as_float(raw[k >> 5][k & 31]));
-      }
-      const float mul = edge ? 1.f : p.scale_log2;
-      float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * fabsf(mul);
-      s_half[st][half][row] = mx;
-      if (any_of(!ok)) {  // after it, both halves have read their scores
-        ok = false;
-        break;
-      }
-      mx = fmaxf(mx, s_half[st][half ^ 1][row]);
-      // a row's first maximum is its reference; later ones only when far past it
-      const bool move = mx > m_ref + (m_ref == -1.0e30f ? 0.f : kPreSlack);
-      if (__any_sync(0xffffffffu, move)) {
-        const float m_new = move ? mx : m_ref;
-        if (j > 0) {  // O is there: bring it to the new reference
-          const float alpha = ex2_approx(m_ref - m_new);
-          l *= alpha;
-          ok = pre_wait(&bars.pv_done, (j - 1) & 1, &s_abort) && ok;
-          __syncwarp();
-          tcgen05_fence_after();
-          const uint32_t ob = tmem + lanes + L::kTmemO + half * (kDV / 2);
-#pragma unroll
-          for (int c = 0; c < kDV / 64; ++c) {
-            uint32_t o[32];
-            tmem_ld32(ob + 32 * c, o);
-            tmem_wait_ld();
-#pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
-            tmem_st32(ob + 32 * c, o);
-          }
-        }
-        m_ref = m_new;
-      }
-      float l4[4] = {0.f, 0.f, 0.f, 0.f};
-      uint32_t packed[32];
-#pragma unroll
-      for (int k = 0; k < 32; ++k) {
-        const float p0 = ex2_approx(fmaf(__uint_as_float(raw[k >> 4][(2 * k) & 31]), mul, -m_ref));
-        const float p1 = ex2_approx(fmaf(__uint_as_float(raw[k >> 4][(2 * k + 1) & 31]), mul, -m_ref));
-        l4[k & 3] += p0 + p1;
-        packed[k] = pre_pack<kBf16>(p0, p1);
-      }
-      l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
-      tmem_st32(sb + 32 * half, packed);
-      if (edge) {
-        constexpr uint16_t kExp = kBf16 ? 0x7f80 : 0x7c00;
-        ok = pre_wait(&bars.v_full[st], (j >> 1) & 1, &s_abort) && ok;
-        uint8_t* vb = smem_p + L::kV + st * L::kVChunks * kChunk;
-        for (int i = st_tid; i < L::kVChunks * kPreK * 8; i += kPreSoft) {
-          const int ch = i / (kPreK * 8), r = (i >> 3) & (kPreK - 1), u = i & 7;
-          uint4* at = reinterpret_cast<uint4*>(vb + ch * kChunk + r * 128 + 16 * u);
-          const uint4 v = *at;
-          uint32_t w[4] = {v.x, v.y, v.z, v.w};
-          bool here = false;
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const uint16_t e = (uint16_t)(w[k >> 1] >> (16 * (k & 1)));
-            if ((e & kExp) == kExp) {
-              atomicMin(s_bad + 64 * ch + 8 * (u ^ (r & 7)) + k, j0 + r);
-              w[k >> 1] &= (k & 1) ? 0x0000ffffu : 0xffff0000u;
-              here = true;
-            }
-          }
-          if (here) *at = make_uint4(w[0], w[1], w[2], w[3]);
-          any_bad |= here;
-        }
-        fence_proxy_async_smem();  // the MMA reads V through the async proxy
-        __syncwarp();
-      }
-      tmem_wait_st();
-      tcgen05_fence_before();
-      mbar_arrive(smem_u32(&bars.p_ready[st]));
-    }
-    if (tiles > 0 && ok) ok = pre_wait(&bars.pv_done, (tiles - 1) & 1, &s_abort);
-    __syncwarp();
-    s_half[0][half][row] = l;
     const bool failed = any_of(!ok);
     any_bad = any_of(any_bad);
     if (failed) {
-      if (st_tid == 0 && p.status != nullptr) atomicOr(p.status, FS_DEV_TIMEOUT);
+      if (grp == 0 && grp_tid == 0 && p.status != nullptr) atomicOr(p.status, FS_DEV_TIMEOUT);
     } else {
       tcgen05_fence_after();
-      l += s_half[0][half ^ 1][row];
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      uint16_t* dst = p.out + ((size_t)(q0 + i0 + min(row, rows - 1)) * p.H + h) * kDV + half * (kDV / 2);
+      uint16_t* dst = p.out + ((size_t)(q0 + first + row) * p.H + h) * kDV;
 #pragma unroll
-      for (int c = 0; c < kDV / 64; ++c) {
-        uint32_t o[32];
-        if (tiles > 0) {
-          tmem_ld32(tmem + lanes + L::kTmemO + half * (kDV / 2) + 32 * c, o);
+      for (int c = 0; c < kDV / 16; ++c) {
+        uint32_t o[16];
+        if (n > 0) {
+          tmem_ld16(ob + 16 * c, o);
           tmem_wait_ld();
         } else {
 #pragma unroll
-          for (int k = 0; k < 32; ++k) o[k] = 0u;
+          for (int k = 0; k < 16; ++k) o[k] = 0u;
         }
         if (row < rows) {
 #pragma unroll
-          for (int k = 0; k < 32; k += 8) {
+          for (int k = 0; k < 16; k += 8) {
             uint32_t w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              float v0 = __uint_as_float(o[k + 2 * e]) * inv, v1 = __uint_as_float(o[k + 2 * e + 1]) * inv;
-              if (any_bad) {
-                const int d = half * (kDV / 2) + 32 * c + k + 2 * e;
-                if (s_bad[d] <= limit) v0 = __int_as_float(0x7fc00000);
-                if (s_bad[d + 1] <= limit) v1 = __int_as_float(0x7fc00000);
+              float v[2];
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                v[u] = __uint_as_float(o[k + 2 * e + u]) * inv;
+                if (any_bad && s_bad[16 * c + k + 2 * e + u] <= limit) v[u] = __int_as_float(0x7fc00000);
               }
-              w[e] = pre_pack<kBf16>(v0, v1);
+              w[e] = pre_pack<kBf16>(v[0], v[1]);
             }
-            *reinterpret_cast<uint4*>(dst + 32 * c + k) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(dst + 16 * c + k) = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
         __syncwarp();
@@ -412,14 +432,14 @@ __global__ void __launch_bounds__(kPreThreads, 1)
   }
 }
 
-// Rows [n, heads * width] of 16-bit elements as boxes of 128 rows by 64 elements; what lies
+// Rows [n, heads * width] of 16-bit elements as boxes of box_rows rows by 64 elements; what lies
 // behind a row's end or behind the last row reads as zero.
-static int pre_map(CUtensorMap* map, const void* base, int64_t n, int64_t row_elems) {
+static int pre_map(CUtensorMap* map, const void* base, int64_t n, int64_t row_elems, int box_rows) {
   EncodeTiledFn enc = encode_fn();
   if (enc == nullptr) return fail_cuda("cuTensorMapEncodeTiled is not available from the driver");
   cuuint64_t dims[2] = {(cuuint64_t)row_elems, (cuuint64_t)n};
   cuuint64_t strides[1] = {(cuuint64_t)row_elems * 2};
-  cuuint32_t box[2] = {64, (cuuint32_t)kPreK};
+  cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(base), dims, strides, box, estr,
                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -431,10 +451,10 @@ template <int kDN, int kDR, int kDV>
 static int launch_prefill(const FsLatentPrefillArgs* a, const PrefillParams& p, int64_t tiles, void* stream) {
   using L = PrefillShape<kDN, kDR, kDV>;
   CUtensorMap mq, mkv, mr;
-  if (int st = pre_map(&mq, a->q, a->q_rows, (int64_t)a->heads * L::kDQ); st != FS_OK) return st;
+  if (int st = pre_map(&mq, a->q, a->q_rows, (int64_t)a->heads * L::kDQ, kPreQ); st != FS_OK) return st;
   if (a->k_rows > 0) {
-    if (int st = pre_map(&mkv, a->kv, a->k_rows, (int64_t)a->heads * (kDN + kDV)); st != FS_OK) return st;
-    if (int st = pre_map(&mr, a->k_rope, a->k_rows, kDR); st != FS_OK) return st;
+    if (int st = pre_map(&mkv, a->kv, a->k_rows, (int64_t)a->heads * (kDN + kDV), kPreK); st != FS_OK) return st;
+    if (int st = pre_map(&mr, a->k_rope, a->k_rows, kDR, kPreK); st != FS_OK) return st;
   } else {
     mkv = mr = mq;  // no key tile is ever loaded
   }
@@ -470,7 +490,7 @@ extern "C" int fs_latent_prefill(const FsLatentPrefillArgs* a, void* stream) {
        reinterpret_cast<uintptr_t>(a->out)) & 15)
     return FS_ERR_ALIGNMENT;
   if (a->q_rows >= (1ll << 30) || a->k_rows >= (1ll << 30) || a->heads > (1 << 20)) return FS_ERR_UNSUPPORTED;
-  const int64_t tiles = a->q_rows / kPreQ + a->batch;  // at least as many as the requests have
+  const int64_t tiles = a->q_rows / (2 * kPreQ) + a->batch;  // at least as many as the requests have
   if (tiles * a->heads >= (1ll << 31)) return FS_ERR_UNSUPPORTED;
   PrefillParams p{};
   p.q_off = a->q_offsets;
