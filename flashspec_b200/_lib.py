@@ -260,6 +260,7 @@ class FsLatentPrefillArgs(C.Structure):
         ("rope_dim", C.c_int32),
         ("value_dim", C.c_int32),
         ("sm_scale", C.c_float),
+        ("clear_rest", C.c_int32),
         ("device_status", C.c_void_p),
     ]
 

@@ -20,7 +20,7 @@ import torch
 
 from . import _lib
 from .quant import (QuantizedTensor, SymQuantizedTensor, build_compression_stats, estimate_quantized_bytes,
-                    require_cuda, stream_of)
+                    device_guard, require_cuda, stream_of)
 
 PAGE_TOKENS = 16  # tokens per kernel step (one page / quant block)
 NUM_WARPS = 4
@@ -110,14 +110,12 @@ def _i64(t: torch.Tensor) -> torch.Tensor:
     return t if t.dtype == torch.int64 and t.is_contiguous() else t.to(torch.int64).contiguous()
 
 
-def _run(entry: str, args: _lib.FsDecodeArgs, device: torch.device, splits_hint: int, xargs=None,
-         weights: Optional[torch.Tensor] = None) -> int:
+def _run(entry: str, args: _lib.FsDecodeArgs, device: torch.device, splits_hint: int, xargs=None) -> int:
     """Plan (cached), workspace and launch of one decode call; ``xargs`` (FsExchangeArgs)
-    selects fs_paged_decode_exchange and its own plan, ``weights`` fs_paged_decode_weights
-    and its."""
+    selects fs_paged_decode_exchange and its own plan."""
     if torch.cuda.current_device() != device.index:
         with torch.cuda.device(device):
-            return _run(entry, args, device, splits_hint, xargs, weights)
+            return _run(entry, args, device, splits_hint, xargs)
     lib = _lib.load()
     stream = stream_of(device)
     args.num_splits = splits_hint
@@ -131,23 +129,13 @@ def _run(entry: str, args: _lib.FsDecodeArgs, device: torch.device, splits_hint:
         nbytes = C.c_size_t(0)
         splits = C.c_int32(0)
         size_fn = lib.fs_paged_decode_exchange_workspace_size if xargs is not None else lib.fs_decode_workspace_size
-        if weights is not None:
-            size_fn = lib.fs_paged_decode_weights_workspace_size
         _lib.check(size_fn(C.byref(args), C.byref(nbytes), C.byref(splits)), entry)
         plan = _plans[key] = (nbytes.value, splits.value)
         if len(_plans) > 256:
             _plans.pop(next(iter(_plans)))
     nbytes = C.c_size_t(plan[0])
     splits = C.c_int32(plan[1])
-    if weights is not None:
-        # scores can be large: scratch of this call (in a capture, of the graph's own pool)
-        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=device)
-        args.workspace = ws.data_ptr()
-        args.workspace_bytes = ws.numel()
-        tk = _weights_tickets(device, stream, args.batch * args.kv_heads)
-        args.tickets = tk.data_ptr()
-        args.ticket_count = tk.numel()
-    elif nbytes.value:
+    if nbytes.value:
         ws = _workspace(device, stream, nbytes.value)
         args.workspace = ws.data_ptr()
         args.workspace_bytes = ws.numel()
@@ -156,10 +144,25 @@ def _run(entry: str, args: _lib.FsDecodeArgs, device: torch.device, splits_hint:
         args.ticket_count = tk.numel()
     if xargs is not None:
         _lib.check(getattr(lib, entry)(C.byref(args), C.byref(xargs), stream), entry)
-    elif weights is not None:
-        _lib.check(lib.fs_paged_decode_weights(C.byref(args), weights.data_ptr(), stream), entry)
     else:
         _lib.check(getattr(lib, entry)(C.byref(args), stream), entry)
+    return splits.value
+
+
+def _run_weights(a: _lib.FsDecodeArgs, weights: torch.Tensor, device: torch.device, splits_hint: int) -> int:
+    """Workspace and launch of one weighted decode.  Scores can be large, so the workspace is
+    this call's own (in a capture, of the graph's pool)."""
+    with device_guard(device):
+        lib, stream = _lib.load(), stream_of(device)
+        a.num_splits = splits_hint
+        nbytes, splits = C.c_size_t(0), C.c_int32(0)
+        _lib.check(lib.fs_paged_decode_weights_workspace_size(C.byref(a), C.byref(nbytes), C.byref(splits)),
+                   "fs_paged_decode_weights")
+        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=device)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes.value
+        tk = _weights_tickets(device, stream, a.batch * a.kv_heads)
+        a.tickets, a.ticket_count = tk.data_ptr(), tk.numel()
+        _lib.check(lib.fs_paged_decode_weights(C.byref(a), weights.data_ptr(), stream), "fs_paged_decode_weights")
     return splits.value
 
 
@@ -351,7 +354,7 @@ def paged_quant_attention_weights_cuda(q: torch.Tensor, cache, weights: torch.Te
     out = torch.empty_like(qc)
     a = _decode_args(_lib.FS_LAYOUT_PAGED, qc, kq, vq, out, lengths, table, num_pages, int(cache.max_seq_len), hkv,
                      device_status, page_size=page)
-    splits = _run("fs_paged_decode_weights", a, q.device, num_splits or _env_splits(), weights=weights)
+    splits = _run_weights(a, weights, q.device, num_splits or _env_splits())
     if not return_stats:
         return out
     dense = 2 * q.shape[0] * hkv * int(cache.max_seq_len) * q.shape[2] * qc.element_size()

@@ -255,10 +255,11 @@ struct QueryFrag {
   // the largest fixed-point value: 127 in every byte (127 * 2^16 + 127 * 2^8 + 127 is left a
   // margin, since at 24 bits amax * (kTop / amax) can round to kTop + 1 and carry)
   static constexpr float kTop = kWts ? 8355000.0f : 32639.0f;
-  uint32_t hi[8], lo[8], lo2[kWts ? 8 : 1];
+  uint32_t hi[8], lo[8];
   int q16sum;
   float qscale;
-  __device__ __forceinline__ void load(const DecodeParams& p, int b, int h, int lane) {
+  // lo2_s (kWts): shared address of the warp's third bytes, two 16-byte words a lane
+  __device__ __forceinline__ void load(const DecodeParams& p, int b, int h, int lane, uint32_t lo2_s = 0) {
     const int g = lane >> 2, c = lane & 3;
     uint32_t raw[16];
     if (g < p.G) {
@@ -311,7 +312,8 @@ struct QueryFrag {
       }
       hi[w] = hw;
       lo[w] = lw;
-      if (kWts) lo2[w] = lw2;
+      if (kWts)
+        asm volatile("st.shared.u32 [%0], %1;" ::"r"(lo2_s + (w >> 2) * 512 + lane * 16 + (w & 3) * 4), "r"(lw2) : "memory");
     }
     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
@@ -332,6 +334,7 @@ struct QueryFrag {
 // of score + log2(V scale): P = 2^(t - m_run) * scale * 2^14 uses fp16's range from the top
 // whatever the scale, while l_run keeps sum 2^(t - m_run) in fp32 (at most 2^100 a token).
 constexpr float kWtsTop = 16384.f;
+constexpr int kLo2Bytes = 1024;  // third bytes of a warp's query fragment
 
 struct WarpState {
   float m_run, l_run, z_run;
@@ -379,24 +382,37 @@ struct WarpState {
 template <int kMode, bool kWts = false>
 __device__ __forceinline__ void consume_page(uint32_t sbase, const StageOffsets& off, uint32_t empty_bar, int lane,
                                              const StageInfo& si, const QueryFrag<kWts>& qf, float qk_scale_log2,
-                                             int pos0, int len_eff, WarpState& ws, float* srow = nullptr) {
+                                             int pos0, int len_eff, WarpState& ws, float* srow = nullptr,
+                                             uint32_t lo2_s = 0) {
   const int c = lane & 3;
   // ---- S = Q K^T on the int8 tensor cores, straight from the stored bytes s = u - 128:
   // sum_d q16 * s = 256 * (hi . s) + (lo . s); u - zp = s + (128 - zp) is applied per page
-  int shi[2][4], slo[2][4], slo2[kWts ? 2 : 1][4];
+  int shi[2][4], slo[2][4];
+  float third[4];  // kWts: sum lo2 . s of tokens 2c, 2c+1, 8+2c, 9+2c
   {
     uint4 kr[2][2];
 #pragma unroll
     for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
       for (int e2 = 0; e2 < 2; ++e2) kr[nt][e2] = lds128(sbase + off.k[nt][e2]);
+    if (kWts) {
+      int s3[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+      for (int e2 = 0; e2 < 2; ++e2) {
+        const uint4 q3 = lds128(lo2_s + e2 * 512 + lane * 16);
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) {
+          mma_16832_s8(s3[nt], q3.x, 0u, q3.y, 0u, kr[nt][e2].x, kr[nt][e2].y);
+          mma_16832_s8(s3[nt], q3.z, 0u, q3.w, 0u, kr[nt][e2].z, kr[nt][e2].w);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) third[k] = (float)s3[k >> 1][k & 1];
+    }
 #pragma unroll
     for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        shi[nt][k] = slo[nt][k] = 0;
-        if (kWts) slo2[nt][k] = 0;
-      }
+      for (int k = 0; k < 4; ++k) shi[nt][k] = slo[nt][k] = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
 #pragma unroll
@@ -406,7 +422,6 @@ __device__ __forceinline__ void consume_page(uint32_t sbase, const StageOffsets&
         const uint32_t b1 = (j & 1) ? kv.w : kv.y;
         mma_16832_s8(shi[nt], qf.hi[2 * j], 0u, qf.hi[2 * j + 1], 0u, b0, b1);
         mma_16832_s8(slo[nt], qf.lo[2 * j], 0u, qf.lo[2 * j + 1], 0u, b0, b1);
-        if (kWts) mma_16832_s8(slo2[nt], qf.lo2[2 * j], 0u, qf.lo2[2 * j + 1], 0u, b0, b1);
       }
     }
   }
@@ -436,12 +451,11 @@ __device__ __forceinline__ void consume_page(uint32_t sbase, const StageOffsets&
     vk[3] = v89.y;
   }
   float t[4];
-  if (kWts) {  // 24 bits of q: the three sums pass 32 bits together, so the top one joins in fp32
+  if (kWts) {  // 24 bits of q: the sums pass 32 bits together, so they join in fp32
     const float zf = (float)(128 - (int)si.kz) * (float)qf.q16sum;
 #pragma unroll
     for (int k = 0; k < 4; ++k)  // tokens 2c, 2c+1, 8+2c, 9+2c
-      t[k] = (fmaf(65536.f, (float)shi[k >> 1][k & 1], (float)((slo[k >> 1][k & 1] << 8) + slo2[k >> 1][k & 1])) + zf) *
-             fk[k];
+      t[k] = (fmaf(256.f, (float)((shi[k >> 1][k & 1] << 8) + slo[k >> 1][k & 1]), third[k]) + zf) * fk[k];
   } else {
     t[0] = (float)((shi[0][0] << 8) + slo[0][0] + zc) * fk[0];  // token 2c
     t[1] = (float)((shi[0][1] << 8) + slo[0][1] + zc) * fk[1];  // token 2c+1
@@ -465,9 +479,13 @@ __device__ __forceinline__ void consume_page(uint32_t sbase, const StageOffsets&
   }
   float mx = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
   if (kWts) {  // the reference point covers V's scale too (WarpState)
-    mx = -INFINITY;
+    if (si.tok != 0u) {
+      mx = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) mx = fmaxf(mx, t[k] + fmaxf(lg2_approx(vk[k]), -100.f));
+      for (int k = 0; k < 4; ++k) mx = fmaxf(mx, t[k] + fmaxf(lg2_approx(vk[k]), -100.f));
+    } else {
+      mx += fmaxf(lg2_approx(si.vs), -100.f);
+    }
   }
   mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
   mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
@@ -748,7 +766,9 @@ __global__ void __launch_bounds__((kW + 1) * 32, kMinBlocks)
   } else {
     // ============================ consumer warps ===============================
     QueryFrag<kWts> qf;
-    qf.load(p, b, h, lane);
+    const uint32_t lo2_s = empty_s + kNS * 8 + warp * kLo2Bytes;  // kWts: behind the barriers
+    qf.load(p, b, h, lane, lo2_s);
+    if (kWts) __syncwarp();
     const StageOffsets off(lane);
     for (int i = warp; i < n; i += kW) {
       const int st = (int)((unsigned)i % kNS);
@@ -767,7 +787,7 @@ __global__ void __launch_bounds__((kW + 1) * 32, kMinBlocks)
       if (kWts && g < p.G)
         srow = p.scores + ((size_t)b * p.Hq + (size_t)h * p.G + g) * p.score_stride + (size_t)(p0 + i) * kPage;
       consume_page<kMode, kWts>(base_s + st * kStageBytes, off, empty_s + 8 * st, lane, si, qf, p.qk_scale_log2,
-                                (p0 + i) * kPage, len_eff, ws, srow);
+                                (p0 + i) * kPage, len_eff, ws, srow, lo2_s);
     }
     ws.l_run += __shfl_xor_sync(0xffffffffu, ws.l_run, 1);
     ws.l_run += __shfl_xor_sync(0xffffffffu, ws.l_run, 2);
@@ -1235,7 +1255,9 @@ __global__ void __maxnreg__(kMaxRegs)
   uint32_t* meta_p = reinterpret_cast<uint32_t*>(base_p + L::kStageRegion);
   const uint32_t full_s = base_s + L::kStageRegion + L::kMetaRegion;
   const uint32_t empty_s = full_s + kNS * 8;
-  int* pre = reinterpret_cast<int*>(base_p + L::kStageRegion + L::kMetaRegion + L::kBarRegion);  // [B + 1]
+  // kWts: the third bytes of q lie between the barriers and the prefix table
+  int* pre = reinterpret_cast<int*>(base_p + L::kStageRegion + L::kMetaRegion + L::kBarRegion +
+                                    (kWts ? kW * kLo2Bytes : 0));  // [B + 1]
 
   const int tid = threadIdx.x;
   const int warp = tid >> 5;
@@ -1367,6 +1389,7 @@ __global__ void __maxnreg__(kMaxRegs)
   const int len_w = starts[warp + 1] - starts[warp];
   const StageOffsets off(lane);
   QueryFrag<kWts> qf;
+  const uint32_t lo2_s = empty_s + kNS * 8 + warp * kLo2Bytes;
   WarpState ws;
   ws.reset();
   int r = 0, h = 0, nb = 1, len_eff = 0;
@@ -1382,7 +1405,9 @@ __global__ void __maxnreg__(kMaxRegs)
       pair_end = pair_P + nb;
       piece_f0 = f;
       window_pages<kPaged>(p, r, lo, hi_cap, &len_eff);
-      qf.load(p, r, h, lane);
+      if (kWts) __syncwarp();  // every lane is done with the third bytes of the piece before
+      qf.load(p, r, h, lane, lo2_s);
+      if (kWts) __syncwarp();
     }
     const int i = j * kW + warp;
     const int st = (int)((unsigned)i % kNS);
@@ -1397,7 +1422,7 @@ __global__ void __maxnreg__(kMaxRegs)
       float* srow = nullptr;
       if (kWts && g < p.G) srow = p.scores + ((size_t)r * p.Hq + (size_t)h * p.G + g) * p.score_stride + pos0;
       consume_page<0, kWts>(base_s + st * kStageBytes, off, empty_s + 8 * st, lane, si, qf, p.qk_scale_log2, pos0,
-                            len_eff, ws, srow);
+                            len_eff, ws, srow, lo2_s);
     } else {
       __syncwarp();
       if (lane == 0) mbar_arrive(empty_s + 8 * st);
@@ -1538,11 +1563,18 @@ static DecodeKernelFn balanced_for(int shape) {
   return trace_ptr() != nullptr ? balanced_inst<kPaged, 0, true>() : balanced_inst<kPaged, 0>();
 }
 
-// The kernels that also store scores and LSEs (weighted decode) exist in shape 0, paged.
+// The kernels that also store scores and LSEs (weighted decode) exist in shape 0, paged, with
+// four stages fewer: their place holds the third byte of q.
+constexpr int kWtsStages = 12;
+static int smem_weights(bool balanced, int batch) {
+  return 1024 + kWtsStages * (kStageBytes + kMetaBytes + 16) + kShapes[0].warps * kLo2Bytes +
+         (balanced ? (4 * (batch + 1) + 4 * (kShapes[0].warps + 1) + 15) & ~15 : 0);
+}
+
 static DecodeKernelFn weights_kernel(bool balanced) {
   constexpr Shape sh = kShapes[0];
-  if (balanced) return decode_balanced_kernel<true, sh.warps, sh.stages, sh.max_regs, false, true>;
-  return decode_kernel<true, sh.warps, sh.stages, sh.min_blocks, 0, true>;
+  if (balanced) return decode_balanced_kernel<true, sh.warps, kWtsStages, sh.max_regs, false, true>;
+  return decode_kernel<true, sh.warps, kWtsStages, sh.min_blocks, 0, true>;
 }
 
 static int smem_bytes(int shape) {
@@ -1585,7 +1617,7 @@ static int configure_weights(int device) {
   if (done[device]) return FS_OK;
   for (int balanced = 0; balanced < 2; ++balanced)
     if (cudaError_t e = cudaFuncSetAttribute(weights_kernel(balanced != 0), cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             balanced ? smem_balanced(0, kMaxSKBatch) : smem_bytes(0));
+                                             smem_weights(balanced != 0, kMaxSKBatch));
         e != cudaSuccess)
       return fail_cuda("shared-memory limit of the weighted decode kernels", e);
   done[device] = true;
@@ -2022,12 +2054,14 @@ static int launch_decode(const FsDecodeArgs* a_in, void* stream, const FsExchang
   p.counters = reinterpret_cast<unsigned*>(a->tickets);
   const int threads = (kShapes[shape].warps + 1) * 32;
   if (pl.balanced) {
-    (w != nullptr ? weights_kernel(true) : balanced_for<kPaged>(shape))<<<(unsigned)pl.ctas, threads, smem_balanced(shape, a->batch),
+    (w != nullptr ? weights_kernel(true) : balanced_for<kPaged>(shape))<<<
+        (unsigned)pl.ctas, threads, w != nullptr ? smem_weights(true, a->batch) : smem_balanced(shape, a->batch),
                                   reinterpret_cast<cudaStream_t>(stream)>>>(tmk, tmv, p);
   } else {
     const int64_t grid = (int64_t)a->batch * a->kv_heads * pl.splits;
     if (grid >= (1ll << 31)) return FS_ERR_UNSUPPORTED;
-    (w != nullptr ? weights_kernel(false) : kernel_for<kPaged>(shape, debug_mode()))<<<(unsigned)grid, threads, smem_bytes(shape),
+    (w != nullptr ? weights_kernel(false) : kernel_for<kPaged>(shape, debug_mode()))<<<
+        (unsigned)grid, threads, w != nullptr ? smem_weights(false, a->batch) : smem_bytes(shape),
                                               reinterpret_cast<cudaStream_t>(stream)>>>(tmk, tmv, p);
   }
   return launch_status(pl.balanced ? "balanced decode kernel launch" : "split decode kernel launch");

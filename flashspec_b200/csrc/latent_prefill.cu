@@ -55,6 +55,7 @@ struct PrefillParams {
   int64_t nq, nk;
   float scale_log2;
   int B, H;
+  int tile_ctas;  // CTAs that may have queries; the ones behind them clear rows of no request
 };
 
 template <int kDN, int kDR, int kDV>
@@ -103,6 +104,64 @@ __device__ __forceinline__ bool pre_wait(uint64_t* bar, uint32_t parity, volatil
   }
 }
 
+// The w-th piece of work, one warp: (request, its 256-query tile), the request -1 when there
+// is none.  Work is dealt by descending tile index, so that tiles with many keys start first:
+// f(t) = tiles with an index of at least t; the w-th one has the largest t with f(t) > w.
+__device__ __forceinline__ int2 pre_find(const PrefillParams& p, int w, int lane) {
+  auto tiles_of = [&](int b) -> int {
+    int64_t lo;
+    int n = 0;
+    if (b < p.B) pre_range(p.q_off, b, p.nq, lo, n);
+    return (n + 2 * kPreQ - 1) / (2 * kPreQ);
+  };
+  const int mine = tiles_of(lane);  // most batches fit one look
+  auto count = [&](int t) -> int {  // f(t)
+    int x = max(0, mine - t);
+    for (int b = 32 + lane; b < p.B; b += 32) x += max(0, tiles_of(b) - t);
+    return (int)__reduce_add_sync(0xffffffffu, (uint32_t)x);
+  };
+  if (count(0) <= w) return make_int2(-1, 0);
+  int lo = 0, hi = (int)(p.nq / (2 * kPreQ)) + 1;  // f(lo) > w, f(hi) = 0
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (count(mid) > w) lo = mid; else hi = mid;
+  }
+  int k = w - count(lo + 1);  // the k-th request that has a tile of this index
+  for (int base = 0; base < p.B; base += 32) {
+    const uint32_t has = __ballot_sync(0xffffffffu, (base == 0 ? mine : tiles_of(base + lane)) > lo);
+    const int n = __popc(has);
+    if (k < n) return make_int2(base + (int)__fns(has, 0, k + 1), lo);
+    k -= n;
+  }
+  return make_int2(-1, 0);
+}
+
+// Zeros in the rows of out that no request covers, 1024 rows a CTA.  Ascending offsets leave
+// only rows before the first and behind the last; others are looked up row by row.
+constexpr int kClearRows = 1024;
+
+template <int kDV>
+__device__ __forceinline__ void pre_clear(const PrefillParams& p, int chunk) {
+  const int64_t r0 = (int64_t)chunk * kClearRows, r1 = min(p.nq, r0 + kClearRows);
+  const int64_t first = p.q_off[0], last = p.q_off[p.B];
+  bool falls = false;
+  for (int b = threadIdx.x; b < p.B; b += kPreThreads) falls |= p.q_off[b + 1] < p.q_off[b];
+  falls = __syncthreads_or(falls ? 1 : 0) != 0;
+  if (!falls && first <= r0 && last >= r1) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int64_t r = r0 + warp; r < r1; r += kPreThreads / 32) {
+    bool covered = r >= first && r < last;
+    if (falls) {
+      covered = false;
+      for (int b = lane; b < p.B; b += 32) covered |= r >= p.q_off[b] && r < p.q_off[b + 1];
+      covered = __any_sync(0xffffffffu, covered);
+    }
+    if (covered) continue;
+    uint4* row = reinterpret_cast<uint4*>(p.out + (size_t)r * p.H * kDV);
+    for (int i = lane; i < p.H * kDV / 8; i += 32) row[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+
 template <int kDN, int kDR, int kDV, bool kBf16>
 __global__ void __launch_bounds__(kPreThreads, 1)
     latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kv,
@@ -115,32 +174,14 @@ __global__ void __launch_bounds__(kPreThreads, 1)
   __shared__ uint32_t s_tmem;
   __shared__ int s_bad[kDV];             // per dim: first key of an edge tile whose value is not finite
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if ((int)blockIdx.x >= p.tile_ctas) {
+    pre_clear<kDV>(p, (int)blockIdx.x - p.tile_ctas);
+    return;
+  }
   const int h = blockIdx.x % p.H;
-  // the tile: counted from the last request's last one back, so that long tiles start first
-  const int want = (int)(gridDim.x / p.H) - 1 - (int)(blockIdx.x / p.H);
   if (warp == 0) {
-    int carry = 0, fb = -1, ft = 0;
-    for (int base = 0; base < p.B && fb < 0; base += 32) {
-      int64_t lo;
-      int n = 0;
-      if (base + lane < p.B) pre_range(p.q_off, base + lane, p.nq, lo, n);
-      int x = (n + 2 * kPreQ - 1) / (2 * kPreQ);
-      const int mine = x;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-      }
-      const int before = carry + x - mine;
-      const unsigned hit = __ballot_sync(0xffffffffu, want >= before && want < before + mine);
-      if (hit) {
-        const int l = __ffs(hit) - 1;
-        fb = base + l;
-        ft = want - __shfl_sync(0xffffffffu, before, l);
-      }
-      carry += __shfl_sync(0xffffffffu, x, 31);
-    }
-    if (lane == 0) s_find[0] = fb, s_find[1] = ft;
+    const int2 at = pre_find(p, (int)(blockIdx.x / p.H), lane);
+    if (lane == 0) s_find[0] = at.x, s_find[1] = at.y;
   }
   if (tid == 32) {
     mbar_init(smem_u32(&bars.q_full), 1);
@@ -448,7 +489,7 @@ static int pre_map(CUtensorMap* map, const void* base, int64_t n, int64_t row_el
 }
 
 template <int kDN, int kDR, int kDV>
-static int launch_prefill(const FsLatentPrefillArgs* a, const PrefillParams& p, int64_t tiles, void* stream) {
+static int launch_prefill(const FsLatentPrefillArgs* a, const PrefillParams& p, void* stream) {
   using L = PrefillShape<kDN, kDR, kDV>;
   CUtensorMap mq, mkv, mr;
   if (int st = pre_map(&mq, a->q, a->q_rows, (int64_t)a->heads * L::kDQ, kPreQ); st != FS_OK) return st;
@@ -462,14 +503,15 @@ static int launch_prefill(const FsLatentPrefillArgs* a, const PrefillParams& p, 
   if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
       e != cudaSuccess)
     return fail_cuda("shared-memory limit of the latent prefill kernel", e);
-  kernel<<<(unsigned)(tiles * p.H), kPreThreads, L::kSmem, reinterpret_cast<cudaStream_t>(stream)>>>(mq, mkv, mr, p);
+  const int64_t ctas = p.tile_ctas + (a->clear_rest ? (a->q_rows + kClearRows - 1) / kClearRows : 0);
+  kernel<<<(unsigned)ctas, kPreThreads, L::kSmem, reinterpret_cast<cudaStream_t>(stream)>>>(mq, mkv, mr, p);
   return launch_status("latent prefill kernel launch");
 }
 
 template <int kDN, int kDR>
-static int launch_prefill_v(const FsLatentPrefillArgs* a, const PrefillParams& p, int64_t tiles, void* stream) {
-  return a->value_dim == 64 ? launch_prefill<kDN, kDR, 64>(a, p, tiles, stream)
-                            : launch_prefill<kDN, kDR, 128>(a, p, tiles, stream);
+static int launch_prefill_v(const FsLatentPrefillArgs* a, const PrefillParams& p, void* stream) {
+  return a->value_dim == 64 ? launch_prefill<kDN, kDR, 64>(a, p, stream)
+                            : launch_prefill<kDN, kDR, 128>(a, p, stream);
 }
 
 }  // namespace fsb
@@ -491,7 +533,7 @@ extern "C" int fs_latent_prefill(const FsLatentPrefillArgs* a, void* stream) {
     return FS_ERR_ALIGNMENT;
   if (a->q_rows >= (1ll << 30) || a->k_rows >= (1ll << 30) || a->heads > (1 << 20)) return FS_ERR_UNSUPPORTED;
   const int64_t tiles = a->q_rows / (2 * kPreQ) + a->batch;  // at least as many as the requests have
-  if (tiles * a->heads >= (1ll << 31)) return FS_ERR_UNSUPPORTED;
+  if (tiles * a->heads + a->q_rows / kClearRows + 1 >= (1ll << 31)) return FS_ERR_UNSUPPORTED;
   PrefillParams p{};
   p.q_off = a->q_offsets;
   p.k_off = a->k_offsets;
@@ -502,7 +544,8 @@ extern "C" int fs_latent_prefill(const FsLatentPrefillArgs* a, void* stream) {
   p.scale_log2 = a->sm_scale * 1.4426950408889634f;
   p.B = a->batch;
   p.H = a->heads;
+  p.tile_ctas = (int)(tiles * a->heads);
   if (a->nope_dim == 64)
-    return a->rope_dim == 32 ? launch_prefill_v<64, 32>(a, p, tiles, stream) : launch_prefill_v<64, 64>(a, p, tiles, stream);
-  return a->rope_dim == 32 ? launch_prefill_v<128, 32>(a, p, tiles, stream) : launch_prefill_v<128, 64>(a, p, tiles, stream);
+    return a->rope_dim == 32 ? launch_prefill_v<64, 32>(a, p, stream) : launch_prefill_v<64, 64>(a, p, stream);
+  return a->rope_dim == 32 ? launch_prefill_v<128, 32>(a, p, stream) : launch_prefill_v<128, 64>(a, p, stream);
 }

@@ -20,7 +20,7 @@ import torch
 
 from . import _lib
 from .attention import _check_weights, _i64
-from .quant import require_cuda, stream_of
+from .quant import device_guard, require_cuda, stream_of
 
 
 def evict_tokens_cuda(cache, weights: torch.Tensor, budget: int, *, recent: int, sinks: int = 0,
@@ -74,7 +74,7 @@ def evict_tokens_cuda(cache, weights: torch.Tensor, budget: int, *, recent: int,
     if table.ndim != 2 or tuple(lengths.shape) != (table.shape[0],):
         raise ValueError("block_table must be [batch, columns] and lengths [batch]")
     b = int(table.shape[0])
-    with torch.cuda.device(device):
+    with device_guard(device):
         kept = torch.empty((b, hkv, budget), dtype=torch.int32, device=device)
         new_lengths = torch.empty(b, dtype=torch.int64, device=device)
         a = _lib.FsEvictArgs()

@@ -26,7 +26,7 @@ import torch
 
 from . import _lib
 from .attention import _i64
-from .quant import require_cuda, stream_of
+from .quant import device_guard, require_cuda, stream_of
 
 LATENT_DIMS = (128, 256, 512)
 ROPE_DIMS = (32, 64)
@@ -95,19 +95,20 @@ class LatentKVCache:
         the cache's dtype (zeros behind a request's count): what a prompt's expanded keys and
         values should be made of to agree with later steps."""
         _check_cache(self)
-        b, dc, dr = self.batch_size, self.latent_dim, self.rope_dim
-        device = self.values.device
-        if latent.ndim != 3 or rope.ndim != 3 or tuple(latent.shape[:2]) != tuple(rope.shape[:2]):
-            raise ValueError("latent and rope must be [batch, tokens, dim] with the same batch and tokens")
-        t = int(latent.shape[1])
-        if int(latent.shape[0]) != b or int(latent.shape[2]) != dc or int(rope.shape[2]) != dr or t <= 0:
+        pages, page, dc = self.values.shape
+        dr = self.ropes.shape[2]
+        device, dtype = self.values.device, self.ropes.dtype
+        if latent.ndim != 3 or rope.ndim != 3:
+            raise ValueError("latent and rope must be [batch, tokens, dim]")
+        b, t, _ = latent.shape
+        if b != self.block_table.shape[0] or t <= 0 or latent.shape[2] != dc or rope.shape != (b, t, dr):
             raise ValueError("latent must be [batch, tokens > 0, latent_dim] and rope [batch, tokens, rope_dim]")
-        if latent.dtype != self.ropes.dtype or rope.dtype != self.ropes.dtype:
+        if latent.dtype != dtype or rope.dtype != dtype:
             raise ValueError("latent and rope must have the cache's dtype")
         if latent.device != device or rope.device != device:
             raise RuntimeError("latent and rope must be on the cache's CUDA device")
         if counts is not None:
-            if tuple(counts.shape) != (b,):
+            if counts.shape != (b,):
                 raise ValueError("counts must have shape [batch]")
             if counts.device != device:
                 raise RuntimeError("counts must be on the cache's CUDA device")
@@ -117,7 +118,7 @@ class LatentKVCache:
         if rope.stride(-1) != 1:
             rope = rope.contiguous()
         table, lengths = _i64(self.block_table), _i64(self.lengths)
-        with torch.cuda.device(device):
+        with device_guard(device):
             new_lengths = torch.empty(b, dtype=torch.int64, device=device)
             held = torch.empty((b, t, dc), dtype=latent.dtype, device=device) if return_held else None
             a = _lib.FsLatentAppendArgs()
@@ -126,7 +127,7 @@ class LatentKVCache:
             a.rope_stride_b, a.rope_stride_t = rope.stride(0), rope.stride(1)
             a.dtype = _dtype(latent)
             a.batch, a.tokens, a.latent_dim, a.rope_dim = b, t, dc, dr
-            a.page_size, a.table_cols, a.num_pages = self.block_size, int(table.shape[1]), int(self.values.shape[0])
+            a.page_size, a.table_cols, a.num_pages = page, table.shape[1], pages
             a.block_table, a.lengths = table.data_ptr(), lengths.data_ptr()
             a.counts = counts.data_ptr() if counts is not None else None
             a.values, a.scale, a.ropes = self.values.data_ptr(), self.scale.data_ptr(), self.ropes.data_ptr()
@@ -134,8 +135,9 @@ class LatentKVCache:
             a.new_lengths = new_lengths.data_ptr()
             a.device_status = device_status.data_ptr() if device_status is not None else None
             _lib.check(_lib.load().fs_latent_append(C.byref(a), stream_of(device)), "fs_latent_append")
-        longest = min(int(self.max_seq_len) + t, self.block_size * int(table.shape[1]))
+        longest = min(int(self.max_seq_len) + t, page * table.shape[1])
         cache = LatentKVCache(self.values, self.scale, self.ropes, self.block_table, new_lengths, longest)
+        object.__setattr__(cache, "_checked", True)  # this one's tensors and lengths of the same kind
         return (cache, held) if return_held else cache
 
 
@@ -144,6 +146,9 @@ def _dtype(t: torch.Tensor) -> int:
 
 
 def _check_cache(cache: LatentKVCache) -> None:
+    """Raises unless the cache's tensors fit together; once per cache, whose fields are frozen."""
+    if getattr(cache, "_checked", False):
+        return
     v, s, r = cache.values, cache.scale, cache.ropes
     require_cuda(v, "the latent cache")
     if v.ndim != 3 or v.dtype != torch.int8 or r.ndim != 3 or r.dtype not in (torch.float16, torch.bfloat16):
@@ -161,6 +166,7 @@ def _check_cache(cache: LatentKVCache) -> None:
     if cache.block_table.ndim != 2 or int(cache.block_table.shape[1]) <= 0 or int(cache.block_table.shape[0]) <= 0 \
             or tuple(cache.lengths.shape) != (int(cache.block_table.shape[0]),):
         raise ValueError("block_table must be [batch, columns] and lengths [batch]")
+    object.__setattr__(cache, "_checked", True)
 
 
 def latent_attention_cuda(q_latent: torch.Tensor, q_rope: torch.Tensor, cache: LatentKVCache, *,
@@ -178,10 +184,12 @@ def latent_attention_cuda(q_latent: torch.Tensor, q_rope: torch.Tensor, cache: L
     single = q_latent.ndim == 3
     if single and q_rope.ndim == 3:
         q_latent, q_rope = q_latent.unsqueeze(1), q_rope.unsqueeze(1)
-    if q_latent.ndim != 4 or q_rope.ndim != 4 or tuple(q_latent.shape[:3]) != tuple(q_rope.shape[:3]):
+    if q_latent.ndim != 4 or q_rope.ndim != 4 or q_latent.shape[:3] != q_rope.shape[:3]:
         raise ValueError("q_latent and q_rope must be [batch, tokens, heads, dim] (or [batch, heads, dim])")
-    b, t, h, dc = (int(x) for x in q_latent.shape)
-    if b != cache.batch_size or dc != cache.latent_dim or int(q_rope.shape[3]) != cache.rope_dim:
+    b, t, h, dc = q_latent.shape
+    pages, page, latent_dim = cache.values.shape
+    dr = cache.ropes.shape[2]
+    if b != cache.block_table.shape[0] or dc != latent_dim or q_rope.shape[3] != dr:
         raise ValueError("q_latent / q_rope batch and dims must match the cache")
     if t <= 0 or h <= 0:
         raise ValueError("q_latent needs at least one token and one head")
@@ -192,15 +200,15 @@ def latent_attention_cuda(q_latent: torch.Tensor, q_rope: torch.Tensor, cache: L
         raise RuntimeError("q_latent and q_rope must be on the cache's CUDA device")
     q, qr = _aligned(q_latent), _aligned(q_rope)
     table, lengths = _i64(cache.block_table), _i64(cache.lengths)
-    with torch.cuda.device(device):
+    with device_guard(device):
         out = torch.empty_like(q)
         a = _lib.FsLatentArgs()
         a.q, a.q_rope, a.out = q.data_ptr(), qr.data_ptr(), out.data_ptr()
         a.dtype = _dtype(q)
-        a.batch, a.tokens, a.heads, a.latent_dim, a.rope_dim = b, t, h, dc, cache.rope_dim
-        a.page_size, a.table_cols, a.max_seq_len = cache.block_size, int(table.shape[1]), int(cache.max_seq_len)
-        a.sm_scale = 1.0 / math.sqrt(dc + cache.rope_dim) if sm_scale is None else float(sm_scale)
-        a.num_pages = int(cache.values.shape[0])
+        a.batch, a.tokens, a.heads, a.latent_dim, a.rope_dim = b, t, h, dc, dr
+        a.page_size, a.table_cols, a.max_seq_len = page, table.shape[1], int(cache.max_seq_len)
+        a.sm_scale = 1.0 / math.sqrt(dc + dr) if sm_scale is None else float(sm_scale)
+        a.num_pages = pages
         a.values, a.scale, a.ropes = cache.values.data_ptr(), cache.scale.data_ptr(), cache.ropes.data_ptr()
         a.block_table, a.lengths = table.data_ptr(), lengths.data_ptr()
         a.device_status = device_status.data_ptr() if device_status is not None else None
@@ -229,20 +237,20 @@ def latent_prefill_attention_cuda(q: torch.Tensor, kv: torch.Tensor, k_rope: tor
     require_cuda(q, "q")
     if q.ndim != 3 or kv.ndim != 3 or k_rope.ndim != 2:
         raise ValueError("q must be [rows, heads, dim], kv [rows, heads, dim] and k_rope [rows, dim]")
-    nq, h, dq = (int(x) for x in q.shape)
-    nk, dr = int(k_rope.shape[0]), int(k_rope.shape[1])
+    nq, h, dq = q.shape
+    nk, dr = k_rope.shape
     dn = dq - dr
-    dv = int(kv.shape[2]) - dn
-    if int(kv.shape[0]) != nk or int(kv.shape[1]) != h or h <= 0:
+    dv = kv.shape[2] - dn
+    if kv.shape[0] != nk or kv.shape[1] != h or h <= 0:
         raise ValueError("kv must have k_rope's rows and q's heads")
     if dn not in (64, 128) or dv not in (64, 128) or dr not in ROPE_DIMS:
         raise ValueError("nope and value dims must be 64 or 128, the rope dim 32 or 64")
     if q.dtype not in (torch.float16, torch.bfloat16) or kv.dtype != q.dtype or k_rope.dtype != q.dtype:
         raise ValueError("q, kv and k_rope must be fp16 or bf16, all of one dtype")
     device = q.device
-    if any(t.device != device for t in (kv, k_rope, q_offsets, k_offsets)):
+    if kv.device != device or k_rope.device != device or q_offsets.device != device or k_offsets.device != device:
         raise RuntimeError("q, kv, k_rope and the offsets must be on one CUDA device")
-    if q_offsets.ndim != 1 or tuple(q_offsets.shape) != tuple(k_offsets.shape) or int(q_offsets.shape[0]) < 2:
+    if q_offsets.ndim != 1 or q_offsets.shape != k_offsets.shape or q_offsets.shape[0] < 2:
         raise ValueError("q_offsets and k_offsets must be [batch + 1]")
     if out is not None:
         if tuple(out.shape) != (nq, h, dv) or out.dtype != q.dtype or not out.is_contiguous() or out.data_ptr() % 16:
@@ -251,10 +259,10 @@ def latent_prefill_attention_cuda(q: torch.Tensor, kv: torch.Tensor, k_rope: tor
             raise RuntimeError("out must be on q's CUDA device")
     qc, kvc, rc = _aligned(q), _aligned(kv), _aligned(k_rope)
     qo, ko = _i64(q_offsets), _i64(k_offsets)
-    with torch.cuda.device(device):
-        if out is None:
-            out = torch.zeros((nq, h, dv), dtype=q.dtype, device=device)
+    with device_guard(device):
         a = _lib.FsLatentPrefillArgs()
+        if out is None:
+            out, a.clear_rest = torch.empty((nq, h, dv), dtype=q.dtype, device=device), 1
         a.q, a.kv, a.k_rope, a.out = qc.data_ptr(), kvc.data_ptr(), rc.data_ptr(), out.data_ptr()
         a.q_offsets, a.k_offsets = qo.data_ptr(), ko.data_ptr()
         a.q_rows, a.k_rows = nq, nk

@@ -9,6 +9,7 @@ by every entry point of this package.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 from dataclasses import dataclass
 from typing import Dict, Optional, Tuple
@@ -44,6 +45,14 @@ def dtype_code(t: torch.Tensor) -> int:
 
 def stream_of(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_CURRENT = contextlib.nullcontext()
+
+
+def device_guard(device: torch.device):
+    """``torch.cuda.device(device)``, or nothing where it is the current one."""
+    return _CURRENT if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def require_cuda(t: torch.Tensor, what: str) -> None:
