@@ -349,7 +349,7 @@ def paged_quant_attention_weights_cuda(q: torch.Tensor, cache, weights: torch.Te
     hkv, _ = _validate_paged(q, cache)
     num_pages, page = int(cache.k_quant.values.shape[0]), int(cache.block_size)
     _check_weights(weights, (num_pages, hkv, page), q.device, "weights")
-    kq, vq = _contig_quant(cache.k_quant), _contig_quant(cache.v_quant)
+    kq, vq = _dense(cache.k_quant), _dense(cache.v_quant)
     qc, table, lengths = q.contiguous(), _i64(cache.block_table), _i64(cache.lengths)
     out = torch.empty_like(qc)
     a = _decode_args(_lib.FS_LAYOUT_PAGED, qc, kq, vq, out, lengths, table, num_pages, int(cache.max_seq_len), hkv,
@@ -361,6 +361,13 @@ def paged_quant_attention_weights_cuda(q: torch.Tensor, cache, weights: torch.Te
     return out, build_compression_stats(dense, cache.estimated_bytes(), materializes_dense_kv=False,
                                         physical_blocks=float(cache.block_table.ge(0).sum().item()),
                                         num_splits=splits, block_n=int(kq.block_size), num_warps=NUM_WARPS)
+
+
+def _dense(qt):
+    """``_contig_quant`` where anything is not contiguous, else the object itself."""
+    zero = getattr(qt, "zero_point", None)
+    dense = qt.values.is_contiguous() and qt.scale.is_contiguous() and (zero is None or zero.is_contiguous())
+    return qt if dense else _contig_quant(qt)
 
 
 def _check_weights(w: torch.Tensor, shape: Tuple[int, ...], device: torch.device, name: str) -> None:

@@ -68,42 +68,98 @@ __device__ __forceinline__ uint16_t lat_b16(float x, int bf16) {
 
 constexpr int kAppendWarps = 8;
 
-// One warp per new token: lane l takes the elements l, l + 32, ... in groups of kVec.  The
-// code and the scale are the symmetric format's (fs_quantize_symmetric): every operation is
-// rounded once, as 32-bit arithmetic does.
+// N consecutive 16-bit elements, in vector words where kVec (16-byte aligned rows).
+template <int N, bool kVec>
+__device__ __forceinline__ void lat_load(const uint16_t* src, uint16_t (&x)[N]) {
+  if (kVec && N >= 8) {
+#pragma unroll
+    for (int i = 0; i < N / 8; ++i) *reinterpret_cast<uint4*>(x + 8 * i) = reinterpret_cast<const uint4*>(src)[i];
+  } else if (kVec) {
+    *reinterpret_cast<uint2*>(x) = *reinterpret_cast<const uint2*>(src);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = src[i];
+  }
+}
+
+// Out of line: the code by the format's own steps.
+static __device__ __noinline__ float latent_code_exact(float x, float scale) {
+  return fminf(fmaxf(rintf(__fdiv_rn(x, scale)), -127.f), 127.f);
+}
+
+// One warp per new token; lane l takes elements [N l, N l + N), N = dc / 32.  The code and the
+// scale are the symmetric format's (fs_quantize_symmetric): scale = max(amax / 127, 1e-8), code
+// = rint(RN(x / scale)) clamped.  Bound by memory (2 dc read, dc and, with `held`, 2 dc written
+// a token), so the division is done once a token: RN(x RN(1 / scale)) is within 127 * 2^-23 +
+// 2^-18 < 2.1e-5 of RN(x / scale), and one farther than 2^-15 (3.1e-5) from a half-integer has
+// the same rint; the others (0.006%) divide.
+template <int kDC, bool kVec>
 __global__ void __launch_bounds__(kAppendWarps * 32) latent_append_kernel(const LatentAppendParams p) {
+  constexpr int N = kDC / 32;
   const int lane = threadIdx.x & 31;
   const int64_t item = (int64_t)blockIdx.x * kAppendWarps + (threadIdx.x >> 5);
   if (item >= (int64_t)p.B * p.T) return;
-  const int b = (int)(item / p.T), t = (int)(item % p.T);
+  const int b = (int)(item / p.T), t = (int)(item - (int64_t)b * p.T);
   const int64_t count = p.counts != nullptr ? min(max(p.counts[b], (int64_t)0), (int64_t)p.T) : p.T;
   const int64_t len = max(p.lengths[b], (int64_t)0);
   if (t == 0 && lane == 0) p.new_lengths[b] = len + count;
-  const uint16_t* src = static_cast<const uint16_t*>(p.latent) + b * p.ls_b + t * p.ls_t;
-  uint16_t* held = p.held != nullptr ? static_cast<uint16_t*>(p.held) + item * p.dc : nullptr;
+  uint16_t* held = p.held != nullptr ? static_cast<uint16_t*>(p.held) + item * kDC + N * lane : nullptr;
+  alignas(16) uint16_t x[N], hv[N];
+  auto put_held = [&]() {
+    if (held == nullptr) return;
+    if (kVec && N >= 8) {
+#pragma unroll
+      for (int i = 0; i < N / 8; ++i) reinterpret_cast<uint4*>(held)[i] = *reinterpret_cast<const uint4*>(hv + 8 * i);
+    } else if (kVec) {
+      *reinterpret_cast<uint2*>(held) = *reinterpret_cast<const uint2*>(hv);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) held[i] = hv[i];
+    }
+  };
   if (t >= count) {
-    if (held != nullptr)
-      for (int e = lane; e < p.dc; e += 32) held[e] = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) hv[i] = 0;
+    put_held();
     return;
   }
+  lat_load<N, kVec>(static_cast<const uint16_t*>(p.latent) + b * p.ls_b + t * p.ls_t + N * lane, x);
   const int64_t pos = len + t, lp = pos / p.page;
   int64_t phys = lp < p.cols ? p.table[(size_t)b * p.cols + lp] : -1;
   if (phys < 0 || phys >= p.num_pages) {  // no page to write to
     if (lane == 0 && p.status != nullptr) atomicOr(p.status, FS_DEV_BAD_PAGE);
     phys = -1;
   }
-  float amax = 0.f;
-  for (int e = lane; e < p.dc; e += 32) amax = fmaxf(amax, fabsf(lat_f32(src[e], p.bf16)));
+  float v[N], amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    v[i] = lat_f32(x[i], p.bf16);
+    amax = fmaxf(amax, fabsf(v[i]));
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  const float scale = fmaxf(__fdiv_rn(amax, 127.0f), 1.0e-8f);
-  const size_t row = phys < 0 ? 0 : (size_t)phys * p.page + (size_t)(pos - lp * p.page);
-  for (int e = lane; e < p.dc; e += 32) {
-    const float q = fminf(fmaxf(rintf(__fdiv_rn(lat_f32(src[e], p.bf16), scale)), -127.f), 127.f);
-    if (phys >= 0) p.values[row * p.dc + e] = (int8_t)(int)q;
-    if (held != nullptr) held[e] = lat_b16(__fmul_rn(q, scale), p.bf16);
+  const float scale = fmaxf(__fdiv_rn(amax, 127.0f), 1.0e-8f), rcp = __frcp_rn(scale);
+  alignas(16) int8_t code[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float q = __fmul_rn(v[i], rcp);
+    float r = rintf(q);
+    // NaN and what infinities leave fail the comparison and take the exact steps too
+    if (!(fabsf(__fsub_rn(q, r)) < 0.5f - 3.0517578125e-5f)) r = latent_code_exact(v[i], scale);
+    r = fminf(fmaxf(r, -127.f), 127.f);
+    code[i] = (int8_t)(int)r;
+    hv[i] = lat_b16(__fmul_rn(r, scale), p.bf16);
   }
+  put_held();
   if (phys < 0) return;
+  const size_t row = (size_t)phys * p.page + (size_t)(pos - lp * p.page);
+  int8_t* dst = p.values + row * kDC + N * lane;  // a row starts on a 128-byte boundary of the pool
+  if (N == 16)
+    *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(code);
+  else if (N == 8)
+    *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(code);
+  else
+    *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(code);
   if (lane == 0) p.scale[row] = scale;
   const uint16_t* rsrc = static_cast<const uint16_t*>(p.rope) + b * p.rs_b + t * p.rs_t;
   uint16_t* rdst = static_cast<uint16_t*>(p.ropes) + row * p.dr;
@@ -804,6 +860,7 @@ int fs_latent_append(const FsLatentAppendArgs* a, void* stream) {
   if ((reinterpret_cast<uintptr_t>(a->latent) | reinterpret_cast<uintptr_t>(a->rope) |
        reinterpret_cast<uintptr_t>(a->ropes) | reinterpret_cast<uintptr_t>(a->held)) & 1)
     return FS_ERR_ALIGNMENT;
+  if ((reinterpret_cast<uintptr_t>(a->values) & 15) || (reinterpret_cast<uintptr_t>(a->scale) & 3)) return FS_ERR_ALIGNMENT;
   LatentAppendParams p{};
   p.latent = a->latent;
   p.rope = a->rope;
@@ -828,8 +885,18 @@ int fs_latent_append(const FsLatentAppendArgs* a, void* stream) {
   p.page = a->page_size;
   p.cols = a->table_cols;
   p.bf16 = a->dtype == FS_BF16;
-  latent_append_kernel<<<(unsigned)blocks, kAppendWarps * 32, 0, reinterpret_cast<cudaStream_t>(stream)>>>(p);
-  return launch_status("latent append kernel launch");
+  // vector words need 16-byte aligned rows (a view of a packed projection may have none)
+  const bool vec = a->latent_stride_b % 8 == 0 && a->latent_stride_t % 8 == 0 &&
+                   ((reinterpret_cast<uintptr_t>(a->latent) | reinterpret_cast<uintptr_t>(a->held)) & 15) == 0;
+  auto go = [&](auto kernel) {
+    kernel<<<(unsigned)blocks, kAppendWarps * 32, 0, reinterpret_cast<cudaStream_t>(stream)>>>(p);
+    return launch_status("latent append kernel launch");
+  };
+  switch (a->latent_dim) {
+    case 128: return vec ? go(latent_append_kernel<128, true>) : go(latent_append_kernel<128, false>);
+    case 256: return vec ? go(latent_append_kernel<256, true>) : go(latent_append_kernel<256, false>);
+    default: return vec ? go(latent_append_kernel<512, true>) : go(latent_append_kernel<512, false>);
+  }
 }
 
 int fs_latent_workspace_size(const FsLatentArgs* a, size_t* bytes) {
