@@ -15,9 +15,10 @@
 //      16-bit fixed point in two signed bytes (error max|q| 2^-16 of a row), two exact
 //      MMAs; the rotary part on 16-bit MMAs.  The warps split rows, dims and tokens (kMT x
 //      kKS x kTS), so q stays in registers; their partial sums meet in shared memory.
-//   2. softmax: running maximum m of score + log2(scale) and sum of 2^(score - m) per row in
-//      fp32; P = 2^(score - m) * scale in fp16, scaled by 2^14 to use its range whatever the
-//      scale (the largest P is 2^14).
+//   2. softmax: reference m, a running maximum of score + log2(scale) that moves only when the
+//      true one is past it by more than 2^8, and the sum of 2^(score - m), per row in fp32; P =
+//      2^(score - m) * scale * 2^6 in fp16, so that P uses fp16's range whatever the scale: at
+//      most 2^14, in full precision down to 2^-20 of the reference.
 //   3. O += P C: each warp owns its part of the dims, of all rows.  A byte becomes the exact fp16
 //      integer (XOR and byte permute against 0x64 exponent bytes, minus 1152).
 // A share that holds a whole (request, row block) writes the output; others leave normalised
@@ -174,7 +175,8 @@ constexpr int kTile = 64;  // tokens
 constexpr int kSPad = 72;  // floats a row of partial scores
 constexpr int kPPad = 72;  // halves a row of P
 constexpr int kLatMaxBatch = 4096;
-constexpr float kPTop = 16384.f;
+constexpr float kPTop = 64.f;     // P of the reference maximum
+constexpr float kLatSlack = 8.f;  // log2 of what the true maximum may be past the reference: P <= 2^14
 constexpr uint64_t kLatTimeoutNs = 2000000000ull;
 
 struct LatentParams {
@@ -552,8 +554,10 @@ __global__ void __launch_bounds__(LatentShape<kDC, kDR, kMT>::kThreads, LatentSh
       }
 #pragma unroll
       for (int o = L::kTPR / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      const float m_new = fmaxf(m_run, mx);
-      const float alpha = ex2_approx(m_run - m_new);
+      // a row's first maximum is its reference; later ones only when far past it, so that O is
+      // rescaled seldom
+      const bool move = mx > m_run + (m_run == -1.0e30f ? 0.f : kLatSlack);
+      const float m_new = move ? mx : m_run, alpha = ex2_approx(m_run - m_new);
       m_run = m_new;
       l_run *= alpha;
 #pragma unroll
@@ -570,28 +574,21 @@ __global__ void __launch_bounds__(LatentShape<kDC, kDR, kMT>::kThreads, LatentSh
         for (int k = 0; k < L::kGV; k += 2) *reinterpret_cast<uint32_t*>(dst + k) = pack_half2(pr[k], pr[k + 1]);
       }
       if (sj == 0) s_alpha[srow] = alpha;
-      __syncthreads();
+      const bool rescale = __syncthreads_or(move && t > t0 ? 1 : 0) != 0;
 
       // ---- 3. O += P C for this warp's dims
-      float al[kMT][2];
-      bool rescale = false;
+      if (rescale) {
 #pragma unroll
-      for (int i = 0; i < kMT; ++i)
-#pragma unroll
-        for (int r2 = 0; r2 < 2; ++r2) {
-          al[i][r2] = s_alpha[16 * i + g + 8 * r2];
-          rescale |= al[i][r2] != 1.f;
-        }
-      if (__any_sync(0xffffffffu, rescale)) {
-#pragma unroll
-        for (int i = 0; i < kMT; ++i)
+        for (int i = 0; i < kMT; ++i) {
+          const float a0 = s_alpha[16 * i + g], a1 = s_alpha[16 * i + g + 8];
 #pragma unroll
           for (int j = 0; j < L::kOT; ++j) {
-            acc[i][j][0] *= al[i][0];
-            acc[i][j][1] *= al[i][0];
-            acc[i][j][2] *= al[i][1];
-            acc[i][j][3] *= al[i][1];
+            acc[i][j][0] *= a0;
+            acc[i][j][1] *= a0;
+            acc[i][j][2] *= a1;
+            acc[i][j][3] *= a1;
           }
+        }
       }
       const uint32_t p_s = smem_s + L::kOffP;
 #pragma unroll
