@@ -188,7 +188,7 @@ struct LatentParams {
   uint16_t* out;    // [B, T, H, dc]
   float* part_o;    // [ctas][2][rows of a block][dc]
   float* part_lse;  // [ctas][2][rows of a block], log2 domain
-  int* prefix;      // [B + 1] tiles before each request (row blocks not counted)
+  int* prefix;      // [B + 1] units before each request (row blocks not counted)
   uint32_t* status;
   int64_t num_pages, max_seq_len;
   float scale_log2;  // sm_scale * log2(e)
@@ -233,8 +233,8 @@ struct LatentShape {
   static constexpr int kPBytes = kRows * kPPad * 2;
   static constexpr int kOffS = kStages * kStage;
   static constexpr int kOffP = kOffS + kSBytes;
-  static constexpr int kOffMisc = kOffP + kPBytes;  // alpha [rows], qscale [rows], scale and lam [tile], prefix
-  static constexpr int kMiscFloats = 2 * kRows + 2 * kTile;
+  static constexpr int kOffMisc = kOffP + kPBytes;  // alpha, lse, amax [rows], scale and lam [tile], prefix
+  static constexpr int kMiscFloats = 3 * kRows + 2 * kTile;
   static_assert(kTS >= 1 && kMT * kKS * kTS == kWarps, "every warp has a part of the scores");
   static constexpr __host__ __device__ int smem(int batch) {
     return 1024 /* alignment */ + kOffMisc + kMiscFloats * 4 + (batch + 1) * 4;
@@ -254,11 +254,35 @@ __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t& r0, uint32_t& r
                : "r"(addr));
 }
 
-// Tiles before each request, into pre[0 .. B] (shared memory); every thread calls it.
+// The work is divided in a cost space where every (request, row block) is charged kLatPiece
+// virtual tiles ahead of its real ones, for what a piece costs whatever its length (reading the
+// queries, closing it): without it the shares with many short requests ended last.  n units on
+// C = min(CTAs, n) shares of n / C units, the first n % C of them one longer.
+constexpr int kLatPiece = 1;
+
+struct LatentShares {
+  int per, rem;
+  __device__ __forceinline__ LatentShares(int n, int ctas) {
+    const int C = min(ctas, n);
+    per = C > 0 ? n / C : 1;
+    rem = n - per * C;
+  }
+  __device__ __forceinline__ int start(int k) const { return k * per + min(k, rem); }
+  __device__ __forceinline__ int owner(int x) const {  // the share that holds unit x
+    const int head = rem * (per + 1);
+    return x < head ? x / (per + 1) : rem + (x - head) / per;
+  }
+};
+
+// Units of a request, for each of its row blocks.
+__device__ __forceinline__ int latent_units(int tiles) { return tiles > 0 ? tiles + kLatPiece : 0; }
+
+// Units before each request (row blocks not counted), into pre[0 .. B] (shared memory); every
+// thread calls it.
 template <int kThreads>
 __device__ __forceinline__ void latent_prefix(const LatentParams& p, int* pre) {
   const int tid = threadIdx.x, lane = tid & 31;
-  for (int r = tid; r < p.B; r += kThreads) pre[r + 1] = (latent_len(p, r) + kTile - 1) / kTile;
+  for (int r = tid; r < p.B; r += kThreads) pre[r + 1] = latent_units((latent_len(p, r) + kTile - 1) / kTile);
   __syncthreads();
   if (tid < 32) {
     int carry = 0;
@@ -277,9 +301,6 @@ __device__ __forceinline__ void latent_prefix(const LatentParams& p, int* pre) {
   __syncthreads();
 }
 
-// n flat tiles on C = min(CTAs, n) shares, none of them empty; share k starts here.
-__device__ __forceinline__ int64_t latent_share(int64_t n, int k, int C) { return n * k / C; }
-
 template <int kDC, int kDR, int kMT, bool kBf16>
 __global__ void __launch_bounds__(LatentShape<kDC, kDR, kMT>::kThreads, LatentShape<kDC, kDR, kMT>::kCtas)
     latent_attention_kernel(const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_r,
@@ -294,8 +315,9 @@ __global__ void __launch_bounds__(LatentShape<kDC, kDR, kMT>::kThreads, LatentSh
   float* s_part = reinterpret_cast<float*>(lat_smem + L::kOffS);  // [kKS][rows][kSPad]
   __half* s_p = reinterpret_cast<__half*>(lat_smem + L::kOffP);   // [rows][kPPad]
   float* s_alpha = reinterpret_cast<float*>(lat_smem + L::kOffMisc);
-  float* s_qscale = s_alpha + L::kRows;
-  float* s_scale = s_qscale + L::kRows;  // by column, -1 where there is no token
+  float* s_lse = s_alpha + L::kRows;
+  uint32_t* s_amax = reinterpret_cast<uint32_t*>(s_lse + L::kRows);
+  float* s_scale = s_lse + 2 * L::kRows;  // by column, -1 where there is no token
   float* s_lam = s_scale + kTile;        // by column, log2 of it
   int* pre = reinterpret_cast<int*>(s_lam + kTile);
 
@@ -311,28 +333,29 @@ __global__ void __launch_bounds__(LatentShape<kDC, kDR, kMT>::kThreads, LatentSh
   latent_prefix<L::kThreads>(p, pre);
   if (blockIdx.x == 0)
     for (int r = tid; r <= p.B; r += L::kThreads) p.prefix[r] = pre[r];
-  const int64_t total = (int64_t)pre[p.B] * p.row_blocks;
-  const int C = (int)min((int64_t)gridDim.x, total);
-  if ((int)blockIdx.x >= C) return;
-  const int64_t f_begin = latent_share(total, blockIdx.x, C), f_end = latent_share(total, blockIdx.x + 1, C);
+  const int total = pre[p.B] * p.row_blocks;
+  if ((int)blockIdx.x >= min((int)gridDim.x, total)) return;
+  const LatentShares shares(total, gridDim.x);
+  const int f_begin = shares.start(blockIdx.x), f_end = shares.start(blockIdx.x + 1);
   bool first = true;
   uint32_t issued = 0, used = 0;  // tiles put into the ring and taken out of it, over all pieces
 
   const int srow = tid / L::kTPR, sj = tid % L::kTPR;  // softmax thread: row and its columns
   const int box_rows = min(p.page, kTile), per_tile = kTile / box_rows;  // pages (or halves of one) a tile
 
-  for (int64_t f = f_begin; f < f_end;) {
+  for (int f = f_begin; f < f_end;) {
     // ---- the piece: tiles [t0, t1) of row block rb of request b
     int lo = 0, hi = p.B;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if ((int64_t)pre[mid] * p.row_blocks <= f) lo = mid; else hi = mid;
+      if (pre[mid] * p.row_blocks <= f) lo = mid; else hi = mid;
     }
-    const int b = lo, nt = pre[b + 1] - pre[b];
-    const int off = (int)(f - (int64_t)pre[b] * p.row_blocks);
-    const int rb = off / nt, t0 = off - rb * nt;
-    const int t1 = (int)min((int64_t)nt, t0 + (f_end - f));
-    f += t1 - t0;
+    const int b = lo, units = pre[b + 1] - pre[b], nt = units - kLatPiece;
+    const int off = f - pre[b] * p.row_blocks, rb = off / units, o0 = off - rb * units;
+    const int o1 = min(units, o0 + (f_end - f));
+    f += o1 - o0;
+    const int t0 = max(0, o0 - kLatPiece), t1 = o1 - kLatPiece;
+    if (t1 <= t0) continue;  // the share ends within the piece's charge
     const int len = latent_len(p, b);
     const int row0 = rb * L::kRows, rows = min(L::kRows, p.R - row0);
     const uint16_t* qb = p.q + ((size_t)b * p.R + row0) * kDC;
@@ -372,62 +395,74 @@ __global__ void __launch_bounds__(LatentShape<kDC, kDR, kMT>::kThreads, LatentSh
       ++issued;
     };
     int64_t next_phys = -1;
+    if (tid < L::kRows) s_amax[tid] = 0u;
     __syncthreads();  // the previous piece is done with the stages and the row state
     if (warp == 0) {
-      for (int i = 0; i < L::kStages - 1 && t0 + i < t1; ++i) issue(t0 + i, lookup(t0 + i));
-      next_phys = lookup(t0 + L::kStages - 1);
+      int64_t phys[L::kStages];
+#pragma unroll
+      for (int i = 0; i < L::kStages; ++i) phys[i] = lookup(t0 + i);
+#pragma unroll
+      for (int i = 0; i < L::kStages - 1; ++i)
+        if (t0 + i < t1) issue(t0 + i, phys[i]);
+      next_phys = phys[L::kStages - 1];
     }
 
-    // ---- q as 16-bit fixed point: row scales, then this warp's fragments
-    for (int r = warp; r < L::kRows; r += L::kWarps) {
-      float amax = 0.f;
-      bool bad = false;
-      if (r < rows) {
-        for (int e = 4 * lane; e < kDC; e += 128) {
-          const uint2 w = *reinterpret_cast<const uint2*>(qb + (size_t)r * kDC + e);
-          const uint32_t ww[2] = {w.x, w.y};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float v = fabsf(lat_f32((uint16_t)(ww[j >> 1] >> (16 * (j & 1))), kBf16));
-            bad |= !(v < INFINITY);
-            amax = fmaxf(amax, v);
-          }
-        }
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-      bad = __any_sync(0xffffffffu, bad);
-      // a row with infinities or NaN has no scale: its output is NaN
-      if (lane == 0) s_qscale[r] = bad ? __int_as_float(0x7fc00000) : amax / 32639.0f;
-    }
-    __syncthreads();
+    // ---- q as 16-bit fixed point: this warp's words, the rows' largest magnitudes (16-bit
+    // patterns, monotone, NaN above infinity above the rest) over all warps, then the bytes
     uint32_t qhi[L::kQSteps][4], qlo[L::kQSteps][4];  // a0..a3 of the m16n8k32 MMAs
     float fq[2];                                       // row scale * sm_scale * log2 e, rows g and g + 8
+    {
+      uint2 raw[2][L::kQSteps][2];
 #pragma unroll
-    for (int r2 = 0; r2 < 2; ++r2) {
-      const int r = 16 * mt + g + 8 * r2;
-      const float qs = s_qscale[r], inv = qs > 0.f ? 1.f / qs : 0.f;
-      fq[r2] = qs * p.scale_log2;
+      for (int r2 = 0; r2 < 2; ++r2) {
+        const int r = 16 * mt + g + 8 * r2;
+        uint32_t top = 0u;
 #pragma unroll
-      for (int j = 0; j < L::kQSteps; ++j) {
+        for (int j = 0; j < L::kQSteps; ++j)
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {  // the words b0 / b1 of step j: dims 64 (j / 2) + 16 c + 8 (j & 1) + 4 w
-          const int d = ks * L::kSlice + 64 * (j >> 1) + 16 * c + 8 * (j & 1) + 4 * w;
-          uint2 raw = make_uint2(0u, 0u);
-          if (r < rows) raw = *reinterpret_cast<const uint2*>(qb + (size_t)r * kDC + d);
-          const uint32_t ww[2] = {raw.x, raw.y};
-          uint32_t h = 0u, l = 0u;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float v = lat_f32((uint16_t)(ww[e >> 1] >> (16 * (e & 1))), kBf16);
-            const int q16 = max(-32639, min(32639, __float2int_rn(v * inv)));
-            const int qh = (q16 + 128) >> 8;
-            h |= (uint32_t)(qh & 0xff) << (8 * e);
-            l |= (uint32_t)((q16 - (qh << 8)) & 0xff) << (8 * e);
+          for (int w = 0; w < 2; ++w) {  // the words b0 / b1 of step j: dims 64 (j / 2) + 16 c + 8 (j & 1) + 4 w
+            const int d = ks * L::kSlice + 64 * (j >> 1) + 16 * c + 8 * (j & 1) + 4 * w;
+            raw[r2][j][w] = make_uint2(0u, 0u);
+            if (r < rows) raw[r2][j][w] = *reinterpret_cast<const uint2*>(qb + (size_t)r * kDC + d);
           }
-          qhi[j][2 * w + r2] = h;
-          qlo[j][2 * w + r2] = l;
-        }
+#pragma unroll
+        for (int j = 0; j < L::kQSteps; ++j)
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const uint32_t ww[2] = {raw[r2][j][w].x, raw[r2][j][w].y};
+#pragma unroll
+            for (int e = 0; e < 2; ++e) top = max(top, max(ww[e] & 0x7fffu, (ww[e] >> 16) & 0x7fffu));
+          }
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        if (c == 0) atomicMax(s_amax + r, top);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int r2 = 0; r2 < 2; ++r2) {
+        const uint32_t top = s_amax[16 * mt + g + 8 * r2];
+        // a row with infinities or NaN has no scale: its output is NaN
+        const float qs = top >= (kBf16 ? 0x7f80u : 0x7c00u) ? __int_as_float(0x7fc00000)
+                                                            : lat_f32((uint16_t)top, kBf16) / 32639.0f;
+        const float inv = qs > 0.f ? 1.f / qs : 0.f;
+        fq[r2] = qs * p.scale_log2;
+#pragma unroll
+        for (int j = 0; j < L::kQSteps; ++j)
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const uint32_t ww[2] = {raw[r2][j][w].x, raw[r2][j][w].y};
+            uint32_t h = 0u, l = 0u;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float v = lat_f32((uint16_t)(ww[e >> 1] >> (16 * (e & 1))), kBf16);
+              const int q16 = max(-32639, min(32639, __float2int_rn(v * inv)));
+              const int qh = (q16 + 128) >> 8;
+              h |= (uint32_t)(qh & 0xff) << (8 * e);
+              l |= (uint32_t)((q16 - (qh << 8)) & 0xff) << (8 * e);
+            }
+            qhi[j][2 * w + r2] = h;
+            qlo[j][2 * w + r2] = l;
+          }
       }
     }
     uint32_t qr[L::kRPer][4];  // rotary fragments of steps ks, ks + kKS, ...: dims 16 s + 4 c .. + 3
@@ -639,13 +674,13 @@ __global__ void __launch_bounds__(LatentShape<kDC, kDR, kMT>::kThreads, LatentSh
     __syncthreads();  // every warp has read the last alphas
     if (sj == 0) {
       s_alpha[srow] = l > 0.f ? 1.f / (l * kPTop) : (l == 0.f ? 0.f : l);  // NaN stays
-      s_qscale[srow] = l > 0.f ? m_run + log2f(l) : (l == 0.f ? -INFINITY : l);
+      s_lse[srow] = l > 0.f ? m_run + log2f(l) : (l == 0.f ? -INFINITY : l);
     }
     __syncthreads();
     const bool whole = t0 == 0 && t1 == nt;
     const size_t slot = ((size_t)blockIdx.x * 2 + (first ? 0 : 1)) * L::kRows;
     first = false;
-    if (!whole && tid < rows) p.part_lse[slot + tid] = s_qscale[tid];
+    if (!whole && tid < rows) p.part_lse[slot + tid] = s_lse[tid];
 #pragma unroll
     for (int i = 0; i < kMT; ++i)
 #pragma unroll
@@ -682,26 +717,19 @@ __global__ void __launch_bounds__(128) latent_merge_kernel(const LatentParams p,
   cudaGridDependencySynchronize();  // launched early: the shares' results are there now
   const int row = blockIdx.x % p.R, b = blockIdx.x / p.R, rb = row / block_rows, r = row - rb * block_rows;
   const int tid = threadIdx.x, threads = blockDim.x;
-  const int nt = p.prefix[b + 1] - p.prefix[b];
+  const int before = p.prefix[b], units = p.prefix[b + 1] - before, total = p.prefix[p.B] * p.row_blocks;
   uint16_t* out = p.out + ((size_t)b * p.R + row) * dc + 4 * tid;
-  if (nt == 0) {
+  if (units == 0) {
     *reinterpret_cast<uint2*>(out) = make_uint2(0u, 0u);
     return;
   }
-  const int64_t total = (int64_t)p.prefix[p.B] * p.row_blocks;
-  const int C = (int)min((int64_t)ctas, total);
-  const int64_t f0 = (int64_t)p.prefix[b] * p.row_blocks + (int64_t)rb * nt, f1 = f0 + nt;
-  // the share that holds flat tile f: the last one that starts at or before it
-  auto owner = [&](int64_t f) -> int {
-    int k = (int)min((int64_t)C - 1, (f + 1) * C / total);
-    while (k > 0 && latent_share(total, k, C) > f) --k;
-    return k;
-  };
-  const int k0 = owner(f0), k1 = owner(f1 - 1);
+  const LatentShares shares(total, ctas);
+  const int u0 = before * p.row_blocks + rb * units;  // the row block's first unit
+  const int k0 = shares.owner(u0 + kLatPiece), k1 = shares.owner(u0 + units - 1);
   if (k0 == k1) return;  // one share wrote the output itself
   // a share's first piece is in slot 0; the first share's piece is a later one where the
   // share starts before this row block
-  const size_t late = latent_share(total, k0, C) < f0 ? 1 : 0;
+  const size_t late = shares.start(k0) < u0 ? 1 : 0;
   auto slot = [&](int k) -> size_t { return ((size_t)k * 2 + (k == k0 ? late : 0)) * block_rows + r; };
   float M = -INFINITY;
   bool nan = false;
@@ -765,9 +793,10 @@ static int latent_check(const FsLatentArgs* a) {
     return FS_ERR_UNSUPPORTED;
   if (a->num_pages * a->page_size >= (1ll << 31) || a->num_pages >= (1ll << 31)) return FS_ERR_UNSUPPORTED;
   if ((int64_t)a->table_cols * a->page_size >= (1ll << 31) - kTile) return FS_ERR_UNSUPPORTED;
-  // flat tiles are counted in 32 bits before the row blocks
+  // units of work (64 tokens of 16 to 64 rows) are counted in 32 bits
   const int64_t longest = std::min<int64_t>(a->max_seq_len, (int64_t)a->table_cols * a->page_size);
-  if ((longest / kTile + 1) * a->batch >= (1ll << 31)) return FS_ERR_UNSUPPORTED;
+  const int64_t rows = (int64_t)a->tokens * a->heads;
+  if ((longest / kTile + 1 + kLatPiece) * a->batch * ((rows + 15) / 16) >= (1ll << 31)) return FS_ERR_UNSUPPORTED;
   if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->q_rope) |
        reinterpret_cast<uintptr_t>(a->values) | reinterpret_cast<uintptr_t>(a->ropes) |
        reinterpret_cast<uintptr_t>(a->scale) | reinterpret_cast<uintptr_t>(a->out)) & 15)
