@@ -569,12 +569,15 @@ static int evict_check(const FsEvictArgs* a) {
     return FS_ERR_INVALID_ARGUMENT;
   // the kernels read `lengths` while new_lengths is being written
   if (static_cast<const int64_t*>(a->new_lengths) == a->lengths) return FS_ERR_INVALID_ARGUMENT;
+  // K and V move at the same time
+  if (a->k_values == a->v_values || a->k_scale == a->v_scale) return FS_ERR_INVALID_ARGUMENT;
   if (a->page_size <= 0 || a->page_size > 64 || a->head_dim <= 0 || a->head_dim % 16 ||
       a->page_size * (a->head_dim + 16) > 12 * 1024)
     return FS_ERR_UNSUPPORTED;
   if (a->num_pages >= (1ll << 31)) return FS_ERR_UNSUPPORTED;
   if ((int64_t)a->batch * a->kv_heads * 2 * kSelMaxCluster >= (1ll << 31)) return FS_ERR_UNSUPPORTED;
-  if ((int64_t)a->table_cols * a->page_size >= (1ll << 31) - 4 * kSelThreads) return FS_ERR_UNSUPPORTED;
+  // positions are counted in 32 bits, strides of the loops over them included
+  if ((int64_t)a->table_cols * a->page_size >= (1ll << 30) || a->budget >= (1 << 30)) return FS_ERR_UNSUPPORTED;
   if ((reinterpret_cast<uintptr_t>(a->k_values) | reinterpret_cast<uintptr_t>(a->v_values)) & 15)
     return FS_ERR_ALIGNMENT;
   if ((reinterpret_cast<uintptr_t>(a->weights) | reinterpret_cast<uintptr_t>(a->weights_out) |

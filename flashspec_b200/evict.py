@@ -59,6 +59,10 @@ def evict_tokens_cuda(cache, weights: torch.Tensor, budget: int, *, recent: int,
         raise RuntimeError("the pool, block_table and lengths must be on one CUDA device")
     if not all(t.is_contiguous() for t in parts):
         raise ValueError("the pool is changed in place: its tensors must be contiguous")
+    if any(t.dtype != want for t, want in zip(parts, (torch.int8,) * 2 + (torch.float32,) * 2 + (torch.int16,) * 2)):
+        raise ValueError("a pool holds int8 values, fp32 scales and int16 zero points")
+    if kq.values.data_ptr() == vq.values.data_ptr():
+        raise ValueError("K and V must be separate pools: both are changed in place")
     shape = (pages, hkv, page)
     _check_weights(weights, shape, device, "weights")
     out = weights if weights_out is None else weights_out
@@ -68,8 +72,8 @@ def evict_tokens_cuda(cache, weights: torch.Tensor, budget: int, *, recent: int,
         if out.data_ptr() != lo and out.data_ptr() < hi and out.data_ptr() + 4 * out.numel() > lo:
             raise ValueError("weights_out must be weights itself or not overlap it")
     budget, recent, sinks = int(budget), int(recent), int(sinks)
-    if budget <= 0 or recent < 0 or sinks < 0 or recent + sinks > budget:
-        raise ValueError("budget must be positive, recent and sinks not negative and together within the budget")
+    if budget <= 0 or budget >= 1 << 30 or recent < 0 or sinks < 0 or recent + sinks > budget:
+        raise ValueError("budget must be positive (below 2^30), recent and sinks not negative and together within the budget")
     table, lengths = _i64(cache.block_table), _i64(cache.lengths)
     if table.ndim != 2 or tuple(lengths.shape) != (table.shape[0],):
         raise ValueError("block_table must be [batch, columns] and lengths [batch]")

@@ -167,7 +167,7 @@ int fs_paged_decode_weights(const FsDecodeArgs* args, float* weights, void* stre
  *   weights_out: as `weights` (the same array for in place, else disjoint): the kept tokens'
  *     weights at their new places and zeros at every other position of the request's pages
  * Quant block = page, 1 .. 64 tokens, head_dim a multiple of 16, page * (head_dim + 16) <=
- * 12 KB.  Workspace: fs_evict_workspace_size bytes (0 for requests up to 393216 tokens). */
+ * 12 KB; fewer than 2^30 positions a request; K and V in separate pools.  Workspace: fs_evict_workspace_size bytes (0 for requests up to 393216 tokens). */
 typedef struct FsEvictArgs {
   int32_t kv_format;
   int32_t batch, kv_heads, head_dim, page_size, table_cols, max_seq_len;
@@ -231,7 +231,7 @@ int fs_latent_append(const FsLatentAppendArgs* args, void* stream);
  * over the tokens j < lengths[b] - tokens + t + 1 (query t is the token at that end; none:
  * zeros).  q and out [batch, tokens, heads, latent_dim], q_rope [batch, tokens, heads,
  * rope_dim], contiguous, 16-byte aligned.  Unallocated pages are skipped.  At most 4096
- * requests and 2^20 rows (tokens * heads) a request.  Workspace: fs_latent_workspace_size
+ * requests, 2^20 rows (tokens * heads) and 2^30 positions a request, 2^31 tokens a pool.  Workspace: fs_latent_workspace_size
  * bytes, 256-byte aligned, any contents. */
 typedef struct FsLatentArgs {
   const void* q;

@@ -177,9 +177,10 @@ def test_long_rows_take_a_cluster():
     check(cache, w, 5000, 300, 4)
 
 
-def test_rows_too_long_for_shared_memory():
-    """400000 tokens: the selection keeps its keys in the workspace."""
-    n, page = 400000, 64
+@pytest.mark.parametrize("n", [390016, 400000])
+def test_rows_at_and_past_what_shared_memory_holds(n):
+    """390016 tokens fill the clusters' shared memory; with 400000 the keys are in the workspace."""
+    page = 64
     pages = n // page
     g = torch.Generator(device="cuda").manual_seed(1)
     v = torch.randint(-127, 128, (pages, 1, page, 16), generator=g, device="cuda", dtype=torch.int8)
@@ -281,6 +282,10 @@ def test_refusals():
                             torch.zeros((1, 1), dtype=torch.int64, device="cuda"), cache.lengths, 32, 32)
     with pytest.raises(ValueError):
         f(two, torch.zeros((4, 1, 32), device="cuda"), 8, recent=1)  # pages of two quantization blocks
+    with pytest.raises(ValueError):
+        f(fs().PagedKVCache(cache.k_quant, cache.k_quant, cache.block_table, cache.lengths, 16, 60), wd, 8, recent=1)
+    with pytest.raises(ValueError):
+        f(cache, wd, 1 << 30, recent=1)
     kq = cache.k_quant
     turned = fs().QuantizedTensor(kq.values.transpose(3, 4).contiguous().transpose(3, 4), kq.scale, kq.zero_point, 16,
                                   kq.original_shape)

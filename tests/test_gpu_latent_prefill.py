@@ -105,6 +105,11 @@ def test_long_and_peaked():
     check([700], [9000], 2, 128, 64, 128, F, seed=6, sm_scale=1.0)
 
 
+@pytest.mark.parametrize("sm_scale", [-0.1, 0.0])
+def test_scales_of_any_sign(sm_scale):
+    check([300, 77], [420, 77], 2, 128, 64, 128, B, seed=14, sm_scale=sm_scale)
+
+
 def test_rows_of_no_request():
     """Padding rows behind the last request stay as they were, or are zeros."""
     nq = nk = [100, 30]

@@ -76,7 +76,8 @@ def evict_args():
     a = _lib.FsEvictArgs()
     a.batch, a.kv_heads, a.head_dim, a.page_size, a.table_cols, a.max_seq_len = 2, 4, 128, 16, 8, 128
     a.budget, a.recent, a.sinks, a.num_pages = 32, 8, 4, 20
-    a.block_table = a.lengths = a.k_values = a.v_values = a.k_scale = a.v_scale = a.k_zero = a.v_zero = 4096
+    a.block_table = a.lengths = a.k_values = a.k_scale = a.k_zero = a.v_zero = 4096
+    a.v_values = a.v_scale = 16384
     a.weights = a.weights_out = a.kept = 4096
     a.new_lengths = 8192
     return a
@@ -86,7 +87,8 @@ def evict_args():
     (dict(budget=0), 1), (dict(recent=30), 1), (dict(sinks=-1), 1), (dict(kv_format=2), 1), (dict(k_zero=None), 1),
     (dict(kept=None), 1), (dict(new_lengths=4096), 1), (dict(page_size=65), 2), (dict(head_dim=72), 2),
     (dict(page_size=64, head_dim=256), 2), (dict(k_values=4104), 5), (dict(weights=4098), 5),
-    (dict(table_cols=1 << 28), 2), (dict(num_pages=0), 1)])
+    (dict(table_cols=1 << 28), 2), (dict(num_pages=0), 1), (dict(table_cols=1 << 26), 2), (dict(budget=1 << 30), 2),
+    (dict(v_values=4096), 1), (dict(v_scale=4096), 1), (dict(num_pages=1 << 31), 2)])
 def test_evict_refuses(change, status):
     from flashspec_b200 import _lib
 
@@ -122,7 +124,8 @@ def latent_args():
 @pytest.mark.parametrize("change,status", [
     (dict(q=None), 1), (dict(lengths=None), 1), (dict(tokens=0), 1), (dict(heads=0), 1), (dict(num_pages=0), 1),
     (dict(dtype=2), 2), (dict(latent_dim=192), 2), (dict(rope_dim=16), 2), (dict(page_size=48), 2),
-    (dict(batch=4097), 2), (dict(tokens=1 << 17), 2), (dict(table_cols=1 << 26), 2), (dict(values=4104), 5),
+    (dict(batch=4097), 2), (dict(tokens=1 << 17), 2), (dict(table_cols=1 << 24), 2), (dict(values=4104), 5),
+    (dict(num_pages=1 << 25), 2),
     (dict(q=4098), 5), (dict(scale=4097), 5)])
 def test_latent_attention_refuses(change, status):
     from flashspec_b200 import _lib
