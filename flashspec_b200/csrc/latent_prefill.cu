@@ -6,9 +6,11 @@
 //   out[i, h]      = sum_j softmax_j(score) kv[j, h, dn:]
 //
 // A CTA takes 256 queries of one head, as two blocks of 128, and walks the keys in tiles of
-// 96.  (With 128 queries a CTA the K and V tiles, 80 KB per 128 keys, came out of L2 at 6.8
-// TB/s and bound the kernel: 220 us at the packed prompts; tiles of 96 keys let two K and two
-// V tiles fit beside the queries.)  Roles:
+// 96, so that two K and two V tiles fit beside the queries.  Four packed prompts (4096 -> 500
+// tokens, 16 heads) take 201 us, 722 TFLOP/s of useful work.  Measured and dropped: 128 queries
+// a CTA (220 us), an O each for even and odd tiles (230), 128 keys a tile with P over S (222),
+// 80 keys with P beside S (244).  Spinning in place of sleeping waits cost 5% of the kernel.
+// The MMA thread takes its descriptors from precomputed words: building them bound it.  Roles:
 //   warp 0      TMA: the queries once, then K (the head's own chunks and the shared rotary
 //               one, side by side, so it is never copied per head) and V tiles
 //   warp 1      tcgen05.mma: S = Q K^T into TMEM, O += P V with P read from TMEM
