@@ -61,6 +61,7 @@ def evict_tokens_cuda(cache, weights: torch.Tensor, budget: int, *, recent: int,
         raise ValueError("the pool is changed in place: its tensors must be contiguous")
     if any(t.dtype != want for t, want in zip(parts, (torch.int8,) * 2 + (torch.float32,) * 2 + (torch.int16,) * 2)):
         raise ValueError("a pool holds int8 values, fp32 scales and int16 zero points")
+    _check_pool(parts, pages, hkv, page, d, sym)
     if kq.values.data_ptr() == vq.values.data_ptr():
         raise ValueError("K and V must be separate pools: both are changed in place")
     shape = (pages, hkv, page)
@@ -105,3 +106,11 @@ def evict_tokens_cuda(cache, weights: torch.Tensor, budget: int, *, recent: int,
 
     cut = PagedKVCache(kq, vq, cache.block_table, new_lengths, page, min(int(cache.max_seq_len), budget))
     return cut, kept
+
+
+def _check_pool(parts, pages: int, hkv: int, page: int, d: int, sym: bool) -> None:
+    """The kernels write to every part of the pool: raises unless K's and V's values, scales
+    and zero points (in that order) have an entry for each page, head and token or block."""
+    blocks = pages * hkv * (page if sym else 1)
+    if any(t.numel() != pages * hkv * page * d for t in parts[:2]) or any(t.numel() != blocks for t in parts[2:]):
+        raise ValueError("a pool's values, scales and zero points must all cover its pages, heads and tokens")

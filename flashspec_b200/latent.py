@@ -257,6 +257,8 @@ def latent_prefill_attention_cuda(q: torch.Tensor, kv: torch.Tensor, k_rope: tor
             raise ValueError("out must be a contiguous, 16-byte aligned [Nq, H, dv] tensor of q's dtype")
         if out.device != device:
             raise RuntimeError("out must be on q's CUDA device")
+        if any(_overlap(out, t) for t in (q, kv, k_rope)):
+            raise ValueError("out must not overlap q, kv or k_rope: other tiles still read them")
     qc, kvc, rc = _aligned(q), _aligned(kv), _aligned(k_rope)
     qo, ko = _i64(q_offsets), _i64(k_offsets)
     with device_guard(device):
@@ -278,3 +280,12 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     """Contiguous, on a 16-byte boundary (a view into a packed tensor may be neither)."""
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the address ranges that two tensors span have a byte in common (strides are
+    not negative)."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    span = lambda t: (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()  # noqa: E731
+    return a.data_ptr() < b.data_ptr() + span(b) and b.data_ptr() < a.data_ptr() + span(a)

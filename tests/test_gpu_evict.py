@@ -345,3 +345,14 @@ def test_serving_run_with_a_budget():
     assert all(alloc._requests[i].length <= 116 for i in alloc.live_request_ids)
     attn = [op for op in log if op[0] == "attn"]
     assert all(np.isfinite(op[3].astype(np.float32)).all() for op in attn)
+
+
+@pytest.mark.parametrize("fmt", ["affine", "symmetric"])
+def test_pool_whose_parts_differ_in_size_is_refused(fmt):
+    cache, w = make_cache(2, 64, [60], 16, fmt, seed=12)
+    kq, wd = cache.k_quant, torch.from_numpy(w).cuda()
+    short = fs().QuantizedTensor(kq.values, kq.scale[1:].contiguous(), kq.zero_point, 16, kq.original_shape) \
+        if fmt == "affine" else type(kq)(kq.values, kq.scale[1:].contiguous(), kq.block_size, kq.original_shape)
+    with pytest.raises(ValueError):
+        fs().evict_tokens_cuda(fs().PagedKVCache(short, cache.v_quant, cache.block_table, cache.lengths, 16, 60), wd,
+                               8, recent=1)

@@ -218,3 +218,12 @@ def test_prompt_then_steps_of_one_model():
     step = torch.einsum("bthc,hdc->bthd", lat.float(), w_uv.float())
     want = torch.stack([prompt[147:150], prompt[246:249]]).float()
     assert torch.allclose(step, want, atol=6e-3, rtol=6e-3), (step - want).abs().max()
+
+
+def test_out_over_an_input_is_refused():
+    q, kv, r = make([10], [10], 2, 64, 64, 128, F, 14)
+    f, o = fs().latent_prefill_attention_cuda, offsets([10])
+    with pytest.raises(ValueError):
+        f(q, kv, r, o, o, out=q)
+    out = torch.empty_like(q)
+    assert torch.equal(f(q, kv, r, o, o, out=out), f(q, kv, r, o, o)) and out.data_ptr() != q.data_ptr()

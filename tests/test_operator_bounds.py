@@ -166,3 +166,30 @@ def test_latent_prefill_refuses(change, status):
     for k, v in change.items():
         setattr(a, k, v)
     assert _lib.load().fs_latent_prefill(C.byref(a), None) == status
+
+
+def test_pool_whose_parts_differ_in_size_is_refused():
+    import torch
+    from flashspec_b200.evict import _check_pool
+
+    pages, hkv, page, d = 5, 2, 16, 8
+    for sym in (False, True):
+        n = pages * hkv * (page if sym else 1)
+        parts = [torch.zeros(pages * hkv * page * d, dtype=torch.int8)] * 2 + [torch.zeros(n)] * 2
+        parts += [] if sym else [torch.zeros(n, dtype=torch.int16)] * 2
+        _check_pool(parts, pages, hkv, page, d, sym)
+        for i in range(len(parts)):
+            short = list(parts)
+            short[i] = parts[i][:-1]
+            with pytest.raises(ValueError):
+                _check_pool(short, pages, hkv, page, d, sym)
+
+
+def test_overlap():
+    import torch
+    from flashspec_b200.latent import _overlap
+
+    x = torch.zeros(4, 6)
+    assert _overlap(x, x) and _overlap(x, x[3:]) and _overlap(x[:, 5:], x[1:2]) and _overlap(x[:2], x[1:])
+    assert not _overlap(x[:2], x[2:]) and not _overlap(x, torch.zeros(4, 6)) and not _overlap(x[:0], x)
+    assert not _overlap(x[:2, :3], x[2:]) and not _overlap(x[2:], x[:2, 3:])
