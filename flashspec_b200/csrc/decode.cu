@@ -428,15 +428,10 @@ __device__ __forceinline__ void consume_page(uint32_t sbase, const StageOffsets&
   uint32_t vr[16];
 #pragma unroll
   for (int k = 0; k < 4; ++k) ldsm_x4_trans(sbase + off.v[k], vr[4 * k], vr[4 * k + 1], vr[4 * k + 2], vr[4 * k + 3]);
-  __syncwarp();
-  if (lane == 0) mbar_arrive(empty_bar);  // the stage may be refilled now
-  if (kMode == 1) {
-    ws.acc[0][0] += __uint_as_float(((uint32_t)shi[0][0] ^ (uint32_t)slo[1][1] ^ vr[0] ^ vr[15]) & 0x007fffffu);
-    return;
-  }
   const float f = si.ks * qf.qscale * qk_scale_log2;
   const int zc = kWts ? 0 : (128 - (int)si.kz) * qf.q16sum;
-  // per-token scales of this thread's tokens 2c, 2c+1, 8+2c, 9+2c (symmetric format)
+  // per-token scales of this thread's tokens 2c, 2c+1, 8+2c, 9+2c (symmetric format); they lie
+  // in the stage, so it is released behind them
   float fk[4] = {f, f, f, f}, vk[4] = {si.vs, si.vs, si.vs, si.vs};
   if (si.tok != 0u) {
     const float2 k01 = lds64f(si.tok + 8 * c), k89 = lds64f(si.tok + 32 + 8 * c);
@@ -449,6 +444,12 @@ __device__ __forceinline__ void consume_page(uint32_t sbase, const StageOffsets&
     vk[1] = v01.y;
     vk[2] = v89.x;
     vk[3] = v89.y;
+  }
+  __syncwarp();
+  if (lane == 0) mbar_arrive(empty_bar);  // the stage may be refilled now
+  if (kMode == 1) {
+    ws.acc[0][0] += __uint_as_float(((uint32_t)shi[0][0] ^ (uint32_t)slo[1][1] ^ vr[0] ^ vr[15]) & 0x007fffffu);
+    return;
   }
   float t[4];
   if (kWts) {  // 24 bits of q: the sums pass 32 bits together, so they join in fp32

@@ -81,3 +81,44 @@ def test_symmetric_fused_decode_vs_oracle():
     kd = fs().dequantize_int8_symmetric(kq).cpu().numpy()
     vd = fs().dequantize_int8_symmetric(vq).cpu().numpy()
     close(out, O.reference_attention(q.cpu().numpy(), kd, vd, lengths.cpu().numpy()))
+
+
+@pytest.mark.parametrize("kernel", ["split", "balanced"])
+def test_scales_of_one_page_do_not_reach_another(monkeypatch, kernel):
+    """Scales that differ by 64 from page to page, over many times the ring's stages: a warp that
+    read the scales of the page that comes next in its stage would be far off.
+
+    Bound per output element, with A = sum_j p_j |v_j| and delta the score error of 16-bit
+    fixed-point q (max|q| / 32639 / 2 * max_j |k_j|_1 / sqrt(D)): P rounds once to fp16 (2^-11),
+    a score enters on both sides of the quotient (2 delta), V's offset of at most 1152 leaves n / 16
+    MMA additions of 2^-23 each, fp32 sums and exp2 2^-12, and the output rounds once (2^-11)."""
+    monkeypatch.setenv("FLASHSPEC_DECODE_KERNEL", kernel)
+    g = torch.Generator().manual_seed(23)
+    b, hkv, grp, d, page, pages = 3, 2, 4, 128, 16, 150
+    n = page * pages
+    perm = torch.randperm(b * pages, generator=g).view(b, pages)
+    codes = [torch.randint(-127, 128, (b * pages, hkv, page, d), generator=g).to(torch.int8) for _ in "kv"]
+    step = torch.tensor([1.0, 64.0, 8.0])[torch.arange(pages) % 3]
+    scale = []
+    for top in (0.02, 1.0):
+        s = torch.rand((b * pages, hkv, page), generator=g) * 0.5 + 0.5
+        s[perm.reshape(-1)] *= (top / step).repeat(b)[:, None, None]
+        scale.append(s)
+    q = torch.randn((b, hkv * grp, d), generator=g).half()
+    pool = [fs().SymQuantizedTensor(c.cuda(), s.cuda(), page, (b * pages, hkv, page, d)) for c, s in zip(codes, scale)]
+    cache = fs().PagedKVCache(*pool, perm.cuda(), torch.full((b,), n).cuda(), page, n)
+    k, v = ((c.double() * s.double()[..., None])[perm].transpose(1, 2).reshape(b, hkv, n, d)
+            for c, s in zip(codes, scale))
+    qd = q.double().view(b, hkv, grp, d)
+    p = torch.softmax(torch.einsum("bhgd,bhnd->bhgn", qd, k) / d ** 0.5, -1)
+    want = torch.einsum("bhgn,bhnd->bhgd", p, v)
+    delta = qd.abs().amax(-1) / 32639 / 2 * k.abs().sum(-1).amax(-1)[..., None] / d ** 0.5
+    a = torch.einsum("bhgn,bhnd->bhgd", p, v.abs())
+    bound = (2 ** -11 + 2 * delta[..., None] + 2 ** -12) * a + 2 ** -11 * want.abs() + n / 16 * 2 ** -23 * 1152 + 2 ** -24
+    weights = torch.zeros((b * pages, hkv, page), device="cuda")
+    for out in (fs().paged_quant_attention_cuda(q.cuda(), cache),
+                fs().paged_quant_attention_weights_cuda(q.cuda(), cache, weights)):
+        err = (out.double().cpu().view(want.shape) - want).abs()
+        assert bool((err <= bound).all()), float((err / bound).max())
+    got = weights.cpu()[perm].transpose(1, 2).reshape(b, hkv, n).double()
+    assert torch.allclose(got, p.sum(2), rtol=1e-4, atol=1e-9)

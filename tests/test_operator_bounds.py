@@ -193,3 +193,14 @@ def test_overlap():
     assert _overlap(x, x) and _overlap(x, x[3:]) and _overlap(x[:, 5:], x[1:2]) and _overlap(x[:2], x[1:])
     assert not _overlap(x[:2], x[2:]) and not _overlap(x, torch.zeros(4, 6)) and not _overlap(x[:0], x)
     assert not _overlap(x[:2, :3], x[2:]) and not _overlap(x[2:], x[:2, 3:])
+
+
+def test_a_decode_stage_is_released_behind_its_last_read():
+    """The decode's consumer hands a ring stage back to the copies; whatever it reads of the stage
+    (K, V, the token scales) has to be read before that, or the next page's bytes may be there."""
+    src = (HEADER.parents[1] / "flashspec_b200" / "csrc" / "decode.cu").read_text()
+    body = src[src.index("void consume_page("):]
+    body = body[:body.index("\n}\n")]
+    release = body.index("mbar_arrive(empty_bar)")
+    reads = [body.rindex(x) for x in ("sbase + off.k", "sbase + off.v", "si.tok +")]
+    assert body.count("mbar_arrive(") == 1 and max(reads) < release
