@@ -663,7 +663,7 @@ int fs_evict_tokens(const FsEvictArgs* a, void* stream) {
   if (int st = evict_check(a); st != FS_OK) return st;
   const size_t need = evict_workspace(a);
   if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need)) return FS_ERR_WORKSPACE;
-  if (need > 0 && (reinterpret_cast<uintptr_t>(a->workspace) & 3)) return FS_ERR_ALIGNMENT;
+  if (need > 0 && (reinterpret_cast<uintptr_t>(a->workspace) & 255)) return FS_ERR_ALIGNMENT;  // keys go by 16 bytes
   EvictParams p{};
   p.table = a->block_table;
   p.lengths = a->lengths;

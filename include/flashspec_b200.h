@@ -167,7 +167,8 @@ int fs_paged_decode_weights(const FsDecodeArgs* args, float* weights, void* stre
  *   weights_out: as `weights` (the same array for in place, else disjoint): the kept tokens'
  *     weights at their new places and zeros at every other position of the request's pages
  * Quant block = page, 1 .. 64 tokens, head_dim a multiple of 16, page * (head_dim + 16) <=
- * 12 KB; fewer than 2^30 positions a request; K and V in separate pools.  Workspace: fs_evict_workspace_size bytes (0 for requests up to 393216 tokens). */
+ * 12 KB; fewer than 2^30 positions a request; K and V in separate pools.  Workspace:
+ * fs_evict_workspace_size bytes (0 for requests up to 393216 tokens), 256-byte aligned. */
 typedef struct FsEvictArgs {
   int32_t kv_format;
   int32_t batch, kv_heads, head_dim, page_size, table_cols, max_seq_len;

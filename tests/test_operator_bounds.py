@@ -204,3 +204,15 @@ def test_a_decode_stage_is_released_behind_its_last_read():
     release = body.index("mbar_arrive(empty_bar)")
     reads = [body.rindex(x) for x in ("sbase + off.k", "sbase + off.v", "si.tok +")]
     assert body.count("mbar_arrive(") == 1 and max(reads) < release
+
+
+@pytest.mark.parametrize("offset,status", [(4, 5), (8, 5), (16, 5), (128, 5)])
+def test_evict_refuses_an_unaligned_workspace(offset, status):
+    """The keys of a long row are read and written 16 bytes at a time."""
+    from flashspec_b200 import _lib
+
+    lib, a, n = _lib.load(), evict_args(), C.c_size_t(0)
+    a.table_cols, a.max_seq_len = 400000 // 16, 400000
+    assert lib.fs_evict_workspace_size(C.byref(a), C.byref(n)) == 0 and n.value > 0
+    a.workspace, a.workspace_bytes = 1 << 20 | offset, n.value
+    assert lib.fs_evict_tokens(C.byref(a), None) == status
