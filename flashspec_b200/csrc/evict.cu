@@ -76,14 +76,15 @@ __device__ __forceinline__ int64_t live_tokens(const EvictParams& p, int b) {
   return max((int64_t)0, min(min(p.lengths[b], p.max_seq_len), (int64_t)p.cols * p.page));
 }
 
-// Physical page behind position `pos` of request b; -1 when unallocated or outside the pool.
-__device__ __forceinline__ int64_t page_at(const EvictParams& p, int b, int lp) {
+// Page of the pool behind logical page lp of request b (fs_evict_tokens keeps pools below 2^31
+// pages); -1 when unallocated (any negative entry) or outside the pool.
+__device__ __forceinline__ int page_at(const EvictParams& p, int b, int lp) {
   const int64_t phys = p.table[(size_t)b * p.cols + lp];
   if (phys >= p.num_pages) {
     if (p.status != nullptr) atomicOr(p.status, FS_DEV_BAD_PAGE);
     return -1;
   }
-  return phys;
+  return phys < 0 ? -1 : (int)phys;
 }
 
 // Larger weight <-> larger key; -0 counts as +0, NaN (of either sign) is above all, and 0 is
@@ -345,14 +346,14 @@ struct PageMove {
       if (kSym) tp[u] = src;
     }
     if (__all_sync(0xffffffffu, stays)) return;
-    dst = (int)page_at(p, b, pg);
+    dst = page_at(p, b, pg);
 #pragma unroll
     for (int c = 0; c < kCh; ++c) {
       const int e = 16 * (32 * c + lane), t = p.by_dim.quot(e);
       sp[c] = -1;
       if (e < p.page * p.D && t < rows) {
         const int src = kept[pg * p.page + t], lp = p.by_page.quot(src);
-        sp[c] = (int)page_at(p, b, lp);
+        sp[c] = page_at(p, b, lp);
         sr[c] = src - lp * p.page;
       }
     }
@@ -362,7 +363,7 @@ struct PageMove {
         if (tp[u] < 0) continue;
         const int lp = p.by_page.quot(tp[u]);
         tr[u] = tp[u] - lp * p.page;
-        tp[u] = (int)page_at(p, b, lp);
+        tp[u] = page_at(p, b, lp);
       }
     }
   }

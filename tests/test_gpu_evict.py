@@ -356,3 +356,21 @@ def test_pool_whose_parts_differ_in_size_is_refused(fmt):
     with pytest.raises(ValueError):
         fs().evict_tokens_cuda(fs().PagedKVCache(short, cache.v_quant, cache.block_table, cache.lengths, 16, 60), wd,
                                8, recent=1)
+
+
+@pytest.mark.parametrize("fmt", ["affine", "symmetric"])
+@pytest.mark.parametrize("bad", [-2, -2 ** 31, 3 - 2 ** 32, 3 - 2 ** 40, -2 ** 63])
+def test_every_negative_table_entry_counts_as_unallocated(fmt, bad):
+    """Entries whose low 32 bits name a page of the pool among them; none is reported as bad."""
+    got = []
+    for entry in (-1, bad):
+        cache, w = make_cache(2, 64, [200], 16, fmt, seed=13)
+        table = cache.block_table.clone()
+        table[0, 1], table[0, 9] = entry, entry
+        c = fs().PagedKVCache(cache.k_quant, cache.v_quant, table, cache.lengths, 16, 200)
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        wd = torch.from_numpy(w).cuda()
+        cut, kept = fs().evict_tokens_cuda(c, wd, 150, recent=100, sinks=40, device_status=status)
+        got.append((kept, wd, cut.k_quant.values, cut.k_quant.scale, cut.v_quant.values))
+        assert int(status) == 0
+    assert all(torch.equal(x, y) for x, y in zip(*got))
