@@ -131,8 +131,9 @@ __global__ void __launch_bounds__(kAppendWarps * 32) latent_append_kernel(const 
   const uint16_t* rsrc = static_cast<const uint16_t*>(p.rope) + b * p.rs_b + t * p.rs_t;
   const uint16_t r0 = rsrc[lane], r1 = p.dr > 32 ? rsrc[lane + 32] : 0;  // dr is 32 or 64; read
   // beside the latent, not behind the codes' stores: kernel 21 -> 19 us for 8 ragged prompts of up to 4096 tokens
-  const int64_t pos = len + t, lp = pos / p.page;
-  int64_t phys = lp < p.cols ? p.table[(size_t)b * p.cols + lp] : -1;
+  // unsigned: a length near the type's largest value must not wrap to a column of the table
+  const uint64_t pos = (uint64_t)len + t, lp = pos / (uint32_t)p.page;
+  int64_t phys = lp < (uint64_t)p.cols ? p.table[(size_t)b * p.cols + lp] : -1;
   if (phys < 0 || phys >= p.num_pages) {  // no page to write to
     if (lane == 0 && p.status != nullptr) atomicOr(p.status, FS_DEV_BAD_PAGE);
     phys = -1;

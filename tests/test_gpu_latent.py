@@ -329,3 +329,14 @@ def test_refusals():
         f.LatentKVCache.empty(1, 10, latent_dim=100)
     with pytest.raises(ValueError):
         f.LatentKVCache.empty(0, 10)
+
+
+def test_append_behind_the_largest_length_finds_no_page():
+    cache = fs().LatentKVCache.empty(2, 128, dtype=B)
+    lens = torch.tensor([2 ** 63 - 3, 2]).cuda()
+    c = fs().LatentKVCache(cache.values, cache.scale, cache.ropes, cache.block_table, lens, 128)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    x = torch.ones((2, 9, 512), dtype=B, device="cuda")
+    c.append(x, x[..., :64], device_status=status)
+    assert int(status) == 1 and not bool(c.values[:2].any()) and bool((c.values[2, 2:11] == 127).all())
+    assert int((c.values != 0).sum()) == 9 * 512
