@@ -593,6 +593,7 @@ __global__ void __launch_bounds__(LatentShape<kDC, kDR, kMT>::kThreads, LatentSh
         for (int k = 0; k < L::kGV; ++k) {
           const bool seen = t * kTile + lat_token(n0 + k) < limit && !(sc[i][k] < 0.f);
           z[i][k] = seen ? v[k] : -INFINITY;
+          sc[i][k] = seen ? sc[i][k] : 0.f;  // P of an unseen token is 0 whatever its scale
           mx = fmaxf(mx, z[i][k] + lm[k]);
         }
       }

@@ -340,3 +340,30 @@ def test_append_behind_the_largest_length_finds_no_page():
     c.append(x, x[..., :64], device_status=status)
     assert int(status) == 1 and not bool(c.values[:2].any()) and bool((c.values[2, 2:11] == 127).all())
     assert int((c.values != 0).sum()) == 9 * 512
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("h,page,n", [(4, 64, 130), (16, 16, 64), (40, 64, 129)])
+def test_a_bad_token_does_not_reach_queries_before_it(bad, h, page, n):
+    """The last drafted tokens have an infinite or undefined scale: the queries that do not see
+    them give what they gave before, the others NaN."""
+    t = 3
+    cache = make_cache([n, 200], 512, 64, page, F, seed=40 + h)
+    q, qr = queries(2, t, h, 512, 64, F, seed=41)
+    ref = fs().latent_attention_cuda(q, qr, cache)
+    cache.scale[cache.block_table[0, (n - 1) // page], (n - 1) % page] = bad
+    cache.scale[cache.block_table[0, (n - 2) // page], (n - 2) % page] = bad
+    out = fs().latent_attention_cuda(q, qr, cache)
+    assert torch.equal(out[0, 0], ref[0, 0]) and torch.equal(out[1], ref[1])
+    assert bool(out[0, 1:].isnan().all())
+
+
+def test_an_infinite_latent_of_a_draft_stays_behind_the_mask():
+    g = torch.Generator().manual_seed(50)
+    rand = lambda *s: torch.randn(s, generator=g).to(B).cuda()  # noqa: E731
+    cache = fs().LatentKVCache.empty(1, 256, dtype=B).append(rand(1, 100, 512), rand(1, 100, 64))
+    c, r, q, qr = rand(1, 2, 512), rand(1, 2, 64), rand(1, 2, 16, 512), rand(1, 2, 16, 64)
+    ref = fs().latent_attention_cuda(q, qr, cache.append(c, r))
+    c[0, 1, 77] = float("inf")
+    out = fs().latent_attention_cuda(q, qr, cache.append(c, r))
+    assert torch.equal(out[0, 0], ref[0, 0]) and bool(out[0, 1].isnan().all())
