@@ -604,7 +604,8 @@ template <typename Kernel>
 static int launch_cluster(Kernel kernel, const char* what, int64_t rows, int cluster, int threads, size_t smem,
                           const EvictParams& p, void* stream) {
   if (smem > 0) {
-    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    // always the largest size: a call on another host thread may be between this and its launch
+    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelSmemKeys * 4);
         e != cudaSuccess)
       return fail_cuda(what, e);
   }

@@ -374,3 +374,53 @@ def test_every_negative_table_entry_counts_as_unallocated(fmt, bad):
         got.append((kept, wd, cut.k_quant.values, cut.k_quant.scale, cut.v_quant.values))
         assert int(status) == 0
     assert all(torch.equal(x, y) for x, y in zip(*got))
+
+
+def evict_args(cache, w, budget, recent, new_lengths, kept):
+    from flashspec_b200 import _lib
+
+    a, kq, vq = _lib.FsEvictArgs(), cache.k_quant, cache.v_quant
+    a.kv_format = _lib.FS_KV_SYMMETRIC
+    a.batch, a.kv_heads, a.head_dim, a.page_size = 1, w.shape[1], kq.values.shape[-1], cache.block_size
+    a.table_cols, a.max_seq_len = cache.block_table.shape[1], cache.max_seq_len
+    a.budget, a.recent, a.num_pages = budget, recent, w.shape[0]
+    a.block_table, a.lengths = cache.block_table.data_ptr(), cache.lengths.data_ptr()
+    a.k_values, a.k_scale = kq.values.data_ptr(), kq.scale.data_ptr()
+    a.v_values, a.v_scale = vq.values.data_ptr(), vq.scale.data_ptr()
+    a.weights = a.weights_out = w.data_ptr()
+    a.kept, a.new_lengths = kept.data_ptr(), new_lengths.data_ptr()
+    return a
+
+
+def test_calls_on_several_host_threads():
+    """Cuts that need much and little shared memory, entered from several threads at once
+    (ctypes lets go of the interpreter during a call)."""
+    import ctypes as C
+    import threading
+
+    from flashspec_b200 import _lib
+
+    lib, states = _lib.load(), []
+    for n in (300000, 40, 40, 40):
+        cache, w = make_cache(1, 32, [n], 16, "symmetric", seed=n)
+        wd = torch.from_numpy(w).cuda()
+        new, kept = torch.empty(1, dtype=torch.int64, device="cuda"), torch.empty(n, dtype=torch.int32, device="cuda")
+        stream = torch.cuda.Stream()
+        states.append((evict_args(cache, wd, n, 0, new, kept), stream, (cache, wd, new, kept), []))
+    torch.cuda.synchronize()
+
+    def work(a, stream, keep, codes):
+        for i in range(1500):
+            codes.append(lib.fs_evict_tokens(C.byref(a), stream.cuda_stream))
+            if i % 50 == 0:
+                stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=s) for s in states]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for a, _, (cache, wd, new, kept), codes in states:
+        assert set(codes) == {0}, codes
+        assert int(new) == a.budget and torch.equal(kept.cpu(), torch.arange(a.budget, dtype=torch.int32))
