@@ -313,6 +313,14 @@ static size_t generic_smem_for(int dim, int qb) {
   }
 }
 
+// Always the largest size: a call on another host thread may be between this and its launch,
+// and the occupancy below must not depend on the calls before.
+template <typename Kernel>
+static cudaError_t generic_limit(Kernel kernel) {
+  constexpr int kMost = kGW * 4 * kGMaxUnitBytes + (kGMaxG * 256 + kGW * kGMaxG * 64) * 4;
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
+}
+
 bool generic_supports(const FsDecodeArgs* a) {
   const int d = a->head_dim, qb = a->block_size;
   if (d != 32 && d != 64 && d != 128 && d != 256) return false;
@@ -330,7 +338,8 @@ static int generic_splits(const FsDecodeArgs* a, int device, size_t smem) {
   if (a->shard_o != nullptr) return 1;
   if (a->num_splits > 0) return a->num_splits;
   int per_sm = 0;
-  cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, decode_generic_kernel<128, false>, kGW * 32, smem);
+  if (generic_limit(decode_generic_kernel<128, false>) == cudaSuccess)
+    cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, decode_generic_kernel<128, false>, kGW * 32, smem);
   if (per_sm <= 0) per_sm = 1;
   const int64_t slots = (int64_t)per_sm * device_sm_count(device) * 2;
   const int64_t pairs = (int64_t)a->batch * a->kv_heads;
@@ -411,8 +420,7 @@ int launch_generic_decode(const FsDecodeArgs* a, int device, void* stream, const
   if (grid >= (1ll << 31)) return FS_ERR_UNSUPPORTED;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   auto go = [&](auto kernel) -> int {
-    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        e != cudaSuccess)
+    if (cudaError_t e = generic_limit(kernel); e != cudaSuccess)
       return fail_cuda("shared-memory limit of the generic decode kernel", e);
     kernel<<<(unsigned)grid, kGW * 32, smem, st>>>(p);
     return launch_status("generic decode kernel launch");

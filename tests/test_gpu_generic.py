@@ -201,3 +201,69 @@ def test_unsupported_shapes_raise():
     q32 = dev(q)  # fp32 q
     with pytest.raises(ValueError):
         fs().paged_quant_attention_cuda(q32, cache_dev(oc))
+
+
+FRESH = """
+import torch, flashspec_b200 as fs
+from flashspec_b200 import attention
+g = torch.Generator(device="cuda").manual_seed(1)
+k, v = (torch.randn((8, 4, 9000, 128), generator=g, device="cuda", dtype=torch.float16) for _ in "kv")
+q = torch.randn((8, 8, 128), generator=g, device="cuda", dtype=torch.float16)
+runs = []
+for _ in range(3):
+    attention._plans.clear()  # each call plans anew, as each process does
+    cache = fs.PagedKVCache.from_dense(k, v, block_size=32)
+    runs.append(fs.paged_quant_attention_cuda(q, cache, return_stats=True))
+assert len({r[1]["num_splits"] for r in runs}) == 1, [r[1]["num_splits"] for r in runs]
+assert all(torch.equal(r[0], runs[0][0]) for r in runs)
+"""
+
+
+def test_the_first_call_of_a_process_plans_as_later_ones_do():
+    """64 KB of shared memory a CTA: more than a kernel may have before its limit is raised."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    root = Path(fs().__file__).resolve().parents[1]
+    done = subprocess.run([sys.executable, "-c", FRESH], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
+
+
+def test_calls_on_several_host_threads():
+    """Quantization blocks that need much and little shared memory, entered from several
+    threads at once (ctypes lets go of the interpreter during a call)."""
+    import ctypes as C
+    import threading
+
+    from flashspec_b200 import _lib
+    from flashspec_b200.attention import _decode_args
+
+    lib, states = _lib.load(), []
+    for qb in (64, 16, 16, 16):
+        g = torch.Generator(device="cuda").manual_seed(qb)
+        k, v = (torch.randn((1, 1, 64, 64), generator=g, device="cuda") for _ in "kv")
+        q = torch.randn((1, 2, 64), generator=g, device="cuda").half()
+        cache = fs().PagedKVCache.from_dense(k, v, block_size=qb)
+        out = torch.empty_like(q)
+        a = _decode_args(_lib.FS_LAYOUT_PAGED, q, cache.k_quant, cache.v_quant, out, cache.lengths, cache.block_table,
+                         64 // qb, 64, 1, None, page_size=qb)
+        a.num_splits = 1
+        want = fs().paged_quant_attention_cuda(q, cache, num_splits=1)
+        states.append((a, torch.cuda.Stream(), (q, cache, out, want), []))
+    torch.cuda.synchronize()
+
+    def work(a, stream, keep, codes):
+        for i in range(1500):
+            codes.append(lib.fs_paged_decode(C.byref(a), stream.cuda_stream))
+            if i % 50 == 0:
+                stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=s) for s in states]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for _, _, (q, cache, out, want), codes in states:
+        assert set(codes) == {0} and torch.equal(out, want)
