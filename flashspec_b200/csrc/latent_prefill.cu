@@ -22,8 +22,10 @@
 //
 // A value that is not finite must not reach queries that do not see its key (0 * inf is NaN).
 // Only tiles on the causal edge are seen by some of a block's queries and not by others (and
-// only they may hold rows of the next request): there such values are set to zero and the
-// first key that has one is noted per dim; the CTA's queries that see that key get NaN.
+// only they may hold rows of the next request): there such values are set to zero.  Elsewhere
+// they go through the MMA, where a probability that 16 bits round to zero makes NaN of an
+// infinity.  A CTA that met one either way looks its values over once more (pre_mend) and gives
+// each query what the definition gives: infinity where it sees infinities of one sign, else NaN.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -50,6 +52,7 @@ constexpr float kPreSlack = 8.f;     // log2 of what the true maximum may be pas
 constexpr uint64_t kPreTimeoutNs = 2000000000ull;
 
 struct PrefillParams {
+  const uint16_t* kv;    // [Nk, H, dn + dv]
   const int64_t* q_off;  // [B + 1]
   const int64_t* k_off;
   uint16_t* out;  // [Nq, H, dv]
@@ -164,6 +167,49 @@ __device__ __forceinline__ void pre_clear(const PrefillParams& p, int chunk) {
   }
 }
 
+// OR of x over the two softmax groups; also orders their shared memory.
+__device__ __forceinline__ bool pre_any(bool x) {
+  uint32_t r;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n bar.red.or.pred q, 1, 256, p;\n selp.b32 %0, 1, 0, q;\n}\n"
+      : "=r"(r)
+      : "r"((uint32_t)x)
+      : "memory");
+  return r != 0;
+}
+
+// The softmax groups of a CTA that met values that are not finite: the first key of each dim
+// whose value is NaN, +inf and -inf (first [3][kDV], shared), among the keys that any query of
+// the CTA sees; then this thread's output row, whose last key is `limit` (-1: no row), gets its
+// infinities and NaN.  Out of line: it costs the kernel no registers, and a V pass when it runs.
+// v0: the first key's value of this head; stride: elements from key to key.
+template <int kDV, bool kBf16>
+static __device__ __noinline__ void pre_mend(const uint16_t* v0, int64_t stride, int keys, int* first, int limit,
+                                             uint16_t* dst) {
+  constexpr int kThreads = 2 * kPreSoft, kUnits = kDV / 8;
+  constexpr uint32_t kInf = kBf16 ? 0x7f80u : 0x7c00u;
+  const int t = threadIdx.x - (kPreThreads - kThreads);
+  for (int i = t; i < 3 * kDV; i += kThreads) first[i] = INT_MAX;
+  pre_any(false);
+  for (int64_t i = t; i < (int64_t)keys * kUnits; i += kThreads) {
+    const int key = (int)(i / kUnits), u = (int)(i % kUnits);
+    const uint4 v = *reinterpret_cast<const uint4*>(v0 + key * stride + 8 * u);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t e = (w[k >> 1] >> (16 * (k & 1))) & 0xffffu;
+      if ((e & 0x7fffu) < kInf) continue;
+      int* at = first + ((e & 0x7fffu) > kInf ? 0 : (e >> 15) + 1) * kDV + 8 * u + k;
+      if (key < *reinterpret_cast<volatile int*>(at)) atomicMin(at, key);
+    }
+  }
+  pre_any(false);
+  for (int d = 0; d < kDV; ++d) {
+    const bool nan = first[d] <= limit, pos = first[kDV + d] <= limit, neg = first[2 * kDV + d] <= limit;
+    if (nan || pos || neg) dst[d] = (uint16_t)(nan || (pos && neg) ? 0x7fffu : pos ? kInf : 0x8000u | kInf);
+  }
+}
+
 template <int kDN, int kDR, int kDV, bool kBf16>
 __global__ void __launch_bounds__(kPreThreads, 1)
     latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kv,
@@ -174,7 +220,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
   __shared__ int s_find[2];
   __shared__ volatile int s_abort;
   __shared__ uint32_t s_tmem;
-  __shared__ int s_bad[kDV];             // per dim: first key of an edge tile whose value is not finite
+  __shared__ int s_first[3 * kDV];  // pre_mend's
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if ((int)blockIdx.x >= p.tile_ctas) {
     pre_clear<kDV>(p, (int)blockIdx.x - p.tile_ctas);
@@ -200,7 +246,6 @@ __global__ void __launch_bounds__(kPreThreads, 1)
     fence_mbar_init();
     fence_proxy_async_smem();
   }
-  if (tid < kDV) s_bad[tid] = INT_MAX;
   __syncthreads();
   const int b = s_find[0];
   if (b < 0) return;  // more CTAs than tiles: the host knows only an upper bound
@@ -394,14 +439,10 @@ __global__ void __launch_bounds__(kPreThreads, 1)
             here |= (((w[k] & kMask) + kLow) & 0x80008000u) != 0u;
           }
           if (here) {
-            const int ch = i / (kPreK * 8), r = (i >> 3) % kPreK, u = i & 7;
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
               const uint16_t e = (uint16_t)(w[k >> 1] >> (16 * (k & 1)));
-              if ((e & kExp) == kExp) {
-                atomicMin(s_bad + 64 * ch + 8 * (u ^ (r & 7)) + k, j0 + r);
-                w[k >> 1] &= (k & 1) ? 0x0000ffffu : 0xffff0000u;
-              }
+              if ((e & kExp) == kExp) w[k >> 1] &= (k & 1) ? 0x0000ffffu : 0xffff0000u;
             }
             *at = make_uint4(w[0], w[1], w[2], w[3]);
             any_bad = true;
@@ -419,23 +460,14 @@ __global__ void __launch_bounds__(kPreThreads, 1)
     }
     if (n > 0 && ok) ok = pre_wait(&bars.pv_done[grp], 0, &s_abort);
     __syncwarp();
-    auto any_of = [](bool x) -> bool {  // OR over both groups; also orders their shared memory
-      uint32_t r;
-      asm volatile(
-          "{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n bar.red.or.pred q, 1, 256, p;\n selp.b32 %0, 1, 0, q;\n}\n"
-          : "=r"(r)
-          : "r"((uint32_t)x)
-          : "memory");
-      return r != 0;
-    };
-    const bool failed = any_of(!ok);
-    any_bad = any_of(any_bad);
+    const bool failed = pre_any(!ok);
+    uint16_t* dst = p.out + ((size_t)(q0 + first + row) * p.H + h) * kDV;
     if (failed) {
       if (grp == 0 && grp_tid == 0 && p.status != nullptr) atomicOr(p.status, FS_DEV_TIMEOUT);
     } else {
       tcgen05_fence_after();
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      uint16_t* dst = p.out + ((size_t)(q0 + first + row) * p.H + h) * kDV;
+      bool bad = false;
 #pragma unroll
       for (int c = 0; c < kDV / 16; ++c) {
         uint32_t o[16];
@@ -456,7 +488,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
 #pragma unroll
               for (int u = 0; u < 2; ++u) {
                 v[u] = __uint_as_float(o[k + 2 * e + u]) * inv;
-                if (any_bad && s_bad[16 * c + k + 2 * e + u] <= limit) v[u] = __int_as_float(0x7fc00000);
+                bad |= !(fabsf(v[u]) < INFINITY);
               }
               w[e] = pre_pack<kBf16>(v[0], v[1]);
             }
@@ -465,6 +497,13 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         }
         __syncwarp();
       }
+      any_bad |= bad && l == l;  // a row whose probabilities are undefined is NaN throughout already
+    }
+    if (pre_any(any_bad && !failed)) {
+      const int keys = min(nk, i0 + min(2 * kPreQ, nq - i0) + shift);
+      const int64_t stride = (int64_t)p.H * (kDN + kDV);
+      pre_mend<kDV, kBf16>(p.kv + k0 * stride + (int64_t)h * (kDN + kDV) + kDN, stride, keys, s_first,
+                           row < rows && l == l ? limit : -1, dst);
     }
     tcgen05_fence_before();
   }
@@ -537,6 +576,7 @@ extern "C" int fs_latent_prefill(const FsLatentPrefillArgs* a, void* stream) {
   const int64_t tiles = a->q_rows / (2 * kPreQ) + a->batch;  // at least as many as the requests have
   if (tiles * a->heads + a->q_rows / kClearRows + 1 >= (1ll << 31)) return FS_ERR_UNSUPPORTED;
   PrefillParams p{};
+  p.kv = static_cast<const uint16_t*>(a->kv);
   p.q_off = a->q_offsets;
   p.k_off = a->k_offsets;
   p.out = static_cast<uint16_t*>(a->out);

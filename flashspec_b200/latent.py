@@ -233,7 +233,9 @@ def latent_prefill_attention_cuda(q: torch.Tensor, kv: torch.Tensor, k_rope: tor
     sees keys j <= i + nk - nq, so a chunk of new tokens sees a cached prefix and, in order,
     itself; a query that sees no key gives zeros.  dn and dv 64 or 128, dr 32 or 64 (dr is read
     from k_rope, dn from q).  Returns out [Nq, H, dv]; a given ``out`` keeps the rows that no
-    request covers, otherwise those are zeros.  sm_scale defaults to 1 / sqrt(dn + dr)."""
+    request covers, otherwise those are zeros.  An infinite or undefined value reaches the
+    queries that see its key and no others: infinities of one sign give infinity, else NaN.
+    sm_scale defaults to 1 / sqrt(dn + dr)."""
     require_cuda(q, "q")
     if q.ndim != 3 or kv.ndim != 3 or k_rope.ndim != 2:
         raise ValueError("q must be [rows, heads, dim], kv [rows, heads, dim] and k_rope [rows, dim]")

@@ -227,3 +227,53 @@ def test_out_over_an_input_is_refused():
         f(q, kv, r, o, o, out=q)
     out = torch.empty_like(q)
     assert torch.equal(f(q, kv, r, o, o, out=out), f(q, kv, r, o, o)) and out.data_ptr() != q.data_ptr()
+
+
+def expect_infinite(q, kv, r, nq, nk, sm_scale):
+    """As expect, for values that may be infinite or NaN: (finite part and bound, where +inf, -inf, NaN)."""
+    dn = q.shape[2] - r.shape[1]
+    plain = kv.clone()
+    plain[..., dn:] = torch.nan_to_num(plain[..., dn:], nan=0.0, posinf=0.0, neginf=0.0)
+    out, bound = expect(q, plain, r, nq, nk, sm_scale)
+    hits = [torch.zeros(out.shape, dtype=torch.bool, device="cuda") for _ in range(3)]
+    q0 = k0 = 0
+    for a, b in zip(nq, nk):
+        v = kv[k0:k0 + b, :, dn:]
+        seen = torch.ones((a, b), dtype=torch.double, device="cuda").tril(b - a)
+        for hit, what in zip(hits, (v.isposinf(), v.isneginf(), v.isnan())):
+            hit[q0:q0 + a] = torch.einsum("ij,jhd->ihd", seen, what.double()) > 0
+        q0, k0 = q0 + a, k0 + b
+    pos, neg, nan = hits
+    nan = nan | (pos & neg)
+    return out, bound, pos & ~nan, neg & ~nan, nan
+
+
+@pytest.mark.parametrize("dtype", [F, B])
+@pytest.mark.parametrize("nq,nk,sm_scale", [([300], [300], None), ([40, 500], [700, 520], None),
+                                            ([40, 500], [700, 520], 1.0), ([200, 9], [150, 2], None)])
+def test_infinite_values_by_the_definition(dtype, nq, nk, sm_scale):
+    """Infinite and undefined values on the causal edge, far inside it, and under probabilities
+    that 16 bits round to zero (sm_scale 1): a query that sees one gets infinity where all that
+    it sees have one sign, else NaN; the other queries and dims what they had."""
+    q, kv, r = make(nq, nk, 2, 128, 64, 128, dtype, 15)
+    g = torch.Generator().manual_seed(16)
+    for k in range(24):
+        key = int(torch.randint(0, sum(nk), (1,), generator=g))
+        kv[key, k % 2, 128 + 5 * k] = (float("inf"), -float("inf"), float("nan"), float("inf"))[k % 4]
+    kv[3, 0, 200], kv[sum(nk) - 4, 0, 200] = float("inf"), -float("inf")  # of one dim
+    out, bound, pos, neg, nan = expect_infinite(q, kv, r, nq, nk, 192 ** -0.5 if sm_scale is None else sm_scale)
+    got = fs().latent_prefill_attention_cuda(q, kv, r, offsets(nq), offsets(nk), sm_scale=sm_scale).double()
+    assert torch.equal(got.isposinf(), pos) and torch.equal(got.isneginf(), neg) and torch.equal(got.isnan(), nan)
+    fine = ~(pos | neg | nan)
+    assert bool(pos.any()) and bool(neg.any()) and bool(nan.any())
+    assert bool(((got - out).abs() <= bound)[fine].all())
+
+
+def test_every_value_infinite():
+    """All of V: the largest number of elements to look over again."""
+    q, kv, r = make([600], [2000], 2, 64, 32, 64, B, 17)
+    kv[..., 64:] = float("inf")
+    kv[1800:, 1, 64:] = -float("inf")
+    out = fs().latent_prefill_attention_cuda(q, kv, r, offsets([600]), offsets([2000]))
+    assert bool(out[:, 0].isposinf().all())
+    assert bool(out[:400, 1].isposinf().all()) and bool(out[400:, 1].isnan().all())
