@@ -17,8 +17,8 @@
 //   warps 4-7   softmax of the first block, one thread a row; warps 8-11 of the second
 // The blocks do not wait for each other: the tensor cores work on one's tile while the other
 // forms exponentials.  P goes back to TMEM in 16 bits over the scores.  The reference maximum
-// moves only when the true one is past it by more than 2^8 (P then stays below 256, sums are
-// in fp32, and O is rescaled seldom instead of once a tile).
+// moves only when the true one is far past it (PreRange; sums are in fp32, and O is rescaled
+// seldom instead of once a tile).
 //
 // A value that is not finite must not reach queries that do not see its key (0 * inf is NaN).
 // Only tiles on the causal edge are seen by some of a block's queries and not by others (and
@@ -48,7 +48,15 @@ constexpr int kPreQ = 128;     // queries of a block, two blocks a CTA
 constexpr int kPreK = 96;      // keys of a tile
 constexpr int kQChunk = kPreQ * 128;  // bytes of a 64-element chunk: rows of 128 bytes
 constexpr int kChunk = kPreK * 128;
-constexpr float kPreSlack = 8.f;     // log2 of what the true maximum may be past the reference
+// P = 2^(score - reference + kLift).  The true maximum may be 2^kSlack past the reference.  fp16
+// ends at 2^16 and loses bits below 2^-14: the lift keeps all of them down to 2^-25 of the
+// maximum, where many far keys beside one near key of small value still make the output
+// (without it 30000 keys at 2^-24.5 were rounded to nothing, and the output with them).  bf16 has
+// the range of fp32 and needs no lift.
+template <bool kBf16>
+struct PreRange {
+  static constexpr float kSlack = kBf16 ? 8.f : 4.f, kLift = kBf16 ? 0.f : 11.f;
+};
 constexpr uint64_t kPreTimeoutNs = 2000000000ull;
 
 struct PrefillParams {
@@ -390,7 +398,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       const float mul = edge ? 1.f : p.scale_log2;
       const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * fabsf(mul);
       // a row's first maximum is its reference; later ones only when far past it
-      const bool move = mx > m_ref + (m_ref == -1.0e30f ? 0.f : kPreSlack);
+      const bool move = mx > m_ref + (m_ref == -1.0e30f ? 0.f : PreRange<kBf16>::kSlack);
       if (__any_sync(0xffffffffu, move)) {
         const float m_new = move ? mx : m_ref;
         if (j > 0) {  // O is there (its MMAs were issued before this tile's): bring it to the new reference
@@ -408,14 +416,15 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         }
         m_ref = m_new;
       }
+      const float up = PreRange<kBf16>::kLift - m_ref;
       float l4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int c = 0; c < kPreK / 32; ++c) {
         uint32_t packed[16];
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
-          const float p0 = ex2_approx(fmaf(__uint_as_float(raw[c][2 * k]), mul, -m_ref));
-          const float p1 = ex2_approx(fmaf(__uint_as_float(raw[c][2 * k + 1]), mul, -m_ref));
+          const float p0 = ex2_approx(fmaf(__uint_as_float(raw[c][2 * k]), mul, up));
+          const float p1 = ex2_approx(fmaf(__uint_as_float(raw[c][2 * k + 1]), mul, up));
           l4[k & 3] += p0 + p1;
           packed[k] = pre_pack<kBf16>(p0, p1);
         }

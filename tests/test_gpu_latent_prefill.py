@@ -277,3 +277,23 @@ def test_every_value_infinite():
     out = fs().latent_prefill_attention_cuda(q, kv, r, offsets([600]), offsets([2000]))
     assert bool(out[:, 0].isposinf().all())
     assert bool(out[:400, 1].isposinf().all()) and bool(out[400:, 1].isnan().all())
+
+
+@pytest.mark.parametrize("dtype", [F, B])
+@pytest.mark.parametrize("near", [0, 100, 29000])
+def test_many_far_keys_beside_a_near_one_without_value(dtype, near):
+    """One key takes nearly all of the weight and has value zero (a sink); the output is what
+    30000 keys at e^-17 of it add up to.  P keeps its relative precision down to 2^-25 (e^-17 is
+    2^-24.5), so the bound of the other cases holds here too; without that fp16 gave zero."""
+    n, nq = 30000, 300
+    q = torch.zeros((nq, 1, 96), dtype=dtype, device="cuda")
+    q[..., 0] = 1
+    kv = torch.zeros((n, 1, 128), dtype=dtype, device="cuda")
+    kv[..., 0], kv[near, 0, 0] = -1.0, 16.0
+    kv[..., 64:] = (torch.rand((n, 1, 64), generator=torch.Generator().manual_seed(1)) + 0.5).to(dtype).cuda()
+    kv[near, 0, 64:] = 0
+    r = torch.zeros((n, 32), dtype=dtype, device="cuda")
+    want, bound = expect(q, kv, r, [nq], [n], 1.0)
+    out = fs().latent_prefill_attention_cuda(q, kv, r, offsets([nq]), offsets([n]), sm_scale=1.0)
+    err = (out.double() - want).abs()
+    assert float(want.min()) > 1e-3 and bool((err <= bound).all()), float((err / bound).max())
