@@ -16,9 +16,10 @@
 //      MMAs; the rotary part on 16-bit MMAs.  The warps split rows, dims and tokens (kMT x
 //      kKS x kTS), so q stays in registers; their partial sums meet in shared memory.
 //   2. softmax: reference m, a running maximum of score + log2(scale) that moves only when the
-//      true one is past it by more than 2^8, and the sum of 2^(score - m), per row in fp32; P =
-//      2^(score - m) * scale * 2^6 in fp16, so that P uses fp16's range whatever the scale: at
-//      most 2^14, in full precision down to 2^-20 of the reference.
+//      true one is past it by more than 2^4, and the sum of 2^(score - m), per row in fp32; P =
+//      2^(score - m) * scale * 2^11 in fp16, so that P uses fp16's range whatever the scale: at
+//      most 2^15, in full precision down to 2^-25 of the reference (many far tokens make the
+//      dims in which one near token is zero).
 //   3. O += P C: each warp owns its part of the dims, of all rows.  A byte becomes the exact fp16
 //      integer (XOR and byte permute against 0x64 exponent bytes, minus 1152).
 // A share that holds a whole (request, row block) writes the output; others leave normalised
@@ -182,8 +183,8 @@ constexpr int kTile = 64;  // tokens
 constexpr int kSPad = 72;  // floats a row of partial scores
 constexpr int kPPad = 72;  // halves a row of P
 constexpr int kLatMaxBatch = 4096;
-constexpr float kPTop = 64.f;     // P of the reference maximum
-constexpr float kLatSlack = 8.f;  // log2 of what the true maximum may be past the reference: P <= 2^14
+constexpr float kPTop = 2048.f;   // P of the reference maximum
+constexpr float kLatSlack = 4.f;  // log2 of what the true maximum may be past the reference: P <= 2^15
 constexpr uint64_t kLatTimeoutNs = 2000000000ull;
 
 struct LatentParams {

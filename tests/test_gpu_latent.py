@@ -367,3 +367,27 @@ def test_an_infinite_latent_of_a_draft_stays_behind_the_mask():
     c[0, 1, 77] = float("inf")
     out = fs().latent_attention_cuda(q, qr, cache.append(c, r))
     assert torch.equal(out[0, 0], ref[0, 0]) and bool(out[0, 1].isnan().all())
+
+
+@pytest.mark.parametrize("h,near", [(16, 0), (16, 700), (64, 0)])
+def test_many_far_tokens_beside_a_near_one(h, near):
+    """One token takes nearly all of the weight and is zero in every dim but the first; the
+    other dims are what 1000 tokens at e^-17 (2^-24.5) of it add up to.  Requests enough that a
+    share holds the near token together with most of the others."""
+    b, n = 320, 1000
+    cache = make_cache([n] * b, 512, 64, 64, F, seed=60)
+    g = torch.Generator(device="cuda").manual_seed(61)
+    cache.values.copy_(torch.randint(40, 128, cache.values.shape, generator=g, device="cuda"))
+    cache.values[..., 0] = 0
+    cache.scale.fill_(1)
+    cache.ropes.zero_()
+    cache.ropes[..., 0] = -1
+    page, row = cache.block_table[:, near // 64], near % 64
+    cache.values[page, row] = 0
+    cache.values[page, row, 0] = 127
+    cache.ropes[page, row, 0] = 16
+    q, qr = queries(b, 1, h, 512, 64, F, seed=62)
+    q.zero_(), qr.zero_()
+    qr[..., 0] = 1
+    out = check(q, qr, cache, sm_scale=1.0)
+    assert float(out[..., 1:].min()) > 2e-3
