@@ -110,6 +110,12 @@ def _i64(t: torch.Tensor) -> torch.Tensor:
     return t if t.dtype == torch.int64 and t.is_contiguous() else t.to(torch.int64).contiguous()
 
 
+def _seq_cap(max_seq_len: int, page: int, cols: int) -> int:
+    """``max_seq_len`` for the library's 32-bit field: what does not fit (a caller's way to say
+    "no limit") becomes the end of the table, which no request passes."""
+    return max_seq_len if max_seq_len < 2 ** 31 else min(page * cols, 2 ** 31 - 1)
+
+
 def _run(entry: str, args: _lib.FsDecodeArgs, device: torch.device, splits_hint: int, xargs=None) -> int:
     """Plan (cached), workspace and launch of one decode call; ``xargs`` (FsExchangeArgs)
     selects fs_paged_decode_exchange and its own plan."""
@@ -186,7 +192,7 @@ def _decode_args(layout, q, kq, vq, out, lengths, table, num_blocks, max_seq_len
     a.block_size = int(kq.block_size)
     a.num_blocks = num_blocks
     a.table_cols = table.shape[1] if table is not None else 0
-    a.max_seq_len = max_seq_len
+    a.max_seq_len = max_seq_len if table is None else _seq_cap(max_seq_len, int(page_size), int(table.shape[1]))
     a.sm_scale = 1.0 / math.sqrt(float(q.shape[2]))
     a.device_status = status.data_ptr() if status is not None else None
     a.q_dtype = _lib.FS_BF16 if q.dtype == torch.bfloat16 else _lib.FS_F16

@@ -19,7 +19,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .attention import _check_weights, _i64
+from .attention import _check_weights, _i64, _seq_cap
 from .quant import device_guard, require_cuda, stream_of
 
 
@@ -85,7 +85,7 @@ def evict_tokens_cuda(cache, weights: torch.Tensor, budget: int, *, recent: int,
         a = _lib.FsEvictArgs()
         a.kv_format = _lib.FS_KV_SYMMETRIC if sym else _lib.FS_KV_AFFINE_BLOCK
         a.batch, a.kv_heads, a.head_dim, a.page_size = b, hkv, d, page
-        a.table_cols, a.max_seq_len = int(table.shape[1]), int(cache.max_seq_len)
+        a.table_cols, a.max_seq_len = int(table.shape[1]), _seq_cap(int(cache.max_seq_len), page, int(table.shape[1]))
         a.budget, a.recent, a.sinks = budget, recent, sinks
         a.num_pages = pages
         a.block_table, a.lengths = table.data_ptr(), lengths.data_ptr()

@@ -25,7 +25,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .attention import _i64
+from .attention import _i64, _seq_cap
 from .quant import device_guard, require_cuda, stream_of
 
 LATENT_DIMS = (128, 256, 512)
@@ -206,7 +206,8 @@ def latent_attention_cuda(q_latent: torch.Tensor, q_rope: torch.Tensor, cache: L
         a.q, a.q_rope, a.out = q.data_ptr(), qr.data_ptr(), out.data_ptr()
         a.dtype = _dtype(q)
         a.batch, a.tokens, a.heads, a.latent_dim, a.rope_dim = b, t, h, dc, dr
-        a.page_size, a.table_cols, a.max_seq_len = page, table.shape[1], int(cache.max_seq_len)
+        a.page_size, a.table_cols = page, table.shape[1]
+        a.max_seq_len = _seq_cap(int(cache.max_seq_len), page, table.shape[1])
         a.sm_scale = 1.0 / math.sqrt(dc + dr) if sm_scale is None else float(sm_scale)
         a.num_pages = pages
         a.values, a.scale, a.ropes = cache.values.data_ptr(), cache.scale.data_ptr(), cache.ropes.data_ptr()

@@ -424,3 +424,10 @@ def test_calls_on_several_host_threads():
     for a, _, (cache, wd, new, kept), codes in states:
         assert set(codes) == {0}, codes
         assert int(new) == a.budget and torch.equal(kept.cpu(), torch.arange(a.budget, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("longest", [2 ** 31, 2 ** 32, 2 ** 62])
+def test_no_limit_on_the_length(longest):
+    cache, w = make_cache(2, 64, [300, 20], 16, "affine", seed=14, extra_cols=1)
+    c = fs().PagedKVCache(cache.k_quant, cache.v_quant, cache.block_table, cache.lengths, 16, longest)
+    check(c, w, 100, 10, 2)

@@ -391,3 +391,12 @@ def test_many_far_tokens_beside_a_near_one(h, near):
     qr[..., 0] = 1
     out = check(q, qr, cache, sm_scale=1.0)
     assert float(out[..., 1:].min()) > 2e-3
+
+
+@pytest.mark.parametrize("longest", [2 ** 31, 2 ** 32, 2 ** 32 + 7, 2 ** 62])
+def test_no_limit_on_the_length(longest):
+    cache = make_cache([300, 77], 512, 64, 64, F, seed=70, extra_cols=1)
+    q, qr = queries(2, 1, 16, 512, 64, F, seed=71)
+    free = fs().LatentKVCache(cache.values, cache.scale, cache.ropes, cache.block_table, cache.lengths, longest)
+    assert torch.equal(check(q, qr, cache), fs().latent_attention_cuda(q, qr, free))
+    assert free.append(q[:, :, 0], qr[:, :, 0]).max_seq_len == 6 * 64

@@ -287,3 +287,13 @@ def test_refusals():
     with pytest.raises(ValueError):
         f(torch.zeros((1, 18, 128), dtype=torch.float16, device="cuda"), cache, ok)  # nine heads a kv head
     assert float(ok.abs().sum()) == 0.0
+
+
+@pytest.mark.parametrize("longest", [2 ** 31, 2 ** 32, 2 ** 62])
+@pytest.mark.parametrize("d", [128, 64])
+def test_no_limit_on_the_length(longest, d):
+    cache = make_cache(2, 2, d, [300, 45], 16, "affine", seed=21)
+    c = fs().PagedKVCache(cache.k_quant, cache.v_quant, cache.block_table, cache.lengths, 16, longest)
+    q = torch.randn((2, 4, d), generator=torch.Generator().manual_seed(13)).half().cuda()
+    out = check(q, c, torch.zeros((cache.k_quant.values.shape[0], 2, 16), device="cuda"))
+    assert torch.allclose(fs().paged_quant_attention_cuda(q, c).float(), out.float(), rtol=2e-3, atol=2e-3)

@@ -216,3 +216,12 @@ def test_evict_refuses_an_unaligned_workspace(offset, status):
     assert lib.fs_evict_workspace_size(C.byref(a), C.byref(n)) == 0 and n.value > 0
     a.workspace, a.workspace_bytes = 1 << 20 | offset, n.value
     assert lib.fs_evict_tokens(C.byref(a), None) == status
+
+
+def test_longest_length_beyond_32_bits():
+    """max_seq_len may say "no limit"; the C field has 32 bits and ctypes would drop the others."""
+    from flashspec_b200.attention import _seq_cap
+
+    assert [_seq_cap(n, 16, 10) for n in (0, 1000, 2 ** 31 - 1)] == [0, 1000, 2 ** 31 - 1]
+    assert [_seq_cap(n, 16, 10) for n in (2 ** 31, 2 ** 32, 2 ** 32 + 5, 2 ** 62)] == [160] * 4
+    assert _seq_cap(2 ** 40, 128, 2 ** 30) == 2 ** 31 - 1
