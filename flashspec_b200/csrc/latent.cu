@@ -497,8 +497,9 @@ __global__ void __launch_bounds__(LatentShape<kDC, kDR, kMT>::kThreads, LatentSh
 #pragma unroll
         for (int k = 0; k < 4; ++k) acc[i][j][k] = 0.f;
     float m_run = -1.0e30f, l_run = 0.f;
-    // tokens that this softmax thread's row sees: query t sees the first len - T + t + 1
-    const int limit = min(len, len - p.T + 1 + (row0 + srow) / p.H);
+    // tokens that this softmax thread's row sees: query t sees the first lengths - T + t + 1, as
+    // far as they are in the table
+    const int limit = (int)max((int64_t)0, min((int64_t)len, p.lengths[b] - p.T + 1 + (row0 + srow) / p.H));
 
     for (int t = t0; t < t1; ++t, ++used) {
       const int st = (int)(used % L::kStages);

@@ -400,3 +400,19 @@ def test_no_limit_on_the_length(longest):
     free = fs().LatentKVCache(cache.values, cache.scale, cache.ropes, cache.block_table, cache.lengths, longest)
     assert torch.equal(check(q, qr, cache), fs().latent_attention_cuda(q, qr, free))
     assert free.append(q[:, :, 0], qr[:, :, 0]).max_seq_len == 6 * 64
+
+
+def test_queries_of_a_request_that_has_outgrown_its_table():
+    """append keeps counting where the table ends; a query's own position still is the one that
+    its request's length gives it: of three at 62, 63 and 64, the first sees 63 tokens, the others
+    all 64."""
+    cache = make_cache([64, 64], 512, 64, 64, F, seed=80)
+    q, qr = queries(2, 3, 16, 512, 64, F, seed=81)
+    for whole, seen in ((64, (62, 63, 64)), (65, (63, 64, 64)), (66, (64, 64, 64)), (1000, (64, 64, 64))):
+        c = fs().LatentKVCache(cache.values, cache.scale, cache.ropes, cache.block_table,
+                               torch.tensor([whole, 64]).cuda(), 64)
+        out = fs().latent_attention_cuda(q, qr, c)
+        for k, n in enumerate(seen):
+            one = fs().LatentKVCache(c.values, c.scale, c.ropes, c.block_table, torch.tensor([n, 62 + k]).cuda(), 64)
+            want = fs().latent_attention_cuda(q[:, k: k + 1].contiguous(), qr[:, k: k + 1].contiguous(), one)
+            assert torch.allclose(out[:, k: k + 1].float(), want.float(), rtol=2 ** -10, atol=2 ** -10)
