@@ -20,7 +20,7 @@ import torch
 
 from . import _lib
 from .quant import (QuantizedTensor, SymQuantizedTensor, build_compression_stats, estimate_quantized_bytes,
-                    device_guard, require_cuda, stream_of)
+                    device_guard, require_cuda, status_word, stream_of)
 
 PAGE_TOKENS = 16  # tokens per kernel step (one page / quant block)
 NUM_WARPS = 4
@@ -194,7 +194,7 @@ def _decode_args(layout, q, kq, vq, out, lengths, table, num_blocks, max_seq_len
     a.table_cols = table.shape[1] if table is not None else 0
     a.max_seq_len = max_seq_len if table is None else _seq_cap(max_seq_len, int(page_size), int(table.shape[1]))
     a.sm_scale = 1.0 / math.sqrt(float(q.shape[2]))
-    a.device_status = status.data_ptr() if status is not None else None
+    a.device_status = status_word(status, q.device)
     a.q_dtype = _lib.FS_BF16 if q.dtype == torch.bfloat16 else _lib.FS_F16
     a.page_size = int(page_size)
     return a

@@ -20,7 +20,7 @@ import torch
 
 from . import _lib
 from .attention import _check_weights, _i64, _seq_cap
-from .quant import device_guard, require_cuda, stream_of
+from .quant import device_guard, require_cuda, status_word, stream_of
 
 
 def evict_tokens_cuda(cache, weights: torch.Tensor, budget: int, *, recent: int, sinks: int = 0,
@@ -95,7 +95,7 @@ def evict_tokens_cuda(cache, weights: torch.Tensor, budget: int, *, recent: int,
             a.k_zero, a.v_zero = kq.zero_point.data_ptr(), vq.zero_point.data_ptr()
         a.weights, a.weights_out = weights.data_ptr(), out.data_ptr()
         a.kept, a.new_lengths = kept.data_ptr(), new_lengths.data_ptr()
-        a.device_status = device_status.data_ptr() if device_status is not None else None
+        a.device_status = status_word(device_status, device)
         lib, need = _lib.load(), C.c_size_t(0)
         _lib.check(lib.fs_evict_workspace_size(C.byref(a), C.byref(need)), "fs_evict_tokens")
         ws = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None

@@ -26,7 +26,7 @@ import torch
 
 from . import _lib
 from .attention import _i64, _seq_cap
-from .quant import device_guard, require_cuda, stream_of
+from .quant import device_guard, require_cuda, status_word, stream_of
 
 LATENT_DIMS = (128, 256, 512)
 ROPE_DIMS = (32, 64)
@@ -133,7 +133,7 @@ class LatentKVCache:
             a.values, a.scale, a.ropes = self.values.data_ptr(), self.scale.data_ptr(), self.ropes.data_ptr()
             a.held = held.data_ptr() if held is not None else None
             a.new_lengths = new_lengths.data_ptr()
-            a.device_status = device_status.data_ptr() if device_status is not None else None
+            a.device_status = status_word(device_status, device)
             _lib.check(_lib.load().fs_latent_append(C.byref(a), stream_of(device)), "fs_latent_append")
         longest = min(int(self.max_seq_len) + t, page * table.shape[1])
         cache = LatentKVCache(self.values, self.scale, self.ropes, self.block_table, new_lengths, longest)
@@ -212,7 +212,7 @@ def latent_attention_cuda(q_latent: torch.Tensor, q_rope: torch.Tensor, cache: L
         a.num_pages = pages
         a.values, a.scale, a.ropes = cache.values.data_ptr(), cache.scale.data_ptr(), cache.ropes.data_ptr()
         a.block_table, a.lengths = table.data_ptr(), lengths.data_ptr()
-        a.device_status = device_status.data_ptr() if device_status is not None else None
+        a.device_status = status_word(device_status, device)
         lib, need = _lib.load(), C.c_size_t(0)
         _lib.check(lib.fs_latent_workspace_size(C.byref(a), C.byref(need)), "fs_latent_attention")
         ws = torch.empty(need.value, dtype=torch.uint8, device=device)
@@ -274,7 +274,7 @@ def latent_prefill_attention_cuda(q: torch.Tensor, kv: torch.Tensor, k_rope: tor
         a.dtype, a.batch, a.heads = _dtype(q), int(qo.shape[0]) - 1, h
         a.nope_dim, a.rope_dim, a.value_dim = dn, dr, dv
         a.sm_scale = 1.0 / math.sqrt(dq) if sm_scale is None else float(sm_scale)
-        a.device_status = device_status.data_ptr() if device_status is not None else None
+        a.device_status = status_word(device_status, device)
         _lib.check(_lib.load().fs_latent_prefill(C.byref(a), stream_of(device)), "fs_latent_prefill")
     return out
 

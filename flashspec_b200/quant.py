@@ -55,6 +55,18 @@ def device_guard(device: torch.device):
     return _CURRENT if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
+def status_word(t: Optional[torch.Tensor], device: torch.device) -> Optional[int]:
+    """Address of a caller's ``device_status`` (a kernel ORs a 32-bit word into its first
+    bytes), or None."""
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.device != device:
+        raise RuntimeError("device_status must be a tensor on the call's CUDA device")
+    if t.is_floating_point() or t.is_complex() or t.element_size() < 4 or t.numel() < 1:
+        raise ValueError("device_status must hold a 32-bit integer")
+    return t.data_ptr()
+
+
 def require_cuda(t: torch.Tensor, what: str) -> None:
     if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
         raise RuntimeError(f"{what} must be a CUDA tensor (flashspec_b200 has no CPU path)")

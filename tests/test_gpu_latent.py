@@ -416,3 +416,28 @@ def test_queries_of_a_request_that_has_outgrown_its_table():
             one = fs().LatentKVCache(c.values, c.scale, c.ropes, c.block_table, torch.tensor([n, 62 + k]).cuda(), 64)
             want = fs().latent_attention_cuda(q[:, k: k + 1].contiguous(), qr[:, k: k + 1].contiguous(), one)
             assert torch.allclose(out[:, k: k + 1].float(), want.float(), rtol=2 ** -10, atol=2 ** -10)
+
+
+def test_a_status_on_the_host_is_refused():
+    """By every operator that reports bad pages; refused before any launch."""
+    f, host = fs(), torch.zeros(1, dtype=torch.int32)
+    cache = make_cache([64], 512, 64, 64, F, seed=90)
+    q, qr = queries(1, 1, 4, 512, 64, F, seed=91)
+    x = torch.zeros((2, 1, 96), dtype=F, device="cuda")
+    o = torch.tensor([0, 2]).cuda()
+    kq = f.quantize_int8_per_block(torch.zeros((4, 1, 16, 128), device="cuda"), 16)
+    kv = f.PagedKVCache(kq, f.quantize_int8_per_block(torch.zeros((4, 1, 16, 128), device="cuda"), 16),
+                        torch.zeros((1, 1), dtype=torch.int64, device="cuda"), torch.ones(1).long().cuda(), 16, 16)
+    w, q1 = torch.zeros((4, 1, 16), device="cuda"), torch.zeros((1, 1, 128), dtype=F, device="cuda")
+    for call in (lambda s: f.latent_attention_cuda(q, qr, cache, device_status=s),
+                 lambda s: cache.append(q[:, :, 0], qr[:, :, 0], device_status=s),
+                 lambda s: f.latent_prefill_attention_cuda(x, torch.zeros((2, 1, 128), dtype=F, device="cuda"),
+                                                           x[:, 0, :32], o, o, device_status=s),
+                 lambda s: f.evict_tokens_cuda(kv, w, 4, recent=1, device_status=s),
+                 lambda s: f.paged_quant_attention_weights_cuda(q1, kv, w, device_status=s),
+                 lambda s: f.paged_quant_attention_cuda(q1, kv, device_status=s)):
+        with pytest.raises(RuntimeError):
+            call(host)
+        with pytest.raises(ValueError):
+            call(torch.zeros(4, dtype=torch.uint8, device="cuda"))
+        call(torch.zeros(1, dtype=torch.int32, device="cuda"))

@@ -225,3 +225,22 @@ def test_longest_length_beyond_32_bits():
     assert [_seq_cap(n, 16, 10) for n in (0, 1000, 2 ** 31 - 1)] == [0, 1000, 2 ** 31 - 1]
     assert [_seq_cap(n, 16, 10) for n in (2 ** 31, 2 ** 32, 2 ** 32 + 5, 2 ** 62)] == [160] * 4
     assert _seq_cap(2 ** 40, 128, 2 ** 30) == 2 ** 31 - 1
+
+
+def test_status_word():
+    """The kernels write to it, so a host address or a short element must not get there."""
+    import torch
+    from flashspec_b200.quant import status_word
+
+    cpu, gpu = torch.device("cpu"), torch.device("cuda", 0)
+    assert status_word(None, gpu) is None
+    for dtype in (torch.int32, torch.int64, torch.uint32):
+        t = torch.zeros(2, dtype=dtype)
+        assert status_word(t, cpu) == t.data_ptr()
+        with pytest.raises(RuntimeError):
+            status_word(t, gpu)
+    for bad in (torch.zeros(4, dtype=torch.int8), torch.zeros(1), torch.zeros(0, dtype=torch.int32)):
+        with pytest.raises(ValueError):
+            status_word(bad, cpu)
+    with pytest.raises(RuntimeError):
+        status_word(0, cpu)
