@@ -556,7 +556,13 @@ __global__ void __launch_bounds__(LatentShape<kDC, kDR, kMT>::kThreads, LatentSh
         s_lam[tid] = fmaxf(lg2_approx(fmaxf(sc, 0.f)), -100.f);
       }
       if (__syncthreads_or(here ? 0 : 1)) {  // a copy that never came: give up, outputs are invalid
-        if (tid == 0 && p.status != nullptr) atomicOr(p.status, FS_DEV_TIMEOUT);
+        if (tid == 0) {
+          if (p.status != nullptr) atomicOr(p.status, FS_DEV_TIMEOUT);
+          // shared memory is given back only behind the copies still on their way to it
+          for (uint32_t i = used; i != issued; ++i)
+            mbar_wait_bounded(smem_u32(&s_full[i % L::kStages]), (i / L::kStages) & 1u, kLatTimeoutNs);
+        }
+        __syncthreads();
         return;
       }
       // every warp is done with tile t - 1: its stage takes tile t + L::kStages - 1

@@ -244,3 +244,39 @@ def test_status_word():
             status_word(bad, cpu)
     with pytest.raises(RuntimeError):
         status_word(0, cpu)
+
+
+class Ring:
+    """mbarriers of a ring of stages, as the hardware counts them: one completion a tile, in any
+    order over the stages; wait(parity) passes when the phase of that parity has completed."""
+
+    def __init__(self, stages):
+        self.stages, self.done = stages, [0] * stages
+
+    def complete(self, tile):
+        assert self.done[tile % self.stages] == tile // self.stages  # in turn on one stage
+        self.done[tile % self.stages] += 1
+
+    def passes(self, tile):
+        return (self.done[tile % self.stages] & 1) != ((tile // self.stages) & 1)
+
+
+@pytest.mark.parametrize("stages", [2, 3])
+def test_giving_up_waits_for_the_copies_in_flight(stages):
+    """The latent attention gives up at tile `used` with tiles [used, issued) on their way (fewer
+    than the stages): its last waits pass for each of them when it has come, and not before."""
+    for used in range(4 * stages):
+        for ahead in range(1, stages):
+            for missing in range(used, used + ahead):
+                ring = Ring(stages)
+                for tile in range(used + ahead):
+                    if tile != missing:
+                        ring.complete(tile)
+                for tile in range(used, used + ahead):
+                    assert ring.passes(tile) == (tile != missing)
+                ring.complete(missing)
+                assert all(ring.passes(tile) for tile in range(used, used + ahead))
+    src = (HEADER.parents[1] / "flashspec_b200" / "csrc" / "latent.cu").read_text()
+    end = src[src.index("if (__syncthreads_or(here ? 0 : 1))"):]
+    end = end[:end.index("return;")]
+    assert "i = used; i != issued" in end and end.count("mbar_wait_bounded") == 1
