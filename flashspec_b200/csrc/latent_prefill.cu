@@ -83,7 +83,7 @@ struct PrefillShape {
 };
 
 struct PreBars {
-  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], pv_done[2];
+  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], pv_done[2], drained;
 };
 
 template <bool kBf16>
@@ -241,6 +241,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
   }
   if (tid == 32) {
     mbar_init(smem_u32(&bars.q_full), 1);
+    mbar_init(smem_u32(&bars.drained), 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&bars.k_full[i]), 1);
       mbar_init(smem_u32(&bars.k_empty[i]), 1);
@@ -277,6 +278,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
     return last > 0 ? (last + kPreK - 1) / kPreK : 0;
   };
   const int n0 = tiles_of(0), n1 = tiles_of(1), tiles = max(n0, n1);
+  int k_sent = 0, v_sent = 0;  // of the TMA thread: tiles whose copies were issued
 
   if (warp == 0) {
     // ================================ TMA ==================================
@@ -299,11 +301,13 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         const int x = h * (kDN + kDV);
         if (j >= 2 && !pre_wait(&bars.k_empty[st], ph, &s_abort)) break;
         mbar_arrive_expect_tx(smem_u32(&bars.k_full[st]), L::kQKChunks * kChunk);
+        k_sent = j + 1;
         const uint32_t kb = smem + L::kK + st * L::kQKChunks * kChunk;
         for (int c = 0; c < kDN / 64; ++c) load(kb + c * kChunk, &map_kv, x + 64 * c, y, &bars.k_full[st]);
         load(kb + (kDN / 64) * kChunk, &map_r, 0, y, &bars.k_full[st]);
         if (j >= 2 && !pre_wait(&bars.v_empty[st], ph, &s_abort)) break;
         mbar_arrive_expect_tx(smem_u32(&bars.v_full[st]), L::kVChunks * kChunk);
+        v_sent = j + 1;
         const uint32_t vb = smem + L::kV + st * L::kVChunks * kChunk;
         for (int c = 0; c < L::kVChunks; ++c) load(vb + c * kChunk, &map_kv, x + kDN + 64 * c, y, &bars.v_full[st]);
       }
@@ -517,6 +521,20 @@ __global__ void __launch_bounds__(kPreThreads, 1)
     tcgen05_fence_before();
   }
   __syncthreads();
+  if (s_abort != 0) {  // a wait gave up: memory is given back behind the copies and MMAs in flight
+    if (warp == 0 && lane == 0 && tiles > 0) {
+      mbar_wait_bounded(smem_u32(&bars.q_full), 0, kPreTimeoutNs);
+      for (int j = max(0, k_sent - 2); j < k_sent; ++j)
+        mbar_wait_bounded(smem_u32(&bars.k_full[j & 1]), (j >> 1) & 1, kPreTimeoutNs);
+      for (int j = max(0, v_sent - 2); j < v_sent; ++j)
+        mbar_wait_bounded(smem_u32(&bars.v_full[j & 1]), (j >> 1) & 1, kPreTimeoutNs);
+    }
+    if (warp == 1 && lane == 0) {  // the thread that issued the MMAs
+      mma_commit(smem_u32(&bars.drained));
+      mbar_wait_bounded(smem_u32(&bars.drained), 0, kPreTimeoutNs);
+    }
+    __syncthreads();
+  }
   if (warp == 2) {
     tcgen05_fence_after();
     tmem_dealloc(tmem, L::kTmemCols);

@@ -280,3 +280,21 @@ def test_giving_up_waits_for_the_copies_in_flight(stages):
     end = src[src.index("if (__syncthreads_or(here ? 0 : 1))"):]
     end = end[:end.index("return;")]
     assert "i = used; i != issued" in end and end.count("mbar_wait_bounded") == 1
+
+
+def test_giving_up_in_a_prompt_waits_for_the_copies_in_flight():
+    """The expanded attention keeps two K and two V tiles in flight at most: a tile is sent when the
+    one two before it was consumed, so the last two sent are all that may be on their way."""
+    for sent in range(1, 12):
+        for arrived in range(max(0, sent - 2), sent + 1):
+            ring = Ring(2)
+            for tile in range(arrived):
+                ring.complete(tile)
+            waits = range(max(0, sent - 2), sent)
+            assert [ring.passes(t) for t in waits] == [t < arrived for t in waits]
+            for tile in range(arrived, sent):
+                ring.complete(tile)
+            assert all(ring.passes(t) for t in waits)
+    src = (HEADER.parents[1] / "flashspec_b200" / "csrc" / "latent_prefill.cu").read_text()
+    end = src[src.index("if (s_abort != 0) {"):src.index("tmem_dealloc(tmem")]
+    assert all(x in end for x in ("bars.q_full", "bars.k_full", "bars.v_full", "mma_commit(smem_u32(&bars.drained))"))
