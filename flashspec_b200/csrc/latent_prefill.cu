@@ -334,7 +334,8 @@ __global__ void __launch_bounds__(kPreThreads, 1)
       if (ok) {
         if (n0 > 0) scores(0, 0);
         if (n1 > 0) scores(1, 0);
-        mma_commit(smem_u32(&bars.k_empty[0]));
+        // a stage is reported free only to a later tile: no arrival is under way when the CTA ends
+        if (tiles > 2) mma_commit(smem_u32(&bars.k_empty[0]));
       }
       for (int j = 0; j < tiles && ok; ++j) {
         const int st = j & 1;
@@ -354,8 +355,8 @@ __global__ void __launch_bounds__(kPreThreads, 1)
           if (j + 1 == n) mma_commit(smem_u32(&bars.pv_done[g]));
           if (j + 1 < n) scores(g, j + 1);  // over the P that was just read
         }
-        mma_commit(smem_u32(&bars.v_empty[st]));
-        mma_commit(smem_u32(&bars.k_empty[st ^ 1]));
+        if (j + 2 < tiles) mma_commit(smem_u32(&bars.v_empty[st]));
+        if (j + 3 < tiles) mma_commit(smem_u32(&bars.k_empty[st ^ 1]));  // of tile j + 1
       }
     }
   } else if (warp >= 4) {

@@ -298,3 +298,20 @@ def test_giving_up_in_a_prompt_waits_for_the_copies_in_flight():
     src = (HEADER.parents[1] / "flashspec_b200" / "csrc" / "latent_prefill.cu").read_text()
     end = src[src.index("if (s_abort != 0) {"):src.index("tmem_dealloc(tmem")]
     assert all(x in end for x in ("bars.q_full", "bars.k_full", "bars.v_full", "mma_commit(smem_u32(&bars.drained))"))
+
+
+def test_every_arrival_of_a_prompt_is_waited_for():
+    """The commits that free the stages of the expanded attention, against the waits for them: K of
+    tile i is free behind the scores of tile i, V behind its P V, and both are waited for by the
+    copies of tile i + 2 alone.  An arrival that nobody waits for could reach a CTA that has ended."""
+    src = (HEADER.parents[1] / "flashspec_b200" / "csrc" / "latent_prefill.cu").read_text()
+    for line in ("if (tiles > 2) mma_commit(smem_u32(&bars.k_empty[0]))",
+                 "if (j + 2 < tiles) mma_commit(smem_u32(&bars.v_empty[st]))",
+                 "if (j + 3 < tiles) mma_commit(smem_u32(&bars.k_empty[st ^ 1]))",
+                 "if (j >= 2 && !pre_wait(&bars.k_empty[st]", "if (j >= 2 && !pre_wait(&bars.v_empty[st]"):
+        assert src.count(line) == 1, line
+    assert src.count("mma_commit(smem_u32(&bars.k_empty") == 2 and src.count("mma_commit(smem_u32(&bars.v_empty") == 1
+    for tiles in range(1, 12):
+        k_free = ([0] if tiles > 2 else []) + [j + 1 for j in range(tiles) if j + 3 < tiles]
+        v_free = [j for j in range(tiles) if j + 2 < tiles]
+        assert k_free == v_free == [j - 2 for j in range(2, tiles)]
