@@ -145,10 +145,15 @@ int fs_paged_decode_noalloc(const FsDecodeArgs* args, void* stream);
  * for every live token, weights fp32 [num_blocks (pages), Hkv, page] beside the pool (the
  * measure fs_evict_tokens keeps tokens by).  No page window, no shard outputs.  The
  * workspace (256-byte aligned; the size comes from fs_paged_decode_weights_workspace_size)
- * also holds the scores, 4 bytes a query head and token.  Weights are off by at most about
- * 1e-6 of themselves (24-bit fixed-point q in the tuned kernels).  A page of one request
- * gets one addition a call; pages shared by requests add up too, in varying order.
- * Requests up to 65535 * 1024 tokens.  No counterpart in the reference. */
+ * also holds the scores.  A weight 2^(x - LSE), x the score in the log2 domain, has the
+ * relative error of its 32-bit exponent: with u = 2^-24 about ln 2 times
+ *   8 u (sizes of the sums of sm_scale log2(e) q k that x comes out of)   tuned kernels, and
+ *   2^-24 max|q| sum|k| sm_scale log2(e)   from q's 24-bit fixed point; or
+ *   head_dim u (sum |q k| sm_scale log2(e))   generic kernel,
+ * plus 4 u |x| + 8 u |LSE| and 2^-21 + (tokens / 16) u of the sums and exponentials: 1e-6 to
+ * 1e-5 for scores of ordinary size, growing with it.  A page of one request gets one addition
+ * a call; pages shared by requests add up too, in varying order.  Requests up to 65535 * 1024
+ * tokens.  No counterpart in the reference. */
 int fs_paged_decode_weights_workspace_size(const FsDecodeArgs* args, size_t* bytes, int32_t* splits);
 int fs_paged_decode_weights(const FsDecodeArgs* args, float* weights, void* stream);
 

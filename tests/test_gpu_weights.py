@@ -297,3 +297,61 @@ def test_no_limit_on_the_length(longest, d):
     q = torch.randn((2, 4, d), generator=torch.Generator().manual_seed(13)).half().cuda()
     out = check(q, c, torch.zeros((cache.k_quant.values.shape[0], 2, 16), device="cuda"))
     assert torch.allclose(fs().paged_quant_attention_cuda(q, c).float(), out.float(), rtol=2e-3, atol=2e-3)
+
+
+@pytest.mark.parametrize("size", [1.0, 6.0])
+@pytest.mark.parametrize("b,hq,hkv,d,page,lens,fmt,dtype", [
+    (2, 8, 2, 128, 16, [3000, 77], "affine", torch.float16),
+    (2, 8, 2, 128, 16, [3000, 77], "symmetric", torch.float16),
+    (40, 16, 16, 128, 16, [100 + 13 * i for i in range(40)], "affine", torch.float16),  # the balanced kernel
+    (2, 8, 2, 64, 16, [900, 37], "affine", torch.bfloat16),
+    (2, 4, 2, 256, 32, [700, 33], "symmetric", torch.bfloat16),
+    (1, 5, 1, 64, 6, [77], "affine", torch.float16)])
+def test_every_weight_is_precise_in_itself(b, hq, hkv, d, page, lens, fmt, dtype, size):
+    """What a call adds to a token, light ones included, against 64 bits and relative to itself.
+
+    With x a score in the log2 domain and u = 2^-24: x comes out of sums of terms that cancel, so its
+    error is u times their size M = sm_scale log2(e) scale (sum |q c| + |offset| |sum q|) a few times
+    over (8: conversions to fp32 and the join of the three byte sums), or D times in the generic
+    kernel's chain of FMAs (without an offset); four roundings of x itself; and in the tuned kernels
+    q's 24-bit fixed point, max|q| / 8355000 / 2 against sum |k|.  The LSE's error is at most that
+    of the worst score, four roundings of itself and of the sum (n / 16 u); exp2 adds 2^-22 on either
+    side.  ln 2 turns an error of the exponent into one of the weight; a weight below 2^-126 may be
+    flushed."""
+    u, ln2 = 2.0 ** -24, float(np.log(2))
+    cache = make_cache(b, hkv, d, lens, page, fmt, seed=200 + d + page)
+    q = (torch.randn((b, hq, d), generator=torch.Generator().manual_seed(14)) * size).to(dtype).cuda()
+    pages = cache.k_quant.values.shape[0]
+    w = torch.zeros((pages, hkv, page), device="cuda")
+    fs().paged_quant_attention_weights_cuda(q, cache, w)
+    tuned = d == 128 and page == 16 and dtype == torch.float16
+    kq, table = cache.k_quant, cache.block_table
+    worst = 0.0
+    for i, n in enumerate(lens):
+        at = table[i, : (n + page - 1) // page]
+        if fmt == "symmetric":
+            c, sc, off = kq.values[at].double(), kq.scale[at].double()[..., None], 0.0
+        else:
+            c = kq.values[at].double()[:, :, 0]
+            sc = kq.scale[at].double()[:, :, 0]
+            off = 128 - kq.zero_point[at].double()[:, :, 0]
+        flat = lambda t: t.expand(len(at), hkv, page, t.shape[-1]).transpose(0, 1).flatten(1, 2)[:, :n]  # noqa: E731
+        k = flat((c + off) * sc)
+        qd = q[i].double().view(hkv, -1, d)
+        x = torch.einsum("hgd,hnd->hgn", qd, k) * d ** -0.5 / ln2
+        lse = torch.logsumexp(x * ln2, -1, keepdim=True) / ln2
+        if tuned:
+            m = torch.einsum("hgd,hnd->hgn", qd.abs(), flat(c.abs() * sc))
+            if fmt == "affine":
+                m = m + qd.sum(-1).abs()[..., None] * flat((off * sc).abs()).squeeze(-1)[:, None]
+            e = 8 * u * m * d ** -0.5 / ln2
+            e = e + qd.abs().amax(-1)[..., None] / 8355000 / 2 * k.abs().sum(-1)[:, None] * d ** -0.5 / ln2
+        else:
+            e = d * u * torch.einsum("hgd,hnd->hgn", qd.abs(), k.abs()) * d ** -0.5 / ln2
+        e = e + 4 * u * x.abs()
+        p = torch.exp2(x - lse)
+        rel = ln2 * (e + e.amax(-1, keepdim=True) + 8 * u * lse.abs()) + 2.0 ** -21 + n / 16 * u
+        got = w[at].double().transpose(0, 1).flatten(1)[:, :n]
+        err, bound = (got - p.sum(1)).abs(), (p * rel).sum(1) + 2.0 ** -126
+        worst = max(worst, float((err / bound).max()))
+    assert worst <= 1, worst
