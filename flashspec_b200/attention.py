@@ -351,7 +351,9 @@ def paged_quant_attention_weights_cuda(q: torch.Tensor, cache, weights: torch.Te
     are).  ``evict_tokens_cuda`` keeps the tokens with the largest sums.  A page of one
     request gets exactly one addition a call, so its sums are reproducible; pages that
     requests share add up as well, in varying order.  The scores take a workspace of 4 bytes
-    a query head and token."""
+    a query head and token of ``cache.max_seq_len``, for every request however short: with
+    one long request among many, calls of requests of like length need less.  No page windows:
+    a sequence-sharded decode cannot track weights."""
     hkv, _ = _validate_paged(q, cache)
     num_pages, page = int(cache.k_quant.values.shape[0]), int(cache.block_size)
     _check_weights(weights, (num_pages, hkv, page), q.device, "weights")

@@ -145,7 +145,9 @@ int fs_paged_decode_noalloc(const FsDecodeArgs* args, void* stream);
  * for every live token, weights fp32 [num_blocks (pages), Hkv, page] beside the pool (the
  * measure fs_evict_tokens keeps tokens by).  No page window, no shard outputs.  The
  * workspace (256-byte aligned; the size comes from fs_paged_decode_weights_workspace_size)
- * also holds the scores.  A weight 2^(x - LSE), x the score in the log2 domain, has the
+ * also holds the scores: 4 bytes a query head and token of max_seq_len (at most the table's
+ * end), for every request however short, so 2.1 GB for 64 requests of 64 heads when one may
+ * have 131072 tokens.  A weight 2^(x - LSE), x the score in the log2 domain, has the
  * relative error of its 32-bit exponent: with u = 2^-24 about ln 2 times
  *   8 u (sizes of the sums of sm_scale log2(e) q k that x comes out of)   tuned kernels, and
  *   2^-24 max|q| sum|k| sm_scale log2(e)   from q's 24-bit fixed point; or
