@@ -35,8 +35,8 @@ LATENT_PAGES = (16, 32, 64, 128)
 
 @dataclass(frozen=True)
 class LatentKVCache:
-    """Paged latent cache: ``values`` int8 [P, page, dc], ``scale`` fp32 [P, page], ``ropes``
-    fp16 / bf16 [P, page, dr], ``block_table`` int64 [B, cols] (-1 = unallocated),
+    """Paged latent cache: ``values`` int8 [P, page, dc], ``scale`` fp32 [P, page] (not
+    negative), ``ropes`` fp16 / bf16 [P, page, dr], ``block_table`` int64 [B, cols] (-1 = unallocated),
     ``lengths`` int64 [B], ``max_seq_len`` no less than any length.  dc 128, 256 or 512, dr 32
     or 64, page 16, 32, 64 or 128."""
 
@@ -179,7 +179,9 @@ def latent_attention_cuda(q_latent: torch.Tensor, q_rope: torch.Tensor, cache: L
     in the cache already): query t sees the first lengths - T + t + 1 tokens, one that sees
     none gives zeros.  Returns sum_j softmax_j(sm_scale (q_latent . c_j + q_rope . r_j)) c_j
     like q_latent.  sm_scale defaults to 1 / sqrt(dc + dr); a model's own is that of its
-    expanded heads, 1 / sqrt(nope + rope)."""
+    expanded heads, 1 / sqrt(nope + rope).  q_latent takes part as 16-bit fixed point of its
+    row (max|q| / 65278 off at most): a dim of q that is hundreds of times the others, over
+    latents that are as much smaller, is better moved into the latents before they are stored."""
     _check_cache(cache)
     single = q_latent.ndim == 3
     if single and q_rope.ndim == 3:

@@ -238,9 +238,13 @@ int fs_latent_append(const FsLatentAppendArgs* args, void* stream);
  *   out[b, t, h]   = sum_j softmax_j(score) scale_j values_j
  * over the tokens j < lengths[b] - tokens + t + 1 (query t is the token at that end; none:
  * zeros).  q and out [batch, tokens, heads, latent_dim], q_rope [batch, tokens, heads,
- * rope_dim], contiguous, 16-byte aligned.  Unallocated pages are skipped.  At most 4096
- * requests, 2^20 rows (tokens * heads) and 2^30 positions a request, 2^31 tokens a pool.  Workspace: fs_latent_workspace_size
- * bytes, 256-byte aligned, any contents. */
+ * rope_dim], contiguous, 16-byte aligned.  Unallocated pages are skipped, and so are tokens of
+ * negative scale.  q (not q_rope) takes part as 16-bit fixed point of its row: a score is off by
+ * at most sm_scale max|q| / 65278 sum|scale values|.  That is below the rounding of the output
+ * for rows of like-sized dims, 1e-3 of the output with one dim of 100 times the others and up to
+ * 1e-2 with one of 1000 times whose latents are as much smaller.  At most 4096
+ * requests, 2^20 rows (tokens * heads) and 2^30 positions a request, 2^31 tokens a pool.
+ * Workspace: fs_latent_workspace_size bytes, 256-byte aligned, any contents. */
 typedef struct FsLatentArgs {
   const void* q;
   const void* q_rope;

@@ -441,3 +441,18 @@ def test_a_status_on_the_host_is_refused():
         with pytest.raises(ValueError):
             call(torch.zeros(4, dtype=torch.uint8, device="cuda"))
         call(torch.zeros(1, dtype=torch.int32, device="cuda"))
+
+
+@pytest.mark.parametrize("large,share", [(100.0, 2e-3), (1000.0, 2e-2)])
+def test_one_large_dim_in_q(large, share):
+    """What the 16-bit fixed point of a row's queries costs when one dim is far above the others
+    and its latents as far below: within the bound of every case, and within the stated share of
+    the largest output."""
+    cache = make_cache([500, 90], 512, 64, 64, F, seed=100)
+    cache.scale.fill_(1 / 73)  # latents of size 1
+    cache.values[..., 5] = (cache.values[..., 5].float() / large).round().to(torch.int8)
+    q, qr = queries(2, 1, 16, 512, 64, F, seed=101)
+    q[..., 5] *= large
+    want, _ = expect(q, qr, cache, 576 ** -0.5)
+    out = check(q, qr, cache)
+    assert float((out.double() - want).abs().max() / want.abs().max()) < share
