@@ -431,3 +431,19 @@ def test_no_limit_on_the_length(longest):
     cache, w = make_cache(2, 64, [300, 20], 16, "affine", seed=14, extra_cols=1)
     c = fs().PagedKVCache(cache.k_quant, cache.v_quant, cache.block_table, cache.lengths, 16, longest)
     check(c, w, 100, 10, 2)
+
+
+@pytest.mark.parametrize("fmt", ["affine", "symmetric"])
+@pytest.mark.parametrize("d,page", [(128, 16), (64, 16), (128, 64)])
+def test_many_rows_move_in_rounds(fmt, d, page):
+    """Rows enough that one CTA of four warps takes each, over several rounds of its pages."""
+    lens = [150 + 7 * (i % 30) for i in range(75)]
+    cache, w = make_cache(4, d, lens, page, fmt, seed=15)
+    check(cache, w, 210, 20, 4)
+
+
+@pytest.mark.parametrize("fmt", ["affine", "symmetric"])
+@pytest.mark.parametrize("d,page", [(128, 16), (256, 32)])
+def test_a_long_row_moves_in_rounds_of_a_cluster(fmt, d, page):
+    cache, w = make_cache(1, d, [9000], page, fmt, seed=16)
+    check(cache, w, 6000, 500, 16)
