@@ -334,6 +334,9 @@ struct QueryFrag {
 // of score + log2(V scale): P = 2^(t - m_run) * scale * 2^14 uses fp16's range from the top
 // whatever the scale, while l_run keeps sum 2^(t - m_run) in fp32 (at most 2^100 a token).
 constexpr float kWtsTop = 16384.f;
+// log2 of a V scale as far as it enters the running maximum: bounded, so that l_run, and with it
+// every weight, stays finite beside a scale of zero or infinity.
+__device__ __forceinline__ float scale_log2(float s) { return fminf(fmaxf(lg2_approx(s), -100.f), 100.f); }
 constexpr int kLo2Bytes = 1024;  // third bytes of a warp's query fragment
 
 struct WarpState {
@@ -483,9 +486,9 @@ __device__ __forceinline__ void consume_page(uint32_t sbase, const StageOffsets&
     if (si.tok != 0u) {
       mx = -INFINITY;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) mx = fmaxf(mx, t[k] + fmaxf(lg2_approx(vk[k]), -100.f));
+      for (int k = 0; k < 4; ++k) mx = fmaxf(mx, t[k] + scale_log2(vk[k]));
     } else {
-      mx += fmaxf(lg2_approx(si.vs), -100.f);
+      mx += scale_log2(si.vs);
     }
   }
   mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));

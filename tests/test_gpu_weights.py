@@ -355,3 +355,23 @@ def test_every_weight_is_precise_in_itself(b, hq, hkv, d, page, lens, fmt, dtype
         err, bound = (got - p.sum(1)).abs(), (p * rel).sum(1) + 2.0 ** -126
         worst = max(worst, float((err / bound).max()))
     assert worst <= 1, worst
+
+
+@pytest.mark.parametrize("fmt", ["affine", "symmetric"])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan"), 0.0])
+def test_weights_do_not_depend_on_v(fmt, bad):
+    """A live token of V whose scale is infinite, undefined or zero: the output shows it, the weights
+    are those of the scores.  Beside an infinite scale the reference lies 2^100 up, so tokens 2^-26
+    below the heaviest no longer count towards the LSE (200 of them: 3e-6)."""
+    cache = make_cache(2, 2, 128, [200, 39], 16, fmt, seed=22)
+    q = torch.randn((2, 4, 128), generator=torch.Generator().manual_seed(15)).half().cuda()
+    runs = []
+    for scale in (None, bad):
+        if scale is not None:
+            s = cache.v_quant.scale.view(cache.v_quant.scale.shape[0], 2, -1)
+            s[cache.block_table[0, 3], :, 0] = scale
+        w = torch.zeros((cache.k_quant.values.shape[0], 2, 16), device="cuda")
+        runs.append((fs().paged_quant_attention_weights_cuda(q, cache, w), w))
+    assert torch.allclose(runs[1][1], runs[0][1], rtol=2e-5, atol=0)
+    assert torch.equal(runs[1][0][1], runs[0][0][1])
+    assert bool(runs[1][0][0].isfinite().all()) == (bad == 0.0)
