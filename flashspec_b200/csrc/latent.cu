@@ -732,7 +732,7 @@ constexpr int kMergeChunk = 128;
 __global__ void __launch_bounds__(128) latent_merge_kernel(const LatentParams p, int block_rows, int dc, int ctas) {
   __shared__ float s_w[kMergeChunk];
   __shared__ float s_max[4];
-  cudaGridDependencySynchronize();  // launched early: the shares' results are there now
+  cudaGridDependencySynchronize();  // behind it the shares' results are there
   const int row = blockIdx.x % p.R, b = blockIdx.x / p.R, rb = row / block_rows, r = row - rb * block_rows;
   const int tid = threadIdx.x, threads = blockDim.x;
   const int before = p.prefix[b], units = p.prefix[b + 1] - before, total = p.prefix[p.B] * p.row_blocks;
@@ -856,7 +856,8 @@ static int launch_latent(const FsLatentArgs* a, const LatentParams& p, const Lat
     return fail_cuda("shared-memory limit of the latent attention kernel", e);
   kernel<<<pl.ctas, L::kThreads, L::smem(p.B), reinterpret_cast<cudaStream_t>(stream)>>>(map_v, map_r, p);
   if (int st = launch_status("latent attention kernel launch"); st != FS_OK) return st;
-  // the merge is launched while the shares still run and waits for them on the device
+  // the merge may be set up before the shares have ended; nothing triggers it earlier, so this
+  // hides its launch latency and no more
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
