@@ -21,7 +21,7 @@
 //
 // Memory traffic is the floor: 4 bytes of weights for every live token, then 2 (D + a scale)
 // bytes read and written for every kept one.  Measured: 64 requests of up to 8192 tokens and 8
-// heads cut to 1000 (floor 38 us): selection 38 us, affine move 148 us, 84 M warp
+// heads cut to 1000 (floor 38 us): selection 38 us, affine move 148 us, 83 M warp
 // instructions; 2 x 131072 tokens cut to 16384 (floor 23 us): selection 51 us,
 // symmetric move 54 us, in clusters of 8 CTAs for each of the 16 rows, one or two CTAs an SM.
 #include <cooperative_groups.h>

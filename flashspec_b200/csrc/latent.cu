@@ -25,7 +25,7 @@
 // A share that holds a whole (request, row block) writes the output; others leave normalised
 // (O, LSE) partials that latent_merge_kernel joins.
 // Measured: 64 ragged requests (8192 -> 128 tokens) x 16 rows 61.5 us (2.8 TB/s; the memory
-// floor is 26.6), 16 requests (8192 -> 4096) x 128 rows 129 us (212 TFLOP/s; warp-level MMAs
+// floor is 26.6), 16 requests (8192 -> 4096) x 128 rows 131 us (209 TFLOP/s; warp-level MMAs
 // end at a measured 557); both issue in under half of the cycles, at 16 and 8 warps an SM.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -7,7 +7,7 @@
 //
 // A CTA takes 256 queries of one head, as two blocks of 128, and walks the keys in tiles of
 // 96, so that two K and two V tiles fit beside the queries.  Four packed prompts (4096 -> 500
-// tokens, 16 heads) take 201 us, 722 TFLOP/s of useful work.  Measured and dropped: 128 queries
+// tokens, 16 heads) take 198 us, 732 TFLOP/s of useful work.  Measured and dropped: 128 queries
 // a CTA (220 us), an O each for even and odd tiles (230), 128 keys a tile with P over S (222),
 // 80 keys with P beside S (244).  Spinning in place of sleeping waits cost 5% of the kernel.
 // The MMA thread takes its descriptors from precomputed words: building them bound it.  Roles:

@@ -7,8 +7,8 @@
 // scores make one round trip (4 bytes a query and token, against the 256 of a token's K
 // and V) instead of K being read and multiplied again (128 bytes).
 //
-// Bound by memory: 4 G bytes of scores and 8 of weights a token (15 us for 64 ragged requests
-// of 32 / 8 heads, 18 us for 2 x 131072 tokens of 64 / 8 heads, under a profiler with cold
+// Bound by memory: 4 G bytes of scores and 8 of weights a token (14 us for 64 ragged requests
+// of 32 / 8 heads, 16 us for 2 x 131072 tokens of 64 / 8 heads, under a profiler with cold
 // caches; the decodes before them take 141 and 121).  A lane takes four tokens
 // of one request and walks the kv head's queries, so a warp reads 512 consecutive bytes a
 // query.  Sums go out as reductions: pages shared by requests add up correctly (their order
