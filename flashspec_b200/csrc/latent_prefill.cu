@@ -58,9 +58,6 @@ struct PreRange {
   static constexpr float kSlack = kBf16 ? 8.f : 4.f, kLift = kBf16 ? 0.f : 11.f;
 };
 constexpr uint64_t kPreTimeoutNs = 2000000000ull;
-// Every CTA looks through the batch's offsets (pre_find), so the work grows with the square of the
-// batch: at this limit it is tens of milliseconds, at 2^20 requests it would be minutes.
-constexpr int kPreMaxBatch = 4096;
 
 struct PrefillParams {
   const uint16_t* kv;    // [Nk, H, dn + dv]
@@ -603,8 +600,7 @@ extern "C" int fs_latent_prefill(const FsLatentPrefillArgs* a, void* stream) {
   if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->kv) | reinterpret_cast<uintptr_t>(a->k_rope) |
        reinterpret_cast<uintptr_t>(a->out)) & 15)
     return FS_ERR_ALIGNMENT;
-  if (a->q_rows >= (1ll << 30) || a->k_rows >= (1ll << 30) || a->heads > (1 << 20) || a->batch > kPreMaxBatch)
-    return FS_ERR_UNSUPPORTED;
+  if (a->q_rows >= (1ll << 30) || a->k_rows >= (1ll << 30) || a->heads > (1 << 20)) return FS_ERR_UNSUPPORTED;
   const int64_t tiles = a->q_rows / (2 * kPreQ) + a->batch;  // at least as many as the requests have
   if (tiles * a->heads + a->q_rows / kClearRows + 1 >= (1ll << 31)) return FS_ERR_UNSUPPORTED;
   PrefillParams p{};

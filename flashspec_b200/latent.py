@@ -235,7 +235,7 @@ def latent_prefill_attention_cuda(q: torch.Tensor, kv: torch.Tensor, k_rope: tor
     k_offsets[b] : k_offsets[b + 1] (int64 [B + 1] on the device, ascending); its query i of nq
     sees keys j <= i + nk - nq, so a chunk of new tokens sees a cached prefix and, in order,
     itself; a query that sees no key gives zeros.  dn and dv 64 or 128, dr 32 or 64 (dr is read
-    from k_rope, dn from q); at most 4096 requests.  Returns out [Nq, H, dv]; a given ``out`` keeps the rows that no
+    from k_rope, dn from q).  Returns out [Nq, H, dv]; a given ``out`` keeps the rows that no
     request covers, otherwise those are zeros.  An infinite or undefined value reaches the
     queries that see its key and no others: infinities of one sign give infinity, else NaN.
     sm_scale defaults to 1 / sqrt(dn + dr)."""

@@ -297,13 +297,3 @@ def test_many_far_keys_beside_a_near_one_without_value(dtype, near):
     out = fs().latent_prefill_attention_cuda(q, kv, r, offsets([nq]), offsets([n]), sm_scale=1.0)
     err = (out.double() - want).abs()
     assert float(want.min()) > 1e-3 and bool((err <= bound).all()), float((err / bound).max())
-
-
-def test_the_largest_batch():
-    """4096 requests of zero to two tokens over short prefixes; one more is refused."""
-    n = [i % 3 for i in range(4096)]
-    check(n, [x + i % 5 for i, x in enumerate(n)], 2, 64, 32, 64, F, seed=18)
-    q, kv, r = make([5], [5], 1, 64, 32, 64, F, 19)
-    o = torch.zeros(4098, dtype=torch.int64, device="cuda")
-    with pytest.raises((RuntimeError, ValueError)):
-        fs().latent_prefill_attention_cuda(q, kv, r, o, o)

@@ -315,15 +315,3 @@ def test_every_arrival_of_a_prompt_is_waited_for():
         k_free = ([0] if tiles > 2 else []) + [j + 1 for j in range(tiles) if j + 3 < tiles]
         v_free = [j for j in range(tiles) if j + 2 < tiles]
         assert k_free == v_free == [j - 2 for j in range(2, tiles)]
-
-
-@pytest.mark.parametrize("batch", [4097, 1 << 20, (1 << 31) - 1])
-def test_latent_prefill_refuses_batches_whose_search_would_not_end(batch):
-    """Every CTA looks through all offsets: the time grows with the square of the batch."""
-    from flashspec_b200 import _lib
-
-    a = _lib.FsLatentPrefillArgs()
-    a.q = a.kv = a.k_rope = a.out = a.q_offsets = a.k_offsets = 4096
-    a.q_rows = a.k_rows = 10
-    a.batch, a.heads, a.nope_dim, a.rope_dim, a.value_dim = batch, 1, 128, 64, 128
-    assert _lib.load().fs_latent_prefill(C.byref(a), None) == 2
