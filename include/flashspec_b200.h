@@ -273,10 +273,11 @@ int fs_latent_attention(const FsLatentArgs* args, void* stream);
  *   q [q_rows, heads, nope_dim + rope_dim]   kv [k_rows, heads, nope_dim + value_dim] (the
  *   key's own part, then the value)   k_rope [k_rows, rope_dim]   out [q_rows, heads, value_dim]
  * all dtype FS_F16 or FS_BF16, contiguous, 16-byte aligned; offsets int64 [batch + 1] on the
- * device, ascending (offsets outside the rows are cut to them).  Rows of out that no request
- * covers are left as they were, or cleared with clear_rest.  nope_dim and value_dim 64 / 128, rope_dim 32 / 64; fewer
- * than 2^30 rows.  device_status receives FS_DEV_TIMEOUT where a bounded wait gave up (that
- * CTA's outputs are not written). */
+ * device, ascending (offsets outside the rows are cut to them; zeros behind the last request are
+ * empty requests, in batches of up to 4096).  Rows of out that no request covers are left as they
+ * were, or cleared with clear_rest.  out must not overlap the inputs.  nope_dim and value_dim
+ * 64 / 128, rope_dim 32 / 64; fewer than 2^30 rows.  device_status receives FS_DEV_TIMEOUT where
+ * a bounded wait gave up (that CTA's outputs are not written). */
 typedef struct FsLatentPrefillArgs {
   const void* q;
   const void* kv;

@@ -297,3 +297,42 @@ def test_many_far_keys_beside_a_near_one_without_value(dtype, near):
     out = fs().latent_prefill_attention_cuda(q, kv, r, offsets([nq]), offsets([n]), sm_scale=1.0)
     err = (out.double() - want).abs()
     assert float(want.min()) > 1e-3 and bool((err <= bound).all()), float((err / bound).max())
+
+
+@pytest.mark.parametrize("b", [33, 100, 1025, 5000])
+@pytest.mark.parametrize("longest", [3, 700])
+def test_large_batches(b, longest):
+    """Requests are searched for: none to several 256-query tiles each, empty ones in runs, prefixes,
+    and rows before the first and behind the last."""
+    g = torch.Generator().manual_seed(b)
+    total = 12000
+    n = torch.randint(0, longest + 1, (b,), generator=g)
+    n[torch.rand(b, generator=g) < 0.4] = 0
+    n = torch.where(torch.cumsum(n, 0) <= total, n, torch.zeros_like(n)).tolist()
+    nk = [x + (i % 4 if x else 0) for i, x in enumerate(n)]
+    front = 300
+    q, kv, r = make([sum(n)], [sum(nk)], 2, 64, 32, 64, F, 18, spare=front)
+    q[:front] = float("nan")
+    # expect() walks from row 0: give it the part that the requests cover
+    want, bound = expect(q[front:], kv, r, n, nk, 96 ** -0.5)
+    qo, ko = offsets(n) + front, offsets(nk)
+    got = fs().latent_prefill_attention_cuda(q, kv, r, qo, ko)
+    assert bool(((got[front:].double() - want).abs() <= bound).all()) and not bool(got[:front].any())
+    if b <= 4096:  # the same batch, padded with zeros behind its last request
+        pad = torch.zeros(b // 3 if b < 2000 else 500, dtype=torch.int64, device="cuda")
+        again = fs().latent_prefill_attention_cuda(q, kv, r, torch.cat([qo, pad]), torch.cat([ko, pad]))
+        assert torch.equal(again, got)
+
+
+def test_the_time_of_a_large_batch_is_linear():
+    """16384 requests of one token: dealt, they would take some seconds."""
+    n = [1] * 16384
+    q, kv, r = make(n, n, 16, 64, 32, 64, F, 19)
+    o = offsets(n)
+    fs().latent_prefill_attention_cuda(q[:40], kv[:40], r[:40], o[:41], o[:41])
+    a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    a.record()
+    out = fs().latent_prefill_attention_cuda(q, kv, r, o, o)
+    b.record()
+    torch.cuda.synchronize()
+    assert torch.equal(out, kv[..., 64:]) and a.elapsed_time(b) < 100
