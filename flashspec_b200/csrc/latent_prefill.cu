@@ -213,6 +213,7 @@ __device__ __forceinline__ void pre_clear(const PrefillParams& p, int chunk) {
 
 // OR of x over the two softmax groups; also orders their shared memory.
 __device__ __forceinline__ bool pre_any(bool x) {
+  __syncwarp();  // the barrier wants whole warps; loops before it may end lane by lane
   uint32_t r;
   asm volatile(
       "{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n bar.red.or.pred q, 1, 256, p;\n selp.b32 %0, 1, 0, q;\n}\n"
